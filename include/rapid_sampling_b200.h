@@ -31,7 +31,8 @@ enum {
     RS_ERR_CUDA = -7,        /* a CUDA runtime call failed; see rs_last_cuda_error()             */
     RS_ERR_TIMEOUT = -8,     /* device status: a bounded on-chip wait gave up                    */
     RS_ERR_LIMIT = -9,       /* size beyond what this entry point supports                       */
-    RS_ERR_INTERNAL = -10    /* device status: an invariant of the cutoff search was violated    */
+    RS_ERR_INTERNAL = -10,   /* device status: an invariant of the cutoff search was violated    */
+    RS_ERR_TOKEN = -11       /* device status: a token id is no column of the logits             */
 };
 
 /* Bytes per row of the RNG state tensor: layout-compatible with curandStatePhilox4_32_10_t
@@ -231,6 +232,57 @@ int rs_vp_stage(const rs_vp_call* call, int32_t stage, int32_t round);
  */
 int rs_vp_tile_begin(const rs_vp_call* call);
 int rs_vp_tile_max(const rs_vp_call* call, const float* tile_device, int64_t ld, int64_t col_begin, int64_t ncols);
+
+/*
+ * Log probabilities of given tokens.  No counterpart in the reference, which returns ids only.
+ *
+ * A call describes B * T rows of V logits: row (b, t) starts at logits + b * stride_b + t * stride_t (elements; any
+ * element-aligned address, V of any size up to RS_LOGPROB_MAX_V, stride 0 repeats a row), its token is
+ * tokens[b * token_stride_b + t * token_stride_t] (token_bits 32 or 64), its temperature likewise where row_temperature
+ * (float32) is not NULL, else `temperature`.  With z = logits / temperature:
+ *   log probability  z_token - logsumexp(z)
+ *   entropy          of softmax(z), in nats
+ * A negative token marks a position that is not scored: its logits are not read, log probability and entropy are 0, the
+ * gradient is 0.  Unlike the samplers, which always have to name a token, these calls do not replace what is not finite:
+ *   -inf             a masked token: probability 0
+ *   nothing but -inf log probability -inf, entropy 0, gradient 0
+ *   NaN or +inf      the row's results are NaN
+ * A token >= V: the row's results are NaN, its gradient 0, and the status word becomes RS_ERR_TOKEN; a row temperature
+ * outside [0.001, 1000]: the row runs at 1 and the status word becomes RS_ERR_TEMPERATURE (rs_logprobs_status, and the host
+ * mirror of rs_set_status_mirror).  The calls need no workspace and allocate nothing.
+ */
+#define RS_LOGPROB_MAX_V 1048576
+#define RS_LOGPROB_MAX_TOP 64
+typedef struct rs_logprob_call {
+    const void* logits;             /* device */
+    const void* tokens;             /* device */
+    const float* row_temperature;   /* device, or NULL */
+    void* stream;                   /* cudaStream_t */
+    int64_t B, T, V, stride_b, stride_t;
+    int64_t token_stride_b, token_stride_t, temperature_stride_b, temperature_stride_t;
+    double temperature;
+    int32_t dtype, token_bits;
+} rs_logprob_call;
+
+/* logprob, entropy: B * T floats.  stats (B * T pairs of floats, 8-byte aligned, or NULL): what the backward call needs. */
+int rs_token_logprobs(const rs_logprob_call* call, float* logprob_device, float* entropy_device, float* stats_device);
+
+/* The gradient of  sum grad_logprob * logprob + grad_entropy * entropy  with respect to the logits, in their type, to
+ * grad_device, (B, T, V) contiguous; entropy and stats are those that rs_token_logprobs wrote for the same call.  Either
+ * incoming gradient may be NULL (zero); each has strides of its own, 0 for a broadcast one. */
+int rs_token_logprobs_backward(const rs_logprob_call* call, const float* entropy_device, const float* stats_device,
+                               const float* grad_logprob_device, int64_t gl_stride_b, int64_t gl_stride_t,
+                               const float* grad_entropy_device, int64_t ge_stride_b, int64_t ge_stride_t, void* grad_device);
+
+/* The same statistics with the token's rank and the top_n (1 .. RS_LOGPROB_MAX_TOP) most probable tokens.
+ * rank = 1 + the number of larger logits + the number of equal ones at a lower index; the list is in that order.  Slots
+ * behind the last token that the mask leaves hold -inf and id -1; a row that is not scored has nothing but such slots and
+ * rank 0, one with NaN or +inf NaN, -1 and rank 0.  call->tokens may be NULL if logprob and rank are. */
+int rs_top_logprobs(const rs_logprob_call* call, int32_t top_n, float* logprob_device, int32_t* rank_device, float* entropy_device,
+                    float* top_device, int32_t* top_ids_device);
+
+/* Reads and clears the current device's status word of the three calls above (synchronises `stream`). */
+int rs_logprobs_status(void* stream);
 
 /*
  * Device status word.  The kernels never trap: a condition they cannot report through a return code is written to

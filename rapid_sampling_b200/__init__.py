@@ -67,6 +67,33 @@ def batch_sampling_rows(logits, states, temperature=None, top_k=None, top_p=None
                                            repetition_penalty, penalty_decay, return_prob)
 
 
+def batch_token_logprobs(logits, tokens, temperature=1.0):
+    """Log probability of one given token per row, and the row's entropy, under softmax(logits / temperature): float32
+    tensors of the tokens' shape.  Differentiable with respect to the logits (both results, first order).
+
+    logits: float32, float16 or bfloat16, (V,), (B, V) or (B, T, V), every position a row; any strides but along V, and any
+    V up to 1048576.  tokens: int32 or int64, the logits' shape without V.  temperature: a number, or a float32 CUDA tensor
+    of one value, one per row, or one per sequence; not differentiated.
+
+    A negative token marks a position that is not scored (padding): 0, 0 and no gradient, and its logits are not read.
+    Unlike the sampling calls, nothing is replaced: -inf masks a token; a row of nothing but -inf has log probability -inf,
+    entropy 0 and gradient 0; NaN or +inf makes its row NaN.  A token >= V gives NaN and no gradient, a temperature outside
+    [0.001, 1000] in a tensor counts as 1, and either raises ValueError from the next call on the device."""
+    from . import logprobs
+    return logprobs.token_logprobs(logits, tokens, temperature)
+
+
+def batch_top_logprobs(logits, top_n, tokens=None, temperature=1.0):
+    """(log probabilities, ranks, entropies, top log probabilities, top ids): what `batch_token_logprobs` computes, the
+    tokens' ranks, and the `top_n` (at most 64) most probable tokens of every row in falling order, equal logits by rising
+    id.  A token's rank (int32, from 1) is its place in that order.  Without tokens the first two are None.
+
+    Slots behind the last token that a mask of -inf leaves hold -inf and id -1; so do all slots of a position that is not
+    scored (negative token; rank 0).  Rows with NaN or +inf: NaN, id -1, rank 0.  Not differentiable."""
+    from . import logprobs
+    return logprobs.top_logprobs(logits, top_n, tokens, temperature)
+
+
 def kernel_launch_count():
     return _load_ext().kernel_launch_count()
 
@@ -85,4 +112,4 @@ def release_workspaces():
 
 __all__ = ["setup_rand", "batch_sampling_temperature_topk_topp", "batch_sampling_repetition_temperature_topk_topp",
            "batch_sampling_temperature_topk_topp_any", "batch_sampling_repetition_temperature_topk_topp_any", "batch_sampling_rows",
-           "kernel_launch_count", "device_status", "release_workspaces"]
+           "batch_token_logprobs", "batch_top_logprobs", "kernel_launch_count", "device_status", "release_workspaces"]

@@ -38,8 +38,8 @@ def _run(cmd, verbose):
         print(r.stdout)
 
 
-CU_SOURCES = ["rs_sampler.cu", "rs_rowcta.cu", "rs_vocab_parallel.cu"]
-HEADERS = [os.path.join(CSRC, h) for h in ("rs_device.cuh", "rs_common.cuh", "rs_rowcta.cuh")] + \
+CU_SOURCES = ["rs_sampler.cu", "rs_rowcta.cu", "rs_vocab_parallel.cu", "rs_logprobs.cu"]
+HEADERS = [os.path.join(CSRC, h) for h in ("rs_device.cuh", "rs_common.cuh", "rs_rowcta.cuh", "rs_host.cuh")] + \
     [os.path.join(INCLUDE, "rapid_sampling_b200.h")]
 OBJ_DIR = os.path.join(HERE, "build")
 

@@ -13,13 +13,15 @@ RS_OK = 0
 RS_ERR_DTYPE, RS_ERR_VOCAB, RS_ERR_BATCH, RS_ERR_TEMPERATURE = -1, -2, -3, -4
 RS_ERR_POINTER, RS_ERR_WORKSPACE, RS_ERR_CUDA, RS_ERR_TIMEOUT, RS_ERR_LIMIT = -5, -6, -7, -8, -9
 RS_ERR_INTERNAL = -10
+RS_ERR_TOKEN = -11
+RS_LOGPROB_MAX_V, RS_LOGPROB_MAX_TOP = 1048576, 64
 RS_STATE_BYTES = 64
 RS_DTYPE_F32, RS_DTYPE_F16, RS_DTYPE_BF16 = 0, 1, 2
 RS_STATIC_SCRATCH_FLOATS = 4194304
 
 SYMBOLS = ["rs_setup_rand", "rs_workspace_bytes", "rs_sample", "rs_sample_debug", "rs_sample_host", "rs_sample_typed", "rs_sample_static_scratch", "rs_rows_workspace_bytes", "rs_sample_rows",
            "rs_device_status", "rs_clear_status", "rs_set_status_mirror", "rs_set_wait_polls", "rs_set_dependent_launch", "rs_selftest_bounded_wait", "rs_set_cluster_override", "rs_set_path_override", "rs_kernel_launch_count", "rs_vp_workspace_bytes", "rs_vp_layout", "rs_vp_fast_layout", "rs_vp_stage", "rs_vp_tile_begin", "rs_vp_tile_max", "rs_status_string",
-           "rs_last_cuda_error", "rs_version"]
+           "rs_last_cuda_error", "rs_version", "rs_token_logprobs", "rs_token_logprobs_backward", "rs_top_logprobs", "rs_logprobs_status"]
 
 
 class Trace(C.Structure):
@@ -35,6 +37,13 @@ class VpCall(C.Structure):
                 ("V_global", C.c_int64), ("col0", C.c_int64), ("top_k", C.c_int64), ("temperature", C.c_double),
                 ("top_p", C.c_double), ("presence_penalty", C.c_double), ("repetition_penalty", C.c_double),
                 ("penalty_decay", C.c_double), ("rank", C.c_int32), ("world", C.c_int32)]
+
+
+class LogprobCall(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("tokens", C.c_void_p), ("row_temperature", C.c_void_p), ("stream", C.c_void_p)] + \
+               [(n, C.c_int64) for n in ("B", "T", "V", "stride_b", "stride_t", "token_stride_b", "token_stride_t",
+                                         "temperature_stride_b", "temperature_stride_t")] + \
+               [("temperature", C.c_double), ("dtype", C.c_int32), ("token_bits", C.c_int32)]
 
 
 VP_MAX, VP_SUM, VP_ROUND, VP_TALLY, VP_WEIGHT, VP_PICK, VP_PENALTY = range(7)
@@ -73,6 +82,11 @@ def load():
     L.rs_vp_stage.argtypes = [C.POINTER(VpCall), C.c_int32, C.c_int32]
     L.rs_vp_tile_begin.argtypes = [C.POINTER(VpCall)]
     L.rs_vp_tile_max.argtypes = [C.POINTER(VpCall), vp, i64, i64, i64]
+    lp = C.POINTER(LogprobCall)
+    L.rs_token_logprobs.argtypes = [lp, vp, vp, vp]
+    L.rs_token_logprobs_backward.argtypes = [lp, vp, vp, vp, i64, i64, vp, i64, i64, vp]
+    L.rs_top_logprobs.argtypes = [lp, C.c_int32, vp, vp, vp, vp, vp]
+    L.rs_logprobs_status.argtypes = [vp]
     L.rs_device_status.argtypes = [vp, vp]
     L.rs_clear_status.argtypes = [vp, vp]
     L.rs_set_status_mirror.argtypes = [vp]

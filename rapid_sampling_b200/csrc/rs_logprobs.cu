@@ -1,0 +1,808 @@
+// Log probabilities of given tokens, their entropy, rank and alternatives, and the gradient with respect to the logits.
+// sm_100a only.
+//
+// With z = x / T, m = max z, s = sum exp(z - m):
+//     log p_t = z_t - m - ln s          H = ln s - sum (z - m) exp(z - m) / s
+//     d/dx_j (g log p_t + h H) = 1/T (g [j = t] - p_j (g + h (ln p_j + H)))
+// A row is read once: every thread keeps the maximum it has seen, and the two sums relative to it.  Maxima are compared on
+// the logits as they are; exponents are taken as ((x - m) log2(e)/T) so that neither masks of the type's lowest value nor a
+// row made of nothing else overflow.  Sums are held without the maximum's own 1 ("excess", s - 1) from the thread level up:
+// log p of a token of probability nearly one is -log1p(excess), which keeps its digits.
+#include "rs_device.cuh"
+#include "rs_host.cuh"
+#include "../../include/rapid_sampling_b200.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstring>
+#include <mutex>
+#include <type_traits>
+
+namespace rs {
+
+constexpr int kLpThreads = 256;
+constexpr int kLpAhead = 4;            // 16-byte loads in flight per thread
+constexpr int kTopMax = 64;            // longest list of alternatives
+constexpr int kTopCap = 1024;          // candidates for a list, per CTA
+constexpr int kTopHot = 128;           // threads whose logits are looked at again
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFloor = -160.f;       // exponent from which on exp2f is zero; keeps 0 * inf out of the second sum
+
+__device__ int g_lp_status;            // status word of these calls on this device (rs_logprobs_status)
+
+struct LpParams {
+    const void* logits;
+    long long sb, st;                  // elements between sequences, between positions
+    long long rows;                    // B * T
+    int T, V;
+    const void* tokens;                // int32 or int64, or null
+    int wide_tokens;
+    long long tok_sb, tok_st;
+    float temperature;
+    const float* row_temperature;      // or null
+    long long tmp_sb, tmp_st;
+    float *logprob, *entropy;          // rows
+    float2* stats;                     // rows: largest logit, log2 of the sum
+    int* rank;                         // rows
+    float* top;                        // rows * top_n
+    int* top_ids;
+    int top_n;
+    int* mirror;
+    // backward
+    const float *g_logprob, *g_entropy;
+    long long gl_sb, gl_st, ge_sb, ge_st;
+    void* grad;                        // (rows, V) contiguous
+    int chunks;                        // CTAs per row
+};
+
+// ---- elements -----------------------------------------------------------------------------------------------------
+template <int DT> struct Elem;
+template <> struct Elem<RS_DTYPE_F32> {
+    using T = float;
+    static constexpr int E = 4;
+    static constexpr uint32_t kNone = 0xFF800000u;      // a word of -inf
+    static __device__ __forceinline__ void wide(const uint4& v, float (&x)[4]) {
+        x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ float one(const T* p) { return *p; }
+    static __device__ __forceinline__ uint4 narrow(const float (&x)[4]) {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    }
+    static __device__ __forceinline__ T to(float x) { return x; }
+};
+template <> struct Elem<RS_DTYPE_F16> {
+    using T = __half;
+    static constexpr int E = 8;
+    static constexpr uint32_t kNone = 0xFC00FC00u;
+    static __device__ __forceinline__ void wide(const uint4& v, float (&x)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ float one(const T* p) { return __half2float(*p); }
+    static __device__ __forceinline__ uint4 narrow(const float (&x)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ T to(float x) { return __float2half_rn(x); }
+};
+template <> struct Elem<RS_DTYPE_BF16> {
+    using T = __nv_bfloat16;
+    static constexpr int E = 8;
+    static constexpr uint32_t kNone = 0xFF80FF80u;
+    static __device__ __forceinline__ void wide(const uint4& v, float (&x)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+    static __device__ __forceinline__ float one(const T* p) { return __bfloat162float(*p); }
+    static __device__ __forceinline__ uint4 narrow(const float (&x)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ T to(float x) { return __float2bfloat16_rn(x); }
+};
+
+__device__ __forceinline__ uint4 ld_stream(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {      // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float warp_max_nan(float v) {
+    float r;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// Order of floats as unsigned integers, -0 equal to +0; NaN above everything or below, which no caller relies on.
+__device__ __forceinline__ uint32_t key_of(float x) {
+    const uint32_t u = __float_as_uint(x + 0.0f);
+    return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float of_key(uint32_t k) {
+    return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+constexpr uint32_t kKeyNone = 0x007FFFFFu;      // key of -inf
+
+// ---- one row's position, token and temperature --------------------------------------------------------------------
+struct LpRow {
+    long long b, t, token;      // token: < 0 where the position is not scored
+    float inv_t, c;             // 1 / T, log2(e) / T
+    bool bad_token, bad_temperature;
+};
+__device__ __forceinline__ LpRow lp_row(const LpParams& p, long long r) {
+    LpRow o;
+    o.b = r / p.T;
+    o.t = r - o.b * p.T;
+    o.token = 0;
+    if (p.tokens) {
+        const long long at = o.b * p.tok_sb + o.t * p.tok_st;
+        o.token = p.wide_tokens ? ((const long long*)p.tokens)[at] : (long long)((const int*)p.tokens)[at];
+    }
+    o.bad_token = o.token >= p.V;
+    float t = p.row_temperature ? p.row_temperature[o.b * p.tmp_sb + o.t * p.tmp_st] : p.temperature;
+    o.bad_temperature = !(t >= 0.001f && t <= 1000.f);
+    if (o.bad_temperature) t = 1.f;
+    o.inv_t = __fdiv_rn(1.f, t);
+    o.c = __fdiv_rn(kLog2e, t);
+    return o;
+}
+__device__ __forceinline__ void lp_report(const LpParams& p, int code) {
+    atomicExch(&g_lp_status, code);
+    if (p.mirror) *reinterpret_cast<volatile int*>(p.mirror) = code;
+}
+
+// ---- running statistics -------------------------------------------------------------------------------------------
+struct Stat {
+    float mx;      // largest logit seen (NaN if any is); -inf: none but -inf
+    float s, u;    // sums of e and of e (x - m) c with e = exp2((x - m) c), m = max(mx, -FLT_MAX)
+};
+__device__ __forceinline__ float ref_of(float mx) { return max_nan(mx, -FLT_MAX); }
+__device__ __forceinline__ void stat_raise(Stat& a, float bm, float c) {
+    const float m0 = ref_of(a.mx);
+    a.mx = max_nan(a.mx, bm);
+    const float d = fmaxf((m0 - ref_of(a.mx)) * c, kFloor), f = ex2(d);
+    a.u = f * fmaf(d, a.s, a.u);
+    a.s *= f;
+}
+template <int N>
+__device__ __forceinline__ void stat_add(Stat& a, const float (&x)[N], float c) {
+    float bm = x[0];
+#pragma unroll
+    for (int i = 1; i < N; i++) bm = max_nan(bm, x[i]);
+    stat_raise(a, bm, c);
+    const float m = ref_of(a.mx);
+    float s = 0.f, u = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const float d = fmaxf((x[i] - m) * c, kFloor), e = ex2(d);
+        s += e;
+        u = fmaf(d, e, u);
+    }
+    a.s += s;
+    a.u += u;
+}
+// The lanes' statistics as one, in every lane.  s comes and goes as the excess: the sum without the maximum's own 1 (-1: no
+// element above -inf).  Terms are added in a fixed order.
+__device__ __forceinline__ Stat stat_warp(Stat a, float c) {
+    Stat r;
+    r.mx = warp_max_nan(a.mx);
+    const float d = fmaxf((ref_of(a.mx) - ref_of(r.mx)) * c, kFloor), f = ex2(d), w = 1.f + a.s;
+    const int owner = __ffs(__ballot_sync(0xffffffffu, a.mx == r.mx)) - 1;
+    r.s = (int)(threadIdx.x & 31) == owner ? a.s : f * w;
+    r.u = f * fmaf(d, w, a.u);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+        r.u += __shfl_xor_sync(0xffffffffu, r.u, o);
+    }
+    return r;
+}
+
+// ---- the part of a row that a CTA reads ----------------------------------------------------------------------------
+// Elements up to the first 16-byte boundary and behind the last whole vector are single ones, taken by the first and the
+// last CTA of the row; the vectors between are split evenly.  Vector v of the CTA belongs to thread v % kLpThreads.
+template <int DT>
+struct Span {
+    using T = typename Elem<DT>::T;
+    const T* row;
+    const uint4* vec;
+    int head, nvec, V;       // of the row
+    int v0, v1;              // this CTA's vectors
+    bool first, last;
+    __device__ __forceinline__ Span(const LpParams& p, const LpRow& w, int part, int parts) {
+        constexpr int E = Elem<DT>::E;
+        row = (const T*)p.logits + w.b * p.sb + w.t * p.st;
+        V = p.V;
+        head = (int)((16u - ((uint32_t)(uintptr_t)row & 15u)) & 15u) / (int)sizeof(T);
+        if (head > V) head = V;
+        nvec = (V - head) / E;
+        vec = reinterpret_cast<const uint4*>(row + head);
+        v0 = (int)((long long)nvec * part / parts);
+        v1 = (int)((long long)nvec * (part + 1) / parts);
+        first = part == 0;
+        last = part == parts - 1;
+    }
+    __device__ __forceinline__ int tail() const { return head + nvec * Elem<DT>::E; }      // index of the first element behind
+    __device__ __forceinline__ int index(int v) const { return head + v * Elem<DT>::E; }
+    // calls f(index, value) for the single elements of thread h
+    template <class F> __device__ __forceinline__ void singles(int h, F&& f) const {
+        if (first && h < head) f(h, Elem<DT>::one(row + h));
+        const int j = tail() + h;
+        if (last && h < Elem<DT>::E && j < V) f(j, Elem<DT>::one(row + j));
+    }
+};
+
+// ---- statistics, rank and alternatives of rows ---------------------------------------------------------------------
+struct LpShared {
+    float mx[16], s[16], u[16];       // warps of the CTA (8), then CTAs of the cluster (16)
+    int cnt[16];
+    float r_mx, r_logs, r_inv_t;
+    float c_mx[16], c_s[16], c_u[16];
+    int c_cnt[16];
+};
+struct TopShared {
+    uint32_t key[kLpThreads];
+    unsigned long long cand[kTopCap];
+    unsigned long long list[16 * kTopMax];     // the cluster's lists, in the first CTA
+    int list_n[16];
+    short hot[kTopHot];
+    int nhot, nfinite, ncand, count;
+    uint32_t tau;
+};
+
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) { st_cluster_u32(addr, __float_as_uint(v)); }
+__device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+
+__device__ __forceinline__ void top_push(TopShared& sh, uint32_t key, int j) {
+    const int at = atomicAdd(&sh.ncand, 1);
+    if (at < kTopCap) sh.cand[at] = ((unsigned long long)key << 32) | (uint32_t)~j;
+}
+// Elements of the CTA's part with a key of at least `at_least`.
+template <int DT>
+__device__ int top_count(const Span<DT>& sp, TopShared& sh, uint32_t at_least) {
+    constexpr int E = Elem<DT>::E;
+    __syncthreads();
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    int n = 0;
+    for (int v = sp.v0 + (int)threadIdx.x; v < sp.v1; v += kLpThreads) {
+        float x[E];
+        Elem<DT>::wide(ld_stream(sp.vec + v), x);
+#pragma unroll
+        for (int i = 0; i < E; i++) n += key_of(x[i]) >= at_least;
+    }
+    sp.singles(threadIdx.x, [&](int, float x) { n += key_of(x) >= at_least; });
+    atomicAdd(&sh.count, n);
+    __syncthreads();
+    return sh.count;
+}
+// The n-th largest key is bisected, what lies above it collected, and the rest filled up with elements equal to it in the
+// order of their indices.  For parts whose n largest elements are not told apart by the threads' maxima: long runs of equal
+// logits, or large ones that crowd in few threads.  About 32 passes over the part at worst, 2 where the threads' n-th
+// largest maximum is the key, as with a mask of the type's lowest value.
+template <int DT>
+__device__ void top_exact(const Span<DT>& sp, TopShared& sh, int n) {
+    constexpr int E = Elem<DT>::E;
+    const int t = threadIdx.x;
+    uint32_t lo = sh.tau, hi = 0xFF800001u;        // count(lo) >= n > count(hi): nothing lies above +inf's key
+    for (uint32_t mid = lo + 1; hi - lo > 1; mid = lo + (hi - lo) / 2) {
+        if (top_count(sp, sh, mid) >= n) lo = mid; else hi = mid;
+    }
+    __syncthreads();
+    if (t == 0) sh.ncand = 0;
+    __syncthreads();
+    for (int v = sp.v0 + t; v < sp.v1; v += kLpThreads) {
+        float x[E];
+        Elem<DT>::wide(ld_stream(sp.vec + v), x);
+#pragma unroll
+        for (int i = 0; i < E; i++)
+            if (key_of(x[i]) > lo) top_push(sh, key_of(x[i]), sp.index(v) + i);
+    }
+    sp.singles(t, [&](int j, float x) { if (key_of(x) > lo) top_push(sh, key_of(x), j); });
+    __syncthreads();
+    if (sp.first) {
+        if (t < sp.head && key_of(Elem<DT>::one(sp.row + t)) == lo) top_push(sh, lo, t);
+        __syncthreads();
+    }
+    constexpr int kStep = 64;                      // vectors at a time: at most 512 entries more than the list needs
+    for (int v = sp.v0; v < sp.v1; v += kStep) {
+        const int have = sh.ncand;
+        __syncthreads();
+        if (have >= n) break;
+        if (t < kStep && v + t < sp.v1) {
+            float x[E];
+            Elem<DT>::wide(ld_stream(sp.vec + v + t), x);
+#pragma unroll
+            for (int i = 0; i < E; i++)
+                if (key_of(x[i]) == lo) top_push(sh, lo, sp.index(v + t) + i);
+        }
+        __syncthreads();
+    }
+    if (sp.last && sh.ncand < n) {
+        const int j = sp.tail() + t;
+        __syncthreads();
+        if (t < E && j < sp.V && key_of(Elem<DT>::one(sp.row + j)) == lo) top_push(sh, lo, j);
+    }
+    __syncthreads();
+}
+// The n largest elements of the CTA's part (larger key first, then lower index), unordered, among sh.cand[0 .. result).
+// At least n of the threads have a maximum that reaches the n-th largest maximum, so the list lies within the elements that
+// reach it too, and those are in the few threads whose maximum does: only their elements are read again.
+template <int DT>
+__device__ int top_collect(const Span<DT>& sp, TopShared& sh, float mx, int n) {
+    constexpr int E = Elem<DT>::E;
+    const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+    const uint32_t mine = key_of(mx);
+    sh.key[t] = mine;
+    if (t == 0) { sh.nhot = 0; sh.ncand = 0; sh.tau = kKeyNone + 1; }
+    const int finite = __syncthreads_count(mine > kKeyNone);
+    if (finite >= n) {
+        int above = 0, reach = 0;
+#pragma unroll 8
+        for (int i = 0; i < kLpThreads / 4; i++) {
+            const uint4 k = reinterpret_cast<const uint4*>(sh.key)[i];
+            above += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
+            reach += (k.x >= mine) + (k.y >= mine) + (k.z >= mine) + (k.w >= mine);
+        }
+        if (above < n && n <= reach) sh.tau = mine;       // the same value from every thread that writes
+        __syncthreads();
+    }
+    const uint32_t tau = sh.tau;
+    if (mine >= tau) {
+        const int at = atomicAdd(&sh.nhot, 1);
+        if (at < kTopHot) sh.hot[at] = (short)t;
+    }
+    __syncthreads();
+    const int nhot = sh.nhot;
+    if (nhot <= kTopHot) {
+        for (int i = w; i < nhot; i += kLpThreads / 32) {
+            const int h = sh.hot[i];
+            for (int v = sp.v0 + h + lane * kLpThreads; v < sp.v1; v += 32 * kLpThreads) {
+                float x[E];
+                Elem<DT>::wide(ld_stream(sp.vec + v), x);
+#pragma unroll
+                for (int k = 0; k < E; k++)
+                    if (key_of(x[k]) >= tau) top_push(sh, key_of(x[k]), sp.index(v) + k);
+            }
+            if (lane == 0) sp.singles(h, [&](int j, float x) { if (key_of(x) >= tau) top_push(sh, key_of(x), j); });
+        }
+        __syncthreads();
+    }
+    if (nhot > kTopHot || sh.ncand > kTopCap) top_exact(sp, sh, n);
+    return min(sh.ncand, kTopCap);      // (a row with NaN may offer more; its list is not used)
+}
+
+// One cluster of gridDim.x / rows CTAs per row (one CTA: no cluster).  Bound by HBM for many rows, by latency for few.
+template <int DT, bool TOP>
+__global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_constant__ LpParams p, int parts) {
+    constexpr int E = Elem<DT>::E;
+    __shared__ LpShared sh;
+    __shared__ typename std::conditional<TOP, TopShared, int>::type top;
+    const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+    const int part = parts > 1 ? (int)cluster_ctarank() : 0;
+    const long long r = parts > 1 ? (long long)blockIdx.x / parts : (long long)blockIdx.x;
+    const LpRow row = lp_row(p, r);
+    if (row.token < 0 || row.bad_token) {         // not scored: the same for the whole cluster
+        if (part == 0) {
+            const float v = row.bad_token ? __int_as_float(0x7FC00000) : 0.f;
+            if (t == 0) {
+                if (row.bad_token) lp_report(p, RS_ERR_TOKEN);
+                if (p.logprob) p.logprob[r] = v;
+                if (p.entropy) p.entropy[r] = v;
+                if (p.stats) p.stats[r] = make_float2(0.f, 0.f);
+                if (p.rank) p.rank[r] = 0;
+            }
+            if (TOP && t < p.top_n) {
+                p.top[r * p.top_n + t] = row.bad_token ? v : -INFINITY;
+                p.top_ids[r * p.top_n + t] = -1;
+            }
+        }
+        return;
+    }
+    if (parts > 1) cluster_arrive();
+    const float c = row.c;
+    const Span<DT> sp(p, row, part, parts);
+    const int token = (int)row.token;
+    const float xt = Elem<DT>::one(sp.row + token);
+    // rank: an element before the token counts from xt on, one behind it only above
+    const uint32_t kt = key_of(xt);
+    const float xt_above = of_key(kt + 1);
+    int cnt = 0;
+
+    Stat a = {-INFINITY, 0.f, 0.f};
+    sp.singles(t, [&](int j, float x) {
+        const float one[1] = {x};
+        stat_add(a, one, c);
+        if (TOP) cnt += j < token ? x >= xt : x > xt;
+    });
+    for (int v = sp.v0 + t; v < sp.v1; v += kLpAhead * kLpThreads) {
+        uint4 raw[kLpAhead];
+#pragma unroll
+        for (int i = 0; i < kLpAhead; i++) {
+            const int at = v + i * kLpThreads;
+            raw[i] = at < sp.v1 ? ld_stream(sp.vec + at) : make_uint4(Elem<DT>::kNone, Elem<DT>::kNone, Elem<DT>::kNone, Elem<DT>::kNone);
+        }
+        float x[kLpAhead * E];
+#pragma unroll
+        for (int i = 0; i < kLpAhead; i++) {
+            float y[E];
+            Elem<DT>::wide(raw[i], y);
+#pragma unroll
+            for (int k = 0; k < E; k++) x[i * E + k] = y[k];
+            if (TOP) {
+                const float from = sp.index(v + i * kLpThreads) < token ? xt : xt_above;
+#pragma unroll
+                for (int k = 0; k < E; k++) cnt += y[k] >= from;
+            }
+        }
+        stat_add(a, x, c);
+    }
+    const float my_mx = a.mx;
+    a.s -= 1.f;
+    a = stat_warp(a, c);
+    if (TOP) cnt = (int)warp_sum_u32((uint32_t)cnt);
+    if (lane == 0) {
+        sh.mx[w] = a.mx; sh.s[w] = a.s; sh.u[w] = a.u;
+        if (TOP) sh.cnt[w] = cnt;
+    }
+    __syncthreads();
+    if (parts > 1) cluster_wait();                // every CTA of the cluster runs: its shared memory may be written
+    if (w == 0) {
+        Stat b = {-INFINITY, -1.f, 0.f};
+        if (lane < kLpThreads / 32) b = {sh.mx[lane], sh.s[lane], sh.u[lane]};
+        b = stat_warp(b, c);
+        int n = TOP ? (int)warp_sum_u32(lane < kLpThreads / 32 ? (uint32_t)sh.cnt[lane] : 0u) : 0;
+        if (parts > 1) {
+            if (lane == 0) {
+                st_cluster_f32(map_to_cta(smem_addr(&sh.c_mx[part]), 0), b.mx);
+                st_cluster_f32(map_to_cta(smem_addr(&sh.c_s[part]), 0), b.s);
+                st_cluster_f32(map_to_cta(smem_addr(&sh.c_u[part]), 0), b.u);
+                if (TOP) st_cluster_u32(map_to_cta(smem_addr(&sh.c_cnt[part]), 0), (uint32_t)n);
+            }
+        } else if (lane == 0) {
+            sh.c_mx[0] = b.mx; sh.c_s[0] = b.s; sh.c_u[0] = b.u;
+            if (TOP) sh.c_cnt[0] = n;
+        }
+    }
+    if constexpr (TOP) {
+        const int n = p.top_n;
+        const int nc = top_collect(sp, top, my_mx, n);
+        for (int i = t; i < nc; i += kLpThreads) {
+            const unsigned long long e = top.cand[i];
+            int at = 0;
+            for (int q = 0; q < nc; q++) at += top.cand[q] > e;
+            if (at < n) st_cluster_u64(map_to_cta(smem_addr(&top.list[part * kTopMax + at]), 0), e);
+        }
+        if (t == 0) st_cluster_u32(map_to_cta(smem_addr(&top.list_n[part]), 0), (uint32_t)min(nc, n));
+    }
+    if (parts > 1) {
+        cluster_arrive();
+        cluster_wait();
+        if (part) return;
+    } else {
+        __syncthreads();
+    }
+    // the first CTA has everything
+    if (w == 0) {
+        Stat b = {-INFINITY, -1.f, 0.f};
+        if (lane < parts) b = {sh.c_mx[lane], sh.c_s[lane], sh.c_u[lane]};
+        b = stat_warp(b, c);
+        int above = TOP ? (int)warp_sum_u32(lane < parts ? (uint32_t)sh.c_cnt[lane] : 0u) : 0;
+        if (lane == 0) {
+            const bool bad = !(b.mx < INFINITY), none = b.mx == -INFINITY;
+            const float nan = __int_as_float(0x7FC00000);
+            const float logs = log1pf(b.s);
+            const float lp = bad ? nan : none ? -INFINITY : (xt - b.mx) * row.inv_t - logs;
+            const float ent = bad ? nan : none ? 0.f : logs - b.u / (1.f + b.s) * 0.6931471805599453f;
+            if (p.logprob) p.logprob[r] = lp;
+            if (p.entropy) p.entropy[r] = ent;
+            if (p.stats) p.stats[r] = make_float2(b.mx, logs * kLog2e);
+            if (row.bad_temperature) lp_report(p, RS_ERR_TEMPERATURE);
+            if (TOP) {
+                if (p.rank) {
+                    // the token's own vector was counted from xt on if it begins before the token
+                    const int v = (token - sp.head) / E, j0 = sp.index(v);
+                    if (token >= sp.head && v < sp.nvec && j0 < token)
+                        for (int j = token; j < j0 + E; j++) above -= Elem<DT>::one(sp.row + j) == xt;
+                    p.rank[r] = bad ? 0 : above + 1;
+                }
+                sh.r_mx = b.mx;
+                sh.r_logs = logs;
+            }
+        }
+    }
+    if constexpr (TOP) {
+        __syncthreads();
+        const int n = p.top_n;
+        const float mx = sh.r_mx, logs = sh.r_logs;
+        const bool bad = !(mx < INFINITY);
+        int total = 0;
+        for (int q = 0; q < parts; q++) total += top.list_n[q];
+        for (int i = t; i < parts * n; i += kLpThreads) {
+            const int q = i / n, k = i - q * n;
+            if (k >= top.list_n[q]) continue;
+            const unsigned long long e = top.list[q * kTopMax + k];
+            int at = k;                                   // the lists are in order: larger ones of its own come before
+            for (int o = 0; o < parts; o++)
+                if (o != q)
+                    for (int z = 0, zn = top.list_n[o]; z < zn && top.list[o * kTopMax + z] > e; z++) at++;
+            if (at < n && !bad) {
+                p.top[r * n + at] = (of_key((uint32_t)(e >> 32)) - mx) * row.inv_t - logs;
+                p.top_ids[r * n + at] = (int)~(uint32_t)e;
+            }
+        }
+        if (t < n && (bad || t >= total)) {
+            p.top[r * n + t] = bad ? __int_as_float(0x7FC00000) : -INFINITY;
+            p.top_ids[r * n + t] = -1;
+        }
+    }
+}
+
+// ---- gradient -------------------------------------------------------------------------------------------------------
+// One element per step of arithmetic: with d = (x - m) c - log2 s, p = 2^d:  p (A + D d), plus g/T at the token itself,
+// where the two are taken together as -expm1(log p) so that a token of probability nearly one keeps its digits.
+template <int DT>
+__global__ void __launch_bounds__(kLpThreads, 4) lp_backward_kernel(const __grid_constant__ LpParams p) {
+    constexpr int E = Elem<DT>::E;
+    using T = typename Elem<DT>::T;
+    const long long r = blockIdx.x / (unsigned)p.chunks;
+    const int part = (int)(blockIdx.x - r * p.chunks), t = threadIdx.x;
+    const LpRow row = lp_row(p, r);
+    const Span<DT> sp(p, row, part, p.chunks);
+    T* const out = (T*)p.grad + r * p.V;
+    const float g = p.g_logprob ? p.g_logprob[row.b * p.gl_sb + row.t * p.gl_st] : 0.f;
+    const float h = p.g_entropy ? p.g_entropy[row.b * p.ge_sb + row.t * p.ge_st] : 0.f;
+    float2 st = p.stats[r];
+    const bool off = row.token < 0 || row.bad_token || st.x == -INFINITY;
+    const float nan = __int_as_float(0x7FC00000);
+    const float m = ref_of(st.x), c = row.c, H = p.entropy[r];
+    float A = -(g + h * H) * row.inv_t, D = -h * row.inv_t * 0.6931471805599453f;
+    if (!(st.x < INFINITY)) A = nan;
+    const int token = off ? -1 : (int)row.token;
+    auto grad = [&](float x) {
+        const float d = fmaxf(fmaf(x - m, c, -st.y), kFloor), e = ex2(d);
+        return e * fmaf(D, d, A);
+    };
+    auto grad_at = [&](float x) {      // the token's own
+        const float d = fmaxf(fmaf(x - m, c, -st.y), kFloor), e = ex2(d);
+        const float q = -expm1f(fmaxf((x - m) * row.inv_t - st.y * 0.6931471805599453f, -1e4f));
+        const float v = g * row.inv_t * q + e * fmaf(D, d, -h * H * row.inv_t);
+        return st.x < INFINITY ? v : nan;
+    };
+    const bool together = (((uintptr_t)(out + sp.head)) & 15) == 0;
+    sp.singles(t, [&](int j, float x) { out[j] = Elem<DT>::to(off ? 0.f : j == token ? grad_at(x) : grad(x)); });
+    if (together) {
+        for (int v = sp.v0 + t; v < sp.v1; v += kLpAhead * kLpThreads) {
+            uint4 raw[kLpAhead];
+#pragma unroll
+            for (int i = 0; i < kLpAhead; i++) {
+                const int at = v + i * kLpThreads;
+                raw[i] = at < sp.v1 && !off ? ld_stream(sp.vec + at) : make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int i = 0; i < kLpAhead; i++) {
+                const int at = v + i * kLpThreads, j0 = sp.index(at);
+                float x[E];
+                Elem<DT>::wide(raw[i], x);
+                if ((unsigned)(token - j0) < (unsigned)E) {
+#pragma unroll
+                    for (int k = 0; k < E; k++) x[k] = j0 + k == token ? grad_at(x[k]) : grad(x[k]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < E; k++) x[k] = grad(x[k]);
+                }
+                if (at < sp.v1) __stcs(reinterpret_cast<uint4*>(out + sp.head) + at, off ? make_uint4(0u, 0u, 0u, 0u) : Elem<DT>::narrow(x));
+            }
+        }
+    } else {                           // logits and gradient start at different places of their 16 bytes: element by element
+        const int j1 = sp.index(sp.v1);
+        for (int j = sp.index(sp.v0) + t; j < j1; j += kLpThreads) {
+            const float x = off ? 0.f : Elem<DT>::one(sp.row + j);
+            out[j] = Elem<DT>::to(off ? 0.f : j == token ? grad_at(x) : grad(x));
+        }
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+static int lp_params(const rs_logprob_call* k, bool needs_tokens, LpParams* p, HostDevice* dev) {
+    if (!k) return RS_ERR_POINTER;
+    if (k->dtype != RS_DTYPE_F32 && k->dtype != RS_DTYPE_F16 && k->dtype != RS_DTYPE_BF16) return RS_ERR_DTYPE;
+    if (k->V <= 0 || k->V > RS_LOGPROB_MAX_V) return RS_ERR_LIMIT;
+    if (k->B <= 0 || k->T <= 0) return RS_ERR_BATCH;
+    if (k->T > 0x7fffffff || k->B > 0x7fffffff / k->T) return RS_ERR_LIMIT;
+    if (!(k->temperature >= 0.001 && k->temperature <= 1000)) return RS_ERR_TEMPERATURE;
+    const uintptr_t size = k->dtype == RS_DTYPE_F32 ? 4 : 2;
+    if (!k->logits || ((uintptr_t)k->logits & (size - 1))) return RS_ERR_POINTER;
+    if (k->token_bits != 32 && k->token_bits != 64) return RS_ERR_DTYPE;
+    if ((needs_tokens && !k->tokens) || ((uintptr_t)k->tokens & (uintptr_t)(k->token_bits / 8 - 1))) return RS_ERR_POINTER;
+    if ((uintptr_t)k->row_temperature & 3) return RS_ERR_POINTER;
+    memset(p, 0, sizeof *p);
+    p->logits = k->logits;
+    p->sb = k->stride_b;
+    p->st = k->stride_t;
+    p->rows = k->B * k->T;
+    p->T = (int)k->T;
+    p->V = (int)k->V;
+    p->tokens = k->tokens;
+    p->wide_tokens = k->token_bits == 64;
+    p->tok_sb = k->token_stride_b;
+    p->tok_st = k->token_stride_t;
+    p->temperature = (float)k->temperature;
+    p->row_temperature = k->row_temperature;
+    p->tmp_sb = k->temperature_stride_b;
+    p->tmp_st = k->temperature_stride_t;
+    const int rc = host_device(dev);
+    if (rc) return rc;
+    p->mirror = dev->mirror;
+    return RS_OK;
+}
+
+template <int DT, bool TOP>
+static int lp_launch(const LpParams& p, int parts, cudaStream_t stream) {
+    auto kern = lp_rows_kernel<DT, TOP>;
+    if (parts > 8) {
+        static std::mutex mu;
+        static bool done[64] = {};      // per device
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return host_cuda_fail(e, "cudaGetDevice");
+        std::lock_guard<std::mutex> lk(mu);
+        if (!done[dev & 63]) {
+            e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute(cluster)");
+            done[dev & 63] = true;
+        }
+    }
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof cfg);
+    cfg.gridDim = dim3((unsigned)(p.rows * parts));
+    cfg.blockDim = dim3(kLpThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)parts;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;      // a cluster of one too: its shared memory is addressed as the cluster's
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, parts);
+    if (e != cudaSuccess) return host_cuda_fail(e, "cudaLaunchKernelEx(logprobs)");
+    host_count_launch();
+    return RS_OK;
+}
+
+// CTAs per row: enough of them that every multiprocessor has two, as long as each keeps 4096 logits to read.
+static int lp_parts(long long rows, int V, int sms) {
+    int parts = 1;
+    while (parts < 16 && rows * parts < 2LL * sms && V / (2 * parts) >= 4096) parts *= 2;
+    return parts;
+}
+
+template <bool TOP>
+static int lp_dispatch(const LpParams& p, int dtype, int sms, cudaStream_t stream) {
+    const int parts = lp_parts(p.rows, p.V, sms);
+    switch (dtype) {
+        case RS_DTYPE_F32: return lp_launch<RS_DTYPE_F32, TOP>(p, parts, stream);
+        case RS_DTYPE_F16: return lp_launch<RS_DTYPE_F16, TOP>(p, parts, stream);
+        default: return lp_launch<RS_DTYPE_BF16, TOP>(p, parts, stream);
+    }
+}
+
+}  // namespace rs
+
+extern "C" {
+
+int rs_token_logprobs(const rs_logprob_call* call, float* logprob_device, float* entropy_device, float* stats_device) {
+    rs::LpParams p;
+    rs::HostDevice dev;
+    const int rc = rs::lp_params(call, true, &p, &dev);
+    if (rc) return rc;
+    if (!logprob_device || !entropy_device || ((uintptr_t)logprob_device & 3) || ((uintptr_t)entropy_device & 3) || ((uintptr_t)stats_device & 7))
+        return RS_ERR_POINTER;
+    p.logprob = logprob_device;
+    p.entropy = entropy_device;
+    p.stats = (float2*)stats_device;
+    return rs::lp_dispatch<false>(p, call->dtype, dev.sms, (cudaStream_t)call->stream);
+}
+
+int rs_token_logprobs_backward(const rs_logprob_call* call, const float* entropy_device, const float* stats_device,
+                               const float* grad_logprob_device, int64_t gl_stride_b, int64_t gl_stride_t,
+                               const float* grad_entropy_device, int64_t ge_stride_b, int64_t ge_stride_t, void* grad_device) {
+    rs::LpParams p;
+    rs::HostDevice dev;
+    const int rc = rs::lp_params(call, true, &p, &dev);
+    if (rc) return rc;
+    const uintptr_t size = call->dtype == RS_DTYPE_F32 ? 4 : 2;
+    if (!entropy_device || !stats_device || !grad_device || ((uintptr_t)entropy_device & 3) || ((uintptr_t)stats_device & 7) ||
+        ((uintptr_t)grad_device & (size - 1)) || ((uintptr_t)grad_logprob_device & 3) || ((uintptr_t)grad_entropy_device & 3))
+        return RS_ERR_POINTER;
+    p.entropy = const_cast<float*>(entropy_device);
+    p.stats = (float2*)const_cast<float*>(stats_device);
+    p.g_logprob = grad_logprob_device;
+    p.gl_sb = gl_stride_b;
+    p.gl_st = gl_stride_t;
+    p.g_entropy = grad_entropy_device;
+    p.ge_sb = ge_stride_b;
+    p.ge_st = ge_stride_t;
+    p.grad = grad_device;
+    // about 16 KB of logits a CTA, fewer where the grid would pass what a launch takes
+    const long long bytes = p.V * (long long)size;
+    long long chunks = (bytes + 16383) / 16384;
+    while (chunks > 1 && p.rows * chunks > 0x7fffffffLL) chunks = (chunks + 1) / 2;
+    p.chunks = (int)chunks;
+    const unsigned grid = (unsigned)(p.rows * chunks);
+    cudaStream_t st = (cudaStream_t)call->stream;
+    switch (call->dtype) {
+        case RS_DTYPE_F32: rs::lp_backward_kernel<RS_DTYPE_F32><<<grid, rs::kLpThreads, 0, st>>>(p); break;
+        case RS_DTYPE_F16: rs::lp_backward_kernel<RS_DTYPE_F16><<<grid, rs::kLpThreads, 0, st>>>(p); break;
+        default: rs::lp_backward_kernel<RS_DTYPE_BF16><<<grid, rs::kLpThreads, 0, st>>>(p);
+    }
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return rs::host_cuda_fail(e, "launch(logprobs backward)");
+    rs::host_count_launch();
+    return RS_OK;
+}
+
+int rs_top_logprobs(const rs_logprob_call* call, int32_t top_n, float* logprob_device, int32_t* rank_device, float* entropy_device,
+                    float* top_device, int32_t* top_ids_device) {
+    rs::LpParams p;
+    rs::HostDevice dev;
+    const int rc = rs::lp_params(call, false, &p, &dev);
+    if (rc) return rc;
+    if (top_n < 1 || top_n > RS_LOGPROB_MAX_TOP) return RS_ERR_LIMIT;
+    if (!entropy_device || !top_device || !top_ids_device || ((uintptr_t)logprob_device & 3) || ((uintptr_t)rank_device & 3) ||
+        ((uintptr_t)entropy_device & 3) || ((uintptr_t)top_device & 3) || ((uintptr_t)top_ids_device & 3))
+        return RS_ERR_POINTER;
+    if (!call->tokens && (logprob_device || rank_device)) return RS_ERR_POINTER;
+    p.logprob = logprob_device;
+    p.rank = rank_device;
+    p.entropy = entropy_device;
+    p.top = top_device;
+    p.top_ids = top_ids_device;
+    p.top_n = top_n;
+    return rs::lp_dispatch<true>(p, call->dtype, dev.sms, (cudaStream_t)call->stream);
+}
+
+int rs_logprobs_status(void* stream) {
+    int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbolAsync(&v, rs::g_lp_status, sizeof v, 0, cudaMemcpyDeviceToHost, (cudaStream_t)stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize((cudaStream_t)stream);
+    if (e == cudaSuccess && v) {
+        const int zero = 0;
+        e = cudaMemcpyToSymbolAsync(rs::g_lp_status, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, (cudaStream_t)stream);
+        if (e == cudaSuccess) e = cudaStreamSynchronize((cudaStream_t)stream);
+    }
+    if (e != cudaSuccess) return rs::host_cuda_fail(e, "status read");
+    return v;
+}
+
+}  // extern "C"

@@ -22,6 +22,7 @@
 // No tensor cores: nothing here is a contraction.  The bound is HBM bandwidth (4 bytes per
 // logit, 12 with penalties) for large batches and launch + barrier latency for tiny ones.
 #include "rs_common.cuh"
+#include "rs_host.cuh"
 #include "rs_rowcta.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -1798,6 +1799,19 @@ static int sample_static_impl(const float* logits, int64_t B, int64_t T, int64_t
     return launch_one<8, false>(p, kSlabOff, (cudaStream_t)stream, *di);
 }
 
+// ---- services of rs_host.cuh ----
+int host_device(HostDevice* out) {
+    DeviceInfo* di = nullptr;
+    const int rc = get_device(&di);
+    if (rc) return rc;
+    std::lock_guard<std::mutex> lk(g_mu);
+    *out = {di->sms, di->smem_optin, di->mirror};
+    return RS_OK;
+}
+int host_cuda_fail(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+void host_count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+uint32_t host_wait_polls() { return g_wait_polls.load(); }
+
 }  // namespace rs
 
 // ------------------------------------------------------------------- C ABI -----------------
@@ -1984,6 +1998,7 @@ const char* rs_status_string(int status) {
         case RS_ERR_TIMEOUT: return "a bounded on-chip wait gave up";
         case RS_ERR_LIMIT: return "size beyond what this entry point supports";
         case RS_ERR_INTERNAL: return "an invariant of the cutoff search was violated";
+        case RS_ERR_TOKEN: return "a token id is no column of the logits";
     }
     return "unknown status";
 }

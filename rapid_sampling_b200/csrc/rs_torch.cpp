@@ -51,6 +51,11 @@ volatile int* mirror_for(int device) {
     }
     return m.word.data_ptr<int>();
 }
+[[noreturn]] void throw_status(const char* what, int device, int v) {
+    std::string msg = std::string(what) + " on cuda:" + std::to_string(device) + " reported: " + rs_status_string(v) + " !\n";
+    if (v == RS_ERR_TEMPERATURE || v == RS_ERR_TOKEN) throw std::invalid_argument(msg);
+    throw std::runtime_error(msg);
+}
 // Raises what an earlier call on this device left in the mirror, once.
 void raise_pending_status(int device, at::Tensor& ws, cudaStream_t stream) {
     volatile int* w = mirror_for(device);
@@ -58,9 +63,7 @@ void raise_pending_status(int device, at::Tensor& ws, cudaStream_t stream) {
     if (v == 0) return;
     *w = 0;
     rs_clear_status(ws.data_ptr(), stream);
-    std::string msg = "an earlier sampling call on cuda:" + std::to_string(device) + " reported: " + rs_status_string(v) + " !\n";
-    if (v == RS_ERR_TEMPERATURE) throw std::invalid_argument(msg);
-    throw std::runtime_error(msg);
+    throw_status("an earlier sampling call", device, v);
 }
 
 struct Shapes {
@@ -203,6 +206,142 @@ at::Tensor sample_repetition_any(at::Tensor& logits, at::Tensor& penalties, at::
                          top_k, top_p, true);
 }
 
+// ---- log probabilities ---------------------------------------------------------------------------------------------
+
+// The same for the calls that have no workspace.  A call that is being captured neither raises nor creates the mirror:
+// both would touch the device outside the graph.
+static void raise_pending_logprobs(int device, cudaStream_t stream) {
+    if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) return;
+    volatile int* w = mirror_for(device);
+    const int v = *w;
+    if (v == 0) return;
+    *w = 0;
+    rs_logprobs_status(stream);      // clears the device's word
+    throw_status("an earlier call", device, v);
+}
+
+// Logits (V,), (B, V) or (B, T, V) with any strides but along V, one token per row, one temperature or one per row.
+static rs_logprob_call logprob_call(const at::Tensor& logits, const c10::optional<at::Tensor>& tokens, double temperature,
+                                    const c10::optional<at::Tensor>& row_temperature) {
+    rs_logprob_call c = {};
+    if (logits.scalar_type() != at::kFloat && logits.scalar_type() != at::kHalf && logits.scalar_type() != at::kBFloat16)
+        throw std::invalid_argument("logits must be float32, float16 or bfloat16, got " + std::string(logits.dtype().name()) + " !\n");
+    if (!logits.is_cuda()) throw std::invalid_argument("logits must be a CUDA tensor !\n");
+    const int64_t d = logits.dim();
+    if (d < 1 || d > 3) throw std::invalid_argument("logits must have shape (V,), (B,V) or (B,T,V) !\n");
+    c.V = logits.size(-1);
+    if (c.V < 1 || c.V > RS_LOGPROB_MAX_V) throw std::invalid_argument("Vocabulary size must lie in [1, 1048576], got " + std::to_string(c.V) + " !\n");
+    if (c.V > 1 && logits.stride(-1) != 1) throw std::invalid_argument("logits must be contiguous along the vocabulary !\n");
+    c.logits = logits.data_ptr();
+    c.dtype = logits.scalar_type() == at::kHalf ? RS_DTYPE_F16 : logits.scalar_type() == at::kBFloat16 ? RS_DTYPE_BF16 : RS_DTYPE_F32;
+    c.B = d >= 2 ? logits.size(0) : 1;
+    c.T = d == 3 ? logits.size(1) : 1;
+    c.stride_b = d >= 2 ? logits.stride(0) : 0;
+    c.stride_t = d == 3 ? logits.stride(1) : 0;
+    const at::IntArrayRef rows = logits.sizes().slice(0, d - 1);
+    c.token_bits = 64;
+    if (tokens.has_value()) {
+        const at::Tensor& t = *tokens;
+        if ((t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) || !t.is_cuda() || t.get_device() != logits.get_device())
+            throw std::invalid_argument("tokens must be an int32 or int64 CUDA tensor on the logits' device !\n");
+        if (t.sizes() != rows) throw std::invalid_argument("tokens must have the logits' shape without the vocabulary !\n");
+        c.tokens = t.data_ptr();
+        c.token_bits = t.scalar_type() == at::kInt ? 32 : 64;
+        c.token_stride_b = d >= 2 ? t.stride(0) : 0;
+        c.token_stride_t = d == 3 ? t.stride(1) : 0;
+    }
+    if (!(temperature >= 0.001 && temperature <= 1000)) fail(RS_ERR_TEMPERATURE, ", got " + std::to_string(temperature));
+    c.temperature = temperature;
+    if (row_temperature.has_value()) {
+        const at::Tensor& t = *row_temperature;
+        if (t.scalar_type() != at::kFloat || !t.is_cuda() || t.get_device() != logits.get_device())
+            throw std::invalid_argument("temperature must be a float32 CUDA tensor on the logits' device !\n");
+        if (t.dim() == 0) {
+        } else if (t.sizes() == rows) {
+            c.temperature_stride_b = d >= 2 ? t.stride(0) : 0;
+            c.temperature_stride_t = d == 3 ? t.stride(1) : 0;
+        } else if (d == 3 && t.dim() == 1 && t.size(0) == c.B) {
+            c.temperature_stride_b = t.stride(0);
+        } else {
+            throw std::invalid_argument("temperature must hold one value, one per row, or one per sequence of (B,T,V) logits !\n");
+        }
+        c.row_temperature = t.data_ptr<float>();
+    }
+    c.stream = at::cuda::getCurrentCUDAStream(logits.get_device()).stream();
+    return c;
+}
+
+static void check_logprobs(int rc) {
+    if (rc != RS_OK) fail(rc, "");
+}
+
+// (log probabilities, entropies, statistics for the backward call or None)
+static pybind11::tuple token_logprobs(const at::Tensor& logits, const at::Tensor& tokens, double temperature,
+                                      const c10::optional<at::Tensor>& row_temperature, bool keep_stats) {
+    rs_logprob_call c = logprob_call(logits, tokens, temperature, row_temperature);
+    c10::cuda::CUDAGuard guard(logits.device());
+    raise_pending_logprobs(logits.get_device(), (cudaStream_t)c.stream);
+    const auto f32 = at::TensorOptions().dtype(at::kFloat).device(logits.device());
+    at::Tensor lp = at::empty(tokens.sizes(), f32), ent = at::empty(tokens.sizes(), f32), stats;
+    if (keep_stats) stats = at::empty({c.B, c.T, 2}, f32);
+    if (lp.numel() > 0)
+        check_logprobs(rs_token_logprobs(&c, lp.data_ptr<float>(), ent.data_ptr<float>(), keep_stats ? stats.data_ptr<float>() : nullptr));
+    return pybind11::make_tuple(lp, ent, keep_stats ? pybind11::cast(stats) : pybind11::none());
+}
+
+static at::Tensor token_logprobs_backward(const at::Tensor& logits, const at::Tensor& tokens, double temperature,
+                                          const c10::optional<at::Tensor>& row_temperature, const at::Tensor& entropy,
+                                          const at::Tensor& stats, const c10::optional<at::Tensor>& g_logprob,
+                                          const c10::optional<at::Tensor>& g_entropy) {
+    rs_logprob_call c = logprob_call(logits, tokens, temperature, row_temperature);
+    c10::cuda::CUDAGuard guard(logits.device());
+    const int64_t d = logits.dim();
+    const float* g[2] = {nullptr, nullptr};
+    int64_t s[2][2] = {{0, 0}, {0, 0}};
+    for (int i = 0; i < 2; i++) {
+        const c10::optional<at::Tensor>& t = i ? g_entropy : g_logprob;
+        if (!t.has_value()) continue;
+        if (t->scalar_type() != at::kFloat || t->sizes() != tokens.sizes() || !t->is_cuda() || t->get_device() != logits.get_device())
+            throw std::invalid_argument("incoming gradients must be float32 CUDA tensors of the tokens' shape !\n");
+        g[i] = t->data_ptr<float>();
+        s[i][0] = d >= 2 ? t->stride(0) : 0;
+        s[i][1] = d == 3 ? t->stride(1) : 0;
+    }
+    for (const at::Tensor* t : {&entropy, &stats})
+        if (t->scalar_type() != at::kFloat || !t->is_contiguous() || t->numel() != c.B * c.T * (t == &stats ? 2 : 1) || !t->is_cuda() ||
+            t->get_device() != logits.get_device())
+            throw std::invalid_argument("entropy and stats must be those of the forward call !\n");
+    at::Tensor grad = at::empty(logits.sizes(), logits.options());
+    if (grad.numel() > 0)
+        check_logprobs(rs_token_logprobs_backward(&c, entropy.data_ptr<float>(), stats.data_ptr<float>(), g[0], s[0][0], s[0][1], g[1],
+                                                  s[1][0], s[1][1], grad.data_ptr()));
+    return grad;
+}
+
+// (log probabilities, ranks, entropies, top log probabilities, top ids); the first two None without tokens
+static pybind11::tuple top_logprobs(const at::Tensor& logits, int64_t top_n, const c10::optional<at::Tensor>& tokens, double temperature,
+                                    const c10::optional<at::Tensor>& row_temperature) {
+    rs_logprob_call c = logprob_call(logits, tokens, temperature, row_temperature);
+    if (top_n < 1 || top_n > RS_LOGPROB_MAX_TOP)
+        throw std::invalid_argument("top_n must lie in [1, " + std::to_string(RS_LOGPROB_MAX_TOP) + "], got " + std::to_string(top_n) + " !\n");
+    c10::cuda::CUDAGuard guard(logits.device());
+    raise_pending_logprobs(logits.get_device(), (cudaStream_t)c.stream);
+    const auto f32 = at::TensorOptions().dtype(at::kFloat).device(logits.device());
+    std::vector<int64_t> rows(logits.sizes().begin(), logits.sizes().end() - 1), slots = rows;
+    slots.push_back(top_n);
+    at::Tensor ent = at::empty(rows, f32), top = at::empty(slots, f32), ids = at::empty(slots, f32.dtype(at::kInt)), lp, rank;
+    if (tokens.has_value()) {
+        lp = at::empty(rows, f32);
+        rank = at::empty(rows, f32.dtype(at::kInt));
+    }
+    if (ent.numel() > 0)
+        check_logprobs(rs_top_logprobs(&c, (int32_t)top_n, tokens.has_value() ? lp.data_ptr<float>() : nullptr,
+                                       tokens.has_value() ? rank.data_ptr<int32_t>() : nullptr, ent.data_ptr<float>(),
+                                       top.data_ptr<float>(), ids.data_ptr<int32_t>()));
+    if (!tokens.has_value()) return pybind11::make_tuple(pybind11::none(), pybind11::none(), ent, top, ids);
+    return pybind11::make_tuple(lp, rank, ent, top, ids);
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     namespace py = pybind11;
     m.def("setup_rand", &setup_rand, py::arg("seed"), py::arg("B"));
@@ -221,6 +360,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("top_k") = py::none(), py::arg("top_p") = py::none(), py::arg("penalties") = py::none(),
           py::arg("presence_penalty") = 0.0, py::arg("repetition_penalty") = 0.0, py::arg("penalty_decay") = 0.0,
           py::arg("return_prob") = false);
+    m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("tokens"), py::arg("temperature"), py::arg("row_temperature"),
+          py::arg("keep_stats"));
+    m.def("token_logprobs_backward", &token_logprobs_backward, py::arg("logits"), py::arg("tokens"), py::arg("temperature"),
+          py::arg("row_temperature"), py::arg("entropy"), py::arg("stats"), py::arg("g_logprob"), py::arg("g_entropy"));
+    m.def("top_logprobs", &top_logprobs, py::arg("logits"), py::arg("top_n"), py::arg("tokens"), py::arg("temperature"),
+          py::arg("row_temperature"));
     m.def("kernel_launch_count", []() { return rs_kernel_launch_count(); });
     m.def("device_status", []() {
         // Synchronises the current stream and returns the status word of its workspace (0 = ok), clearing word and mirror.
@@ -229,6 +374,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         at::Tensor ws = workspace_for(dev, stream, 256);
         int v = rs_device_status(ws.data_ptr(), stream);
         if (v != 0) rs_clear_status(ws.data_ptr(), stream);
+        const int lp = rs_logprobs_status(stream);      // the word of the calls without a workspace
+        if (v == 0) v = lp;
         volatile int* w = mirror_for(dev);
         if (v == 0) v = *w;     // a status raised through another workspace of this device
         *w = 0;

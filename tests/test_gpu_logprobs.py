@@ -1,0 +1,383 @@
+"""GPU: log probabilities of given tokens, their gradient, ranks and alternatives, against plain 64-bit forms."""
+import math
+
+import pytest
+import torch
+
+from logprob_ref import close, close_grad, reference
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def make(rows, V, dtype, seed, sigma=2.5):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = (torch.randn(tuple(rows) + (V,), generator=gen, device="cuda") * sigma).to(DT[dtype])
+    t = torch.randint(0, V, tuple(rows), generator=gen, device="cuda")
+    return x, t
+
+
+def check_all(x, t, temperature=1.0, top_n=5, grads=True):
+    """Every output of both calls, and the gradient of both results."""
+    import rapid_sampling_b200 as rs
+    V = x.shape[-1]
+    gen = torch.Generator(device="cuda").manual_seed(99)
+    g = torch.randn(x.shape[:-1], generator=gen, device="cuda")
+    h = torch.randn(x.shape[:-1], generator=gen, device="cuda")
+    want = reference(x, t, temperature, top_n, g, h)
+    lp, ent = rs.batch_token_logprobs(x, t, temperature)
+    assert lp.dtype == ent.dtype == torch.float32 and lp.shape == t.shape
+    close(lp, want["logprobs"], V)
+    close(ent, want["entropy"], V)
+    lp2, rank, ent2, top, ids = rs.batch_top_logprobs(x, top_n, t, temperature)
+    close(lp2, want["logprobs"], V)
+    close(ent2, want["entropy"], V)
+    assert rank.dtype == ids.dtype == torch.int32
+    assert torch.equal(rank, want["ranks"])
+    assert torch.equal(ids, want["ids"])
+    close(top, want["top"], V)
+    if grads:
+        leaf = x.detach().clone(memory_format=torch.preserve_format).requires_grad_(True)
+        lp3, ent3 = rs.batch_token_logprobs(leaf, t, temperature)
+        close(lp3.detach(), want["logprobs"], V)      # (a row's bits depend on its address within 16 bytes, and a copy's differs)
+        close(ent3.detach(), want["entropy"], V)
+        got, = torch.autograd.grad((lp3, ent3), leaf, (g, h))
+        assert got.dtype == x.dtype and got.shape == x.shape
+        close_grad(got, want["grad"], x, g, h, temperature, want)
+    assert rs.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,V", [((1,), 1), ((3,), 2), ((2,), 7), ((5,), 31), ((4,), 256), ((3,), 257), ((2, 3), 1000), ((37,), 4099),
+                                    ((1,), 32768), ((2, 2), 50303), ((700,), 515), ((1,), 151936)])
+def test_sizes_and_types(rows, V, dtype):
+    x, t = make(rows, V, dtype, V + 1)
+    check_all(x, t, 1.0, top_n=min(20, 64))
+
+
+@pytest.mark.parametrize("n", [1, 2, 31, 64])
+def test_list_lengths(n):
+    x, t = make((6,), 5000, "f32", n)
+    check_all(x, t, 0.7, top_n=n, grads=False)
+    x, t = make((6,), 40, "bf16", n)       # fewer ids than slots for the longest
+    check_all(x, t, 0.7, top_n=n, grads=False)
+
+
+@pytest.mark.parametrize("temperature", [0.001, 0.1, 1.7, 1000.0])
+def test_temperatures(temperature):
+    x, t = make((9,), 3000, "f32", 5)
+    check_all(x, t, temperature)
+
+
+def test_row_temperatures():
+    x, t = make((4, 5), 2049, "bf16", 6)
+    per_row = 0.3 + torch.rand(4, 5, device="cuda")
+    check_all(x, t, per_row)
+    check_all(x, t, per_row[:, 0].contiguous())       # one per sequence
+    wide = (0.3 + torch.rand(5, 8, device="cuda"))[:, ::2].t()
+    check_all(x, t, wide)                              # any strides
+    check_all(x, t, torch.tensor(0.6, device="cuda"))
+    check_all(x[:, 0], t[:, 0], per_row[:, 0])
+
+
+def test_views_and_token_types():
+    big, t = make((3, 7), 1001, "f16", 7)
+    check_all(big[:, :-1], t[:, 1:])                                   # shifted, rows at odd addresses
+    check_all(big[:, 1:], t[:, :-1].int())
+    check_all(big[:, ::2], t[:, ::2])
+    check_all(big[1], t[1])
+    check_all(big[:, :, 3:], t % 998)                                  # columns cut off on the left
+    check_all(big[..., :513], t % 513)
+    check_all(big[0, 0], t[0, 0])                                      # (V,)
+    check_all(big[:1, 0].expand(4, 1001), t[0, :4])                    # one row for four tokens
+    check_all(big.transpose(0, 1), t.t())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_masks(dtype):
+    x, t = make((12,), 3001, dtype, 8)
+    low = torch.finfo(DT[dtype]).min
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x[0] = -math.inf                                                   # nothing left
+    x[1] = low                                                         # nothing but the lowest value: uniform
+    x[2, torch.rand(3001, generator=gen, device="cuda") < 0.99] = -math.inf
+    x[3, torch.rand(3001, generator=gen, device="cuda") < 0.99] = low
+    x[4] = -math.inf
+    x[4, 2999] = 1.0                                                   # one left
+    x[5] = low
+    x[5, 17] = 3.0
+    x[6, int(t[6])] = -math.inf                                        # the token itself masked
+    x[7] = -math.inf
+    x[7, :3] = 2.0                                                     # three left, all equal
+    x[8, ::2] = -math.inf
+    x[9] = 0.0
+    x[9, ::3] = -0.0                                                   # zeros of either sign are equal
+    check_all(x, t, 1.0, top_n=20)
+    check_all(x, t, 0.01, top_n=20)
+    check_all(x, t, 100.0, top_n=20)
+
+
+def test_not_finite_rows():
+    x, t = make((6,), 2050, "f32", 9)
+    x[1, 5] = math.nan
+    x[3, 2049] = math.inf
+    x[4, 7] = -math.nan
+    check_all(x, t, 1.0, top_n=4)
+    x[5] = math.nan
+    check_all(x, t, 1.0, top_n=64)
+
+
+def test_padded_positions():
+    x, t = make((4, 9), 777, "bf16", 10)
+    t[1, 4:] = -1
+    t[2] = -100
+    x[2] = math.nan                                                    # never read
+    check_all(x, t, 1.0, top_n=3)
+
+
+@pytest.mark.parametrize("V", [600, 5003, 40000, 151936])
+def test_ties(V):
+    gen = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.zeros(8, V, device="cuda")
+    x[1] = torch.randint(0, 16, (V,), generator=gen, device="cuda").float() * 0.5
+    x[2] = torch.randint(0, 2, (V,), generator=gen, device="cuda").float()
+    x[3, V // 2:] = 1.0
+    x[4, V - 3:] = 1.0
+    x[5] = torch.arange(V, device="cuda").float() / V                  # rising: the last ones win
+    x[6] = -torch.arange(V, device="cuda").float() / V
+    x[7, ::7] = 2.0
+    t = torch.tensor([0, 1, V - 1, V // 2, V - 1, V - 5, 3, 8], device="cuda")
+    check_all(x, t, 1.0, top_n=20)
+    check_all(x.half(), t, 1.0, top_n=64, grads=False)
+
+
+@pytest.mark.parametrize("dtype,E", [("f32", 4), ("bf16", 8)])
+def test_large_logits_crowded_in_few_threads(dtype, E):
+    """More large logits in the vectors of a few threads than the candidate list holds, most of them different."""
+    V = 200000
+    x, t = make((3,), V, dtype, 12, sigma=0.1)
+    j = torch.arange(V, device="cuda")
+    for r, threads in enumerate([1, 7, 30]):
+        crowd = ((j // E) % 256) < threads
+        x[r, crowd] = (5 + torch.rand(int(crowd.sum()), device="cuda")).to(x.dtype)
+    check_all(x, t, 1.0, top_n=64, grads=False)
+
+
+def test_confident_rows_keep_their_digits():
+    """log p = -log1p(the rest) where p is nearly 1: relative, not absolute, accuracy (three roundings and the sum's error).
+    The rest's terms are added apart from the maximum's own 1 but for those of the one thread that holds it, in which they
+    may be lost: with the rest spread evenly that is 1/256 of it at most."""
+    import rapid_sampling_b200 as rs
+    V = 65536
+    x = torch.full((3, V), 0.0, device="cuda")
+    for r, top in enumerate([20.0, 30.0, 40.0]):
+        x[r, 1234] = top
+    t = torch.full((3,), 1234, device="cuda")
+    lp, ent = rs.batch_token_logprobs(x, t)
+    want = reference(x, t)
+    assert bool(((lp.double() - want["logprobs"]).abs() <= (1 / 256 + 1e-4) * want["logprobs"].abs()).all()), (lp, want["logprobs"])
+    assert bool(((ent.double() - want["entropy"]).abs() <= (1 / 256 + 1e-4) * want["entropy"].abs()).all())
+
+
+def test_gradient_against_differences():
+    import rapid_sampling_b200 as rs
+    x, t = make((2,), 50, "f32", 13, sigma=1.0)
+    leaf = x.clone().requires_grad_(True)
+    lp, ent = rs.batch_token_logprobs(leaf, t, 0.8)
+    (2 * lp.sum() - 0.3 * ent.sum()).backward()
+    step = 1e-4
+    x64 = x.double()
+
+    def value(y):
+        w = reference(y, t, 0.8)
+        return float(2 * w["logprobs"].sum() - 0.3 * w["entropy"].sum())
+    for j in range(0, 50, 7):
+        a, b = x64.clone(), x64.clone()
+        a[1, j] += step
+        b[1, j] -= step
+        slope = (value(a) - value(b)) / (2 * step)
+        # central differences in 64 bits: step^2 * third derivative (below 10 here) + rounding 1e-12; the kernel's: 3e-5
+        assert abs(slope - float(leaf.grad[1, j])) < 1e-4
+
+
+def test_incoming_gradients():
+    """One result unused, a broadcast gradient, one with strides of its own, and a padded slice of the leaf."""
+    import rapid_sampling_b200 as rs
+    x, t = make((3, 6), 900, "f32", 14)
+    ones = torch.ones(3, 6, device="cuda")
+    leaf = x.clone().requires_grad_(True)
+    rs.batch_token_logprobs(leaf, t)[0].sum().backward()
+    want = reference(x, t, 1.0, 0, ones, None)
+    close_grad(leaf.grad, want["grad"], x, ones, None, 1.0, want)
+    leaf.grad = None
+    rs.batch_token_logprobs(leaf, t)[1].sum().backward()
+    want = reference(x, t, 1.0, 0, None, ones)
+    close_grad(leaf.grad, want["grad"], x, None, ones, 1.0, want)
+    leaf.grad = None
+    g = torch.randn(6, 3, device="cuda").t()
+    lp, _ = rs.batch_token_logprobs(leaf, t)
+    lp.backward(g)
+    want = reference(x, t, 1.0, 0, g, None)
+    close_grad(leaf.grad, want["grad"], x, g, None, 1.0, want)
+    leaf.grad = None
+    lp, _ = rs.batch_token_logprobs(leaf[:, :-1], t[:, 1:])
+    lp.sum().backward()
+    want = reference(x[:, :-1], t[:, 1:], 1.0, 0, ones[:, 1:], None)
+    close_grad(leaf.grad[:, :-1], want["grad"], x[:, :-1], ones[:, 1:], None, 1.0, want)
+    assert not leaf.grad[:, -1].any()
+    row = x[0, 0].clone().requires_grad_(True)                     # a row used by several tokens: gradients add up
+    rs.batch_token_logprobs(row.expand(6, 900), t[0])[0].sum().backward()
+    want = reference(x[0, 0].expand(6, 900), t[0], 1.0, 0, ones[0], None)["grad"].sum(0)
+    assert float((row.grad.double() - want).abs().max()) < 6 * 3 * 5e-6 + 1e-6
+
+
+def test_refusals_and_device_errors():
+    import rapid_sampling_b200 as rs
+    x, t = make((4,), 128, "f32", 15)
+    for bad in (lambda: rs.batch_token_logprobs(x.double(), t), lambda: rs.batch_token_logprobs(x.cpu(), t),
+                lambda: rs.batch_token_logprobs(x, t.float()), lambda: rs.batch_token_logprobs(x, t[:3]),
+                lambda: rs.batch_token_logprobs(x.t(), t[:1].expand(128)), lambda: rs.batch_token_logprobs(x, t.cpu()),
+                lambda: rs.batch_token_logprobs(x, t, 0.0), lambda: rs.batch_token_logprobs(x, t, 2000.0),
+                lambda: rs.batch_token_logprobs(x, t, float("nan")), lambda: rs.batch_token_logprobs(x, t, torch.ones(3, device="cuda")),
+                lambda: rs.batch_token_logprobs(x, t, torch.ones(4)), lambda: rs.batch_token_logprobs(x, t, torch.ones(4, device="cuda").double()),
+                lambda: rs.batch_token_logprobs(x, t, torch.ones(4, device="cuda", requires_grad=True)),
+                lambda: rs.batch_top_logprobs(x, 0), lambda: rs.batch_top_logprobs(x, 65), lambda: rs.batch_top_logprobs(x[None, None], 3),
+                lambda: rs.batch_token_logprobs(torch.zeros(1, 1048577, device="cuda"), t[:1]),
+                lambda: rs.batch_token_logprobs(torch.zeros(4, 0, device="cuda"), t)):
+        with pytest.raises(ValueError):
+            bad()
+    lp, ent = rs.batch_token_logprobs(x[:0], t[:0])                 # no rows: no work
+    assert lp.shape == ent.shape == (0,)
+    assert rs.batch_top_logprobs(x[:0], 3)[3].shape == (0, 3)
+    # a token that is no column: its row NaN, no gradient, the others untouched, and the next call raises
+    t2 = t.clone()
+    t2[2] = 128
+    leaf = x.clone().requires_grad_(True)
+    lp, ent = rs.batch_token_logprobs(leaf, t2)
+    torch.cuda.synchronize()
+    assert torch.isnan(lp[2]) and torch.isnan(ent[2]) and not torch.isnan(lp[[0, 1, 3]]).any()
+    grad, = torch.autograd.grad(lp[[0, 1, 3]].sum(), leaf)
+    assert not grad[2].any() and bool(grad[3].any())
+    with pytest.raises(ValueError, match="token"):
+        rs.batch_token_logprobs(x, t)
+    assert rs.device_status() == 0
+    # a temperature out of range counts as 1
+    heat = torch.tensor([1.0, 0.0, 1.0, float("nan")], device="cuda")
+    lp, _ = rs.batch_token_logprobs(x, t, heat)
+    close(lp, reference(x, t)["logprobs"], 128)
+    with pytest.raises(ValueError, match="Temperature"):
+        rs.batch_top_logprobs(x, 2)
+    assert rs.device_status() == 0
+    _, _, _, _, ids = rs.batch_top_logprobs(x, 2, t2)
+    assert rs.device_status() == -11 and ids[2].tolist() == [-1, -1]     # the explicit read clears what it reports
+    rs.batch_top_logprobs(x, 2)
+
+
+def test_without_tokens():
+    import rapid_sampling_b200 as rs
+    x, _ = make((5,), 1234, "bf16", 16)
+    lp, rank, ent, top, ids = rs.batch_top_logprobs(x, 7, temperature=0.5)
+    want = reference(x, None, 0.5, 7)
+    assert lp is None and rank is None
+    close(ent, want["entropy"], 1234)
+    close(top, want["top"], 1234)
+    assert torch.equal(ids, want["ids"])
+
+
+def test_same_bits_every_time_and_in_every_batch():
+    """A row's results do not depend on the run; the list does not depend on how many CTAs share the row either."""
+    import rapid_sampling_b200 as rs
+    x, t = make((600,), 20000, "bf16", 17)
+    a = rs.batch_top_logprobs(x, 20, t)
+    b = rs.batch_top_logprobs(x, 20, t)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    c = rs.batch_top_logprobs(x[:2], 20, t[:2])
+    assert torch.equal(a[4][:2], c[4]) and torch.equal(a[1][:2], c[1])
+    close(c[0], a[0][:2].double(), 20000)
+
+
+def test_capture_streams_and_two_graphs():
+    """First calls inside a capture, replays with new inputs, two graphs at once on two streams."""
+    import rapid_sampling_b200 as rs
+    x, t = make((16,), 30001, "bf16", 18)
+    y, s = make((16,), 30001, "bf16", 19)
+    graphs, outs, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for a, b, st in ((x, t, streams[0]), (y, s, streams[1])):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            outs.append(rs.batch_top_logprobs(a, 20, b) + tuple(rs.batch_token_logprobs(a, b)))
+        graphs.append(graph)
+    for rep in range(3):
+        x.copy_(make((16,), 30001, "bf16", 20 + rep)[0])
+        torch.cuda.synchronize()
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for out, a, b in ((outs[0], x, t), (outs[1], y, s)):
+            want = rs.batch_top_logprobs(a, 20, b) + tuple(rs.batch_token_logprobs(a, b))
+            assert all(torch.equal(p, q) for p, q in zip(out, want))
+    with torch.cuda.stream(streams[0]):
+        got = rs.batch_token_logprobs(y, s)
+    streams[0].synchronize()
+    assert torch.equal(got[0], rs.batch_token_logprobs(y, s)[0])
+
+
+def test_captured_training_step():
+    import rapid_sampling_b200 as rs
+    x, t = make((2, 40), 5001, "f32", 21)
+    leaf = x.clone().requires_grad_(True)
+    g = torch.randn(2, 40, device="cuda")
+
+    def step():
+        lp, ent = rs.batch_token_logprobs(leaf, t, 0.9)
+        return torch.autograd.grad((lp * g).sum() + 0.1 * ent.sum(), leaf)[0]
+    want = step().clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_offsets_beyond_32_bits():
+    """Rows of one tensor whose element offsets pass 2^31, read and, for the gradient, written."""
+    import rapid_sampling_b200 as rs
+    V = 1048576
+    rows = 2 ** 31 // V + 3
+    x = torch.empty(rows, V, dtype=torch.bfloat16, device="cuda")
+    t = torch.full((rows,), -1, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for r in (0, rows - 1):
+        x[r] = torch.randn(V, generator=gen, device="cuda").bfloat16()
+        t[r] = 77 + r
+    pick = [0, rows - 1]
+    want = reference(x[pick], t[pick], 1.0, 5, torch.ones(2, device="cuda"), None)
+    lp, rank, ent, top, ids = rs.batch_top_logprobs(x, 5, t)
+    close(lp[pick], want["logprobs"], V)
+    assert torch.equal(ids[pick], want["ids"]) and torch.equal(rank[pick], want["ranks"])
+    x.requires_grad_(True)
+    lp, ent = rs.batch_token_logprobs(x, t)
+    grad, = torch.autograd.grad(lp.sum(), x)
+    close_grad(grad[pick], want["grad"], x[pick], torch.ones(2, device="cuda"), None, 1.0, want)
+    assert not grad[1].any() and not grad[rows - 2].any()
+
+
+def test_follows_a_sampling_call():
+    """As a serving step uses them: sample, then the sampled ids' log probabilities, ranks and alternatives."""
+    import rapid_sampling_b200 as rs
+    x, _ = make((8,), 50304, "f32", 22)
+    T = torch.tensor([0.7, 1.0] * 4, device="cuda")
+    ids, prob, _ = rs.batch_sampling_rows(x, rs.setup_rand(3, 8), T, torch.full((8,), 40, dtype=torch.int32, device="cuda"),
+                                          torch.full((8,), 0.95, device="cuda"), return_prob=True)
+    lp, rank, ent, top, top_ids = rs.batch_top_logprobs(x, 40, ids, T)
+    # the sampler's probability is a 32-bit softmax of its own: 2e-6 relative
+    assert bool(((lp.exp() - prob).abs() <= 2e-5 * prob).all())
+    assert bool((rank <= 40).all()) and torch.equal(top_ids.gather(1, (rank.long() - 1)[:, None])[:, 0], ids)
