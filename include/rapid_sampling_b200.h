@@ -281,8 +281,31 @@ int rs_token_logprobs_backward(const rs_logprob_call* call, const float* entropy
 int rs_top_logprobs(const rs_logprob_call* call, int32_t top_n, float* logprob_device, int32_t* rank_device, float* entropy_device,
                     float* top_device, int32_t* top_ids_device);
 
-/* Reads and clears the current device's status word of the three calls above (synchronises `stream`). */
+/* Reads and clears the current device's status word of the three calls above and of rs_head_logits (synchronises `stream`). */
 int rs_logprobs_status(void* stream);
+
+/*
+ * The lm_head in 8-bit floating point, whose logits the calls above and below take.  No counterpart in the reference, which
+ * starts from finished logits.
+ *
+ * rs_head_quantize: weights (V, K), rows row_stride elements apart, to e4m3 codes (V, K) contiguous, 16-byte aligned, and
+ * scales (ceil(V / 128), ceil(K / 128)), one for each block of 128 x 128: scale = max(amax / 448, 2^-126), code = the e4m3
+ * value nearest to weight / scale (quotients and scales in 32 bits, ties to even).  NaN or infinity make NaN of what they touch.
+ *
+ * rs_head_logits: out[m, v] = sum_k hidden[m, k] * weight[v, k] for M rows of hidden states, which the call quantizes in
+ * the same way, a scale for each row's 128 columns.  Products are exact, sums fp32.  out (M, V): rows out_stride elements
+ * apart, fp32, fp16 or bf16.  K is a multiple of 16 and at most RS_HEAD_MAX_K; hidden rows are hidden_stride apart (0: one
+ * row for all).  Workspace: rs_head_workspace_bytes(M, K), 256-byte aligned, any content; calls that overlap on the GPU need
+ * one each.  A wait that gives up (RS_ERR_TIMEOUT, the results are void) is reported by rs_logprobs_status and the mirror.
+ */
+#define RS_HEAD_MAX_K 65536
+#define RS_HEAD_MAX_ROWS 16777216
+int rs_head_quantize(const void* weight_device, int32_t dtype, int64_t V, int64_t K, int64_t row_stride, void* codes_device,
+                     float* scales_device, void* stream);
+size_t rs_head_workspace_bytes(int64_t M, int64_t K);
+int rs_head_logits(const void* hidden_device, int32_t hidden_dtype, int64_t M, int64_t K, int64_t hidden_stride, const void* codes_device,
+                   const float* scales_device, int64_t V, void* out_device, int32_t out_dtype, int64_t out_stride, void* workspace_device,
+                   size_t workspace_bytes, void* stream);
 
 /*
  * Device status word.  The kernels never trap: a condition they cannot report through a return code is written to

@@ -94,6 +94,25 @@ def batch_top_logprobs(logits, top_n, tokens=None, temperature=1.0):
     return logprobs.top_logprobs(logits, top_n, tokens, temperature)
 
 
+def lm_head_quantize(weight):
+    """(codes, scales) of an lm_head's weights (V, K), float32, float16 or bfloat16, K a multiple of 16: float8_e4m3fn codes
+    (V, K) and float32 scales (ceil(V / 128), ceil(K / 128)), one for each block of 128 x 128:
+    scale = max(amax / 448, 2^-126), code = the value nearest to weight / scale."""
+    return _load_ext().lm_head_quantize(weight)
+
+
+def lm_head_logits(hidden, codes, scales, dtype=None, out=None):
+    """Logits (..., V) = hidden (..., K) times the weights that `codes` and `scales` stand for (`lm_head_quantize`, or any
+    e4m3 checkpoint with a float32 scale for each block of 128 x 128).  The hidden states (float32, float16 or bfloat16) are
+    quantized within the call, a scale for each row's 128 columns; sums are float32.  The result has `dtype` (float32,
+    float16 or bfloat16; float32 unless `out` says otherwise) and goes to `out` where given, whose rows may lie apart.
+    Rows of hidden and out lie at equal distances.  Not differentiable."""
+    import torch
+    if dtype is None:
+        dtype = torch.float32 if out is None else out.dtype
+    return _load_ext().lm_head_logits(hidden, codes, scales, dtype, out)
+
+
 def kernel_launch_count():
     return _load_ext().kernel_launch_count()
 
@@ -112,4 +131,5 @@ def release_workspaces():
 
 __all__ = ["setup_rand", "batch_sampling_temperature_topk_topp", "batch_sampling_repetition_temperature_topk_topp",
            "batch_sampling_temperature_topk_topp_any", "batch_sampling_repetition_temperature_topk_topp_any", "batch_sampling_rows",
-           "batch_token_logprobs", "batch_top_logprobs", "kernel_launch_count", "device_status", "release_workspaces"]
+           "batch_token_logprobs", "batch_top_logprobs", "lm_head_quantize", "lm_head_logits",
+           "kernel_launch_count", "device_status", "release_workspaces"]

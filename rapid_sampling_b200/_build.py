@@ -38,7 +38,7 @@ def _run(cmd, verbose):
         print(r.stdout)
 
 
-CU_SOURCES = ["rs_sampler.cu", "rs_rowcta.cu", "rs_vocab_parallel.cu", "rs_logprobs.cu"]
+CU_SOURCES = ["rs_sampler.cu", "rs_rowcta.cu", "rs_vocab_parallel.cu", "rs_logprobs.cu", "rs_head.cu"]
 HEADERS = [os.path.join(CSRC, h) for h in ("rs_device.cuh", "rs_common.cuh", "rs_rowcta.cuh", "rs_host.cuh")] + \
     [os.path.join(INCLUDE, "rapid_sampling_b200.h")]
 OBJ_DIR = os.path.join(HERE, "build")

@@ -21,7 +21,8 @@ RS_STATIC_SCRATCH_FLOATS = 4194304
 
 SYMBOLS = ["rs_setup_rand", "rs_workspace_bytes", "rs_sample", "rs_sample_debug", "rs_sample_host", "rs_sample_typed", "rs_sample_static_scratch", "rs_rows_workspace_bytes", "rs_sample_rows",
            "rs_device_status", "rs_clear_status", "rs_set_status_mirror", "rs_set_wait_polls", "rs_set_dependent_launch", "rs_selftest_bounded_wait", "rs_set_cluster_override", "rs_set_path_override", "rs_kernel_launch_count", "rs_vp_workspace_bytes", "rs_vp_layout", "rs_vp_fast_layout", "rs_vp_stage", "rs_vp_tile_begin", "rs_vp_tile_max", "rs_status_string",
-           "rs_last_cuda_error", "rs_version", "rs_token_logprobs", "rs_token_logprobs_backward", "rs_top_logprobs", "rs_logprobs_status"]
+           "rs_last_cuda_error", "rs_version", "rs_token_logprobs", "rs_token_logprobs_backward", "rs_top_logprobs", "rs_logprobs_status",
+           "rs_head_quantize", "rs_head_workspace_bytes", "rs_head_logits"]
 
 
 class Trace(C.Structure):
@@ -87,6 +88,10 @@ def load():
     L.rs_token_logprobs_backward.argtypes = [lp, vp, vp, vp, i64, i64, vp, i64, i64, vp]
     L.rs_top_logprobs.argtypes = [lp, C.c_int32, vp, vp, vp, vp, vp]
     L.rs_logprobs_status.argtypes = [vp]
+    L.rs_head_quantize.argtypes = [vp, C.c_int32, i64, i64, i64, vp, vp, vp]
+    L.rs_head_workspace_bytes.argtypes = [i64, i64]
+    L.rs_head_workspace_bytes.restype = C.c_size_t
+    L.rs_head_logits.argtypes = [vp, C.c_int32, i64, i64, i64, vp, vp, i64, vp, C.c_int32, i64, vp, C.c_size_t, vp]
     L.rs_device_status.argtypes = [vp, vp]
     L.rs_clear_status.argtypes = [vp, vp]
     L.rs_set_status_mirror.argtypes = [vp]

@@ -15,5 +15,6 @@ int host_device(HostDevice* out);                       // of the current device
 int host_cuda_fail(cudaError_t e, const char* what);    // keeps the message for rs_last_cuda_error, returns RS_ERR_CUDA
 void host_count_launch();                               // counts one kernel for rs_kernel_launch_count
 uint32_t host_wait_polls();                             // poll limit of the kernels' bounded waits
+int host_status_word(int** out);                        // device address of the word that rs_logprobs_status reads (rs_logprobs.cu)
 
 }  // namespace rs

@@ -717,6 +717,23 @@ static int lp_dispatch(const LpParams& p, int dtype, int sms, cudaStream_t strea
     }
 }
 
+int host_status_word(int** out) {
+    static std::mutex mu;
+    static int* at[64] = {};      // per device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return host_cuda_fail(e, "cudaGetDevice");
+    std::lock_guard<std::mutex> lk(mu);
+    if (!at[dev & 63]) {
+        void* a = nullptr;
+        e = cudaGetSymbolAddress(&a, g_lp_status);
+        if (e != cudaSuccess) return host_cuda_fail(e, "cudaGetSymbolAddress(status)");
+        at[dev & 63] = (int*)a;
+    }
+    *out = at[dev & 63];
+    return RS_OK;
+}
+
 }  // namespace rs
 
 extern "C" {

@@ -342,6 +342,85 @@ static pybind11::tuple top_logprobs(const at::Tensor& logits, int64_t top_n, con
     return pybind11::make_tuple(lp, rank, ent, top, ids);
 }
 
+// ---- lm_head -------------------------------------------------------------------------------------------------------
+
+static int dtype_of(const at::Tensor& t, const char* name) {
+    if (t.scalar_type() == at::kFloat) return RS_DTYPE_F32;
+    if (t.scalar_type() == at::kHalf) return RS_DTYPE_F16;
+    if (t.scalar_type() == at::kBFloat16) return RS_DTYPE_BF16;
+    throw std::invalid_argument(std::string(name) + " must be float32, float16 or bfloat16, got " + std::string(t.dtype().name()) + " !\n");
+}
+// Elements between the rows of (..., n); every row must follow the one before at the same distance.
+static int64_t row_stride(const at::Tensor& t, const char* name) {
+    const int64_t d = t.dim();
+    if (t.size(-1) > 1 && t.stride(-1) != 1) throw std::invalid_argument(std::string(name) + " must be contiguous along the last dimension !\n");
+    int64_t step = 0, rows = 1;      // of the dimensions so far, from the last
+    for (int64_t i = d - 2; i >= 0; i--) {
+        if (t.size(i) == 1) continue;
+        if (rows == 1) step = t.stride(i);
+        else if (t.stride(i) != step * rows) throw std::invalid_argument(std::string(name) + " must have rows at equal distances !\n");
+        rows *= t.size(i);
+    }
+    return rows == 1 ? t.size(-1) : step;
+}
+
+static pybind11::tuple lm_head_quantize(const at::Tensor& weight) {
+    const int dt = dtype_of(weight, "weight");
+    if (!weight.is_cuda() || weight.dim() != 2) throw std::invalid_argument("weight must be a CUDA tensor of shape (V, K) !\n");
+    const int64_t V = weight.size(0), K = weight.size(1);
+    if (V < 1 || V > RS_HEAD_MAX_ROWS || K < 16 || K > RS_HEAD_MAX_K || K % 16 != 0)
+        throw std::invalid_argument("K must be a multiple of 16 in [16, 65536] and V at least 1, got V=" + std::to_string(V) + ", K=" + std::to_string(K) + " !\n");
+    const int64_t step = row_stride(weight, "weight");
+    c10::cuda::CUDAGuard guard(weight.device());
+    at::Tensor codes = at::empty({V, K}, weight.options().dtype(at::kFloat8_e4m3fn).memory_format(at::MemoryFormat::Contiguous));
+    at::Tensor scales = at::empty({(V + 127) / 128, (K + 127) / 128}, codes.options().dtype(at::kFloat));
+    const int rc = rs_head_quantize(weight.data_ptr(), dt, V, K, step, codes.data_ptr(), scales.data_ptr<float>(),
+                                    at::cuda::getCurrentCUDAStream(weight.get_device()).stream());
+    if (rc != RS_OK) fail(rc, "");
+    return pybind11::make_tuple(codes, scales);
+}
+
+static at::Tensor lm_head_logits(const at::Tensor& hidden, const at::Tensor& codes, const at::Tensor& scales, at::ScalarType dtype,
+                                 const c10::optional<at::Tensor>& out_) {
+    const int hdt = dtype_of(hidden, "hidden");
+    if (!hidden.is_cuda() || hidden.dim() < 1) throw std::invalid_argument("hidden must be a CUDA tensor of shape (..., K) !\n");
+    const int dev = hidden.get_device();
+    if (codes.scalar_type() != at::kFloat8_e4m3fn || codes.dim() != 2 || !codes.is_cuda() || codes.get_device() != dev || !codes.is_contiguous() ||
+        ((uintptr_t)codes.data_ptr() & 15))
+        throw std::invalid_argument("codes must be a contiguous, 16-byte aligned float8_e4m3fn tensor of shape (V, K) on the hidden states' device !\n");
+    const int64_t V = codes.size(0), K = codes.size(1), M = hidden.numel() / std::max<int64_t>(hidden.size(-1), 1);
+    if (V < 1 || V > RS_HEAD_MAX_ROWS || K < 16 || K > RS_HEAD_MAX_K || K % 16 != 0 || M > RS_HEAD_MAX_ROWS)
+        throw std::invalid_argument("K must be a multiple of 16 in [16, 65536] and V at least 1, got V=" + std::to_string(V) + ", K=" + std::to_string(K) + " !\n");
+    if (hidden.size(-1) != K) throw std::invalid_argument("hidden must have the codes' K columns !\n");
+    if (scales.scalar_type() != at::kFloat || !scales.is_cuda() || scales.get_device() != dev || !scales.is_contiguous() || scales.dim() != 2 ||
+        scales.size(0) != (V + 127) / 128 || scales.size(1) != (K + 127) / 128)
+        throw std::invalid_argument("scales must be a contiguous float32 tensor with one value for each block of 128 x 128 codes !\n");
+    const int64_t step = row_stride(hidden, "hidden");
+    std::vector<int64_t> shape(hidden.sizes().begin(), hidden.sizes().end() - 1);
+    shape.push_back(V);
+    c10::cuda::CUDAGuard guard(hidden.device());
+    cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev).stream();
+    raise_pending_logprobs(dev, stream);
+    at::Tensor out;
+    if (out_.has_value()) {
+        out = *out_;
+        if (!out.is_cuda() || out.get_device() != dev || out.sizes() != at::IntArrayRef(shape) || out.scalar_type() != dtype)
+            throw std::invalid_argument("out must have the hidden states' shape with V columns, the requested type, and their device !\n");
+    } else {
+        out = at::empty(shape, at::TensorOptions().dtype(dtype).device(hidden.device()));
+    }
+    const int odt = dtype_of(out, "dtype");
+    const int64_t ostep = row_stride(out, "out");
+    if (M > 1 && ostep < V) throw std::invalid_argument("out must have rows that do not overlap !\n");
+    if (M == 0) return out;
+    // the caching allocator hands the workspace out per stream and, while capturing, per graph: no two calls share it
+    at::Tensor ws = at::empty({(int64_t)rs_head_workspace_bytes(M, K)}, at::TensorOptions().dtype(at::kByte).device(hidden.device()));
+    const int rc = rs_head_logits(hidden.data_ptr(), hdt, M, K, step, codes.data_ptr(), scales.data_ptr<float>(), V, out.data_ptr(), odt,
+                                  std::max(ostep, V), ws.data_ptr(), (size_t)ws.numel(), stream);
+    if (rc != RS_OK) fail(rc, "");
+    return out;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     namespace py = pybind11;
     m.def("setup_rand", &setup_rand, py::arg("seed"), py::arg("B"));
@@ -366,6 +445,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("row_temperature"), py::arg("entropy"), py::arg("stats"), py::arg("g_logprob"), py::arg("g_entropy"));
     m.def("top_logprobs", &top_logprobs, py::arg("logits"), py::arg("top_n"), py::arg("tokens"), py::arg("temperature"),
           py::arg("row_temperature"));
+    m.def("lm_head_quantize", &lm_head_quantize, py::arg("weight"));
+    m.def("lm_head_logits", [](const at::Tensor& hidden, const at::Tensor& codes, const at::Tensor& scales, py::object dtype,
+                               c10::optional<at::Tensor> out) {
+        if (!THPDtype_Check(dtype.ptr())) throw std::invalid_argument("dtype must be a torch.dtype !\n");
+        return lm_head_logits(hidden, codes, scales, reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type, out);
+    }, py::arg("hidden"), py::arg("codes"), py::arg("scales"), py::arg("dtype"), py::arg("out"));
     m.def("kernel_launch_count", []() { return rs_kernel_launch_count(); });
     m.def("device_status", []() {
         // Synchronises the current stream and returns the status word of its workspace (0 = ok), clearing word and mirror.
