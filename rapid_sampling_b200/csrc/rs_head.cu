@@ -79,9 +79,11 @@ __device__ __forceinline__ uint32_t head_amax4(const float (&x)[4]) {
 // One warp per row and block of 128 columns.  scales: (blocks, pitch), a column per row, as the product reads them.
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(256) head_quantize_rows_kernel(const void* src, long long stride, int M, int K, int blocks, uint8_t* codes,
-                                                                 float* scales, int pitch) {
+                                                                 float* scales, int pitch, int* arrived, int counters) {
     using T = typename HeadIn<DT>::T;
     grid_dependents_may_launch();
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < counters; i += 256) arrived[i] = 0;      // the product's
     const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31, m = (int)(item / blocks), b = (int)(item - (long long)m * blocks);
     if (m >= M) return;
@@ -93,38 +95,133 @@ __global__ void __launch_bounds__(256) head_quantize_rows_kernel(const void* src
     if (lane == 0) scales[(long long)b * pitch + m] = s;
 }
 
-// One CTA per block of 128 x 128 weights: a warp's lanes are 128 columns, a warp takes every eighth row.
+// Two fp32 at a time (the compiler does not pair scalar operations by itself).
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+// Codes of a pair by div_by's steps (a + b r with -s for the remainders).
+__device__ __forceinline__ uint32_t head_codes2(float a, float b, uint64_t minus_s, uint64_t r) {
+    const uint64_t x = f2_pack(a, b);
+    uint64_t q = f2_mul(x, r);
+    q = f2_fma(f2_fma(q, minus_s, x), r, q);
+    q = f2_fma(f2_fma(q, minus_s, x), r, q);
+    f2_unpack(q, a, b);
+    uint16_t c;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(b), "f"(a));
+    return c;
+}
+
+// 16 bytes of weights, as they lie in memory.
 template <int DT, bool VEC>
-__global__ void __launch_bounds__(256) head_quantize_blocks_kernel(const void* src, long long stride, int V, int K, int blocks, uint8_t* codes,
-                                                                   float* scales) {
+__device__ __forceinline__ uint4 head_ld16(const typename HeadIn<DT>::T* p) {
     using T = typename HeadIn<DT>::T;
+    uint4 v;
+    if constexpr (VEC) {
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    } else {
+        T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+        for (int i = 0; i < 16 / (int)sizeof(T); i++) e[i] = p[i];
+    }
+    return v;
+}
+// The bits of the largest |x| of a word (fp32), or of either half (bf16, fp16: positive patterns compare as integers, NaN
+// above infinity).
+template <int DT>
+__device__ __forceinline__ uint32_t head_abs_max(uint32_t m, uint32_t w) {
+    if constexpr (DT == RS_DTYPE_F32) return max(m, w & 0x7FFFFFFFu);
+    else return __vmaxu2(m, w & 0x7FFF7FFFu);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t head_abs_bits(uint32_t m) {      // as the bits of a float
+    if constexpr (DT == RS_DTYPE_F32) return m;
+    const uint32_t h = max(m & 0xFFFFu, m >> 16);
+    if constexpr (DT == RS_DTYPE_BF16) return h << 16;
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h))) & 0x7FFFFFFFu;
+}
+template <int DT>
+__device__ __forceinline__ void head_pair(uint32_t w, float& a, float& b) {      // both halves of a 16-bit pair
+    if constexpr (DT == RS_DTYPE_BF16) {
+        a = __uint_as_float(w << 16);
+        b = __uint_as_float(w & 0xFFFF0000u);
+    } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        a = f.x;
+        b = f.y;
+    }
+}
+
+// One CTA per block of 128 x 128 weights, which stays in registers as it was read (16-bit: 32 a thread, four CTAs an SM): 16
+// bytes a load, a warp's lanes along the rows.
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(256, DT == RS_DTYPE_F32 ? 2 : 4)
+    head_quantize_blocks_kernel(const void* src, long long stride, int V, int K, int blocks, uint8_t* codes, float* scales) {
+    using T = typename HeadIn<DT>::T;
+    constexpr int E = 16 / (int)sizeof(T), PER_ROW = 128 / E, ROWS = 256 / PER_ROW, N = 128 / ROWS;
     __shared__ uint32_t sh[8];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int t = threadIdx.x;
     const int vb = (int)(blockIdx.x / (unsigned)blocks), b = (int)(blockIdx.x - (unsigned)vb * (unsigned)blocks);
-    const int k = b * kHeadBlock + lane * 4;
-    float x[16][4];
-    uint32_t amax = 0u;
+    const int k = b * kHeadBlock + (t % PER_ROW) * E, v0 = vb * kHeadBlock + t / PER_ROW;
+    const T* p = (const T*)src + v0 * stride + k;
+    uint4 x[N];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int v = vb * kHeadBlock + i * 8 + w;
-        x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
-        if (v < V && k < K) head_ld4<VEC>((const T*)src + v * stride + k, x[i]);
+    for (int i = 0; i < N; i++) {
+        x[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (v0 + i * ROWS < V && k < K) x[i] = head_ld16<DT, VEC>(p + i * ROWS * stride);
     }
+    uint32_t m = 0u;
 #pragma unroll
-    for (int i = 0; i < 16; i++) amax = max(amax, head_amax4(x[i]));
-    amax = __reduce_max_sync(0xffffffffu, amax);
-    if (lane == 0) sh[w] = amax;
+    for (int i = 0; i < N; i++) m = head_abs_max<DT>(head_abs_max<DT>(head_abs_max<DT>(head_abs_max<DT>(m, x[i].x), x[i].y), x[i].z), x[i].w);
+    m = __reduce_max_sync(0xffffffffu, head_abs_bits<DT>(m));
+    if ((t & 31) == 0) sh[t >> 5] = m;
     __syncthreads();
-    amax = sh[0];
+    m = sh[0];
 #pragma unroll
-    for (int i = 1; i < 8; i++) amax = max(amax, sh[i]);
-    const float s = head_scale(amax), r = __frcp_rn(s);
+    for (int i = 1; i < 8; i++) m = max(m, sh[i]);
+    const float s = head_scale(m), r = __frcp_rn(s);
+    const uint64_t minus_s = f2_pack(-s, -s), rr = f2_pack(r, r);
+    const bool quick = s >= 8.6736174e-19f && s <= 1e30f;       // as in head_quotient
+    uint8_t* out = codes + (long long)v0 * K + k;
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int v = vb * kHeadBlock + i * 8 + w;
-        if (v < V && k < K) *reinterpret_cast<uint32_t*>(codes + (long long)v * K + k) = head_codes4(x[i], s, r);
+    for (int i = 0; i < N; i++) {
+        if (v0 + i * ROWS < V && k < K) {
+            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            if constexpr (E == 4) {
+                float f[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) f[j] = __uint_as_float(w[j]);
+                *reinterpret_cast<uint32_t*>(out + (long long)i * ROWS * K) =
+                    quick ? head_codes2(f[0], f[1], minus_s, rr) | (head_codes2(f[2], f[3], minus_s, rr) << 16) : head_codes4(f, s, r);
+            } else {
+                float f[8];
+#pragma unroll
+                for (int j = 0; j < 4; j++) head_pair<DT>(w[j], f[2 * j], f[2 * j + 1]);
+                uint2 c;
+                if (quick) {
+                    c.x = head_codes2(f[0], f[1], minus_s, rr) | (head_codes2(f[2], f[3], minus_s, rr) << 16);
+                    c.y = head_codes2(f[4], f[5], minus_s, rr) | (head_codes2(f[6], f[7], minus_s, rr) << 16);
+                } else {
+                    const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
+                    c = make_uint2(head_codes4(lo, s, r), head_codes4(hi, s, r));
+                }
+                *reinterpret_cast<uint2*>(out + (long long)i * ROWS * K) = c;
+            }
+        }
     }
-    if (threadIdx.x == 0) scales[(long long)vb * blocks + b] = s;
+    if (t == 0) scales[(long long)vb * blocks + b] = s;
 }
 
 // ---- tcgen05 ------------------------------------------------------------------------------------------------------------
@@ -132,8 +229,8 @@ __global__ void __launch_bounds__(256) head_quantize_blocks_kernel(const void* s
 __device__ __forceinline__ uint64_t head_desc(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-// e4m3 by e4m3, both along K, fp32 sums; M = 128 lanes, N columns
-__device__ __forceinline__ uint32_t head_idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24); }
+// e4m3 by e4m3, both along K, fp32 sums; m lanes (128 a CTA), n columns
+__device__ __forceinline__ uint32_t head_idesc(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
 __device__ __forceinline__ void head_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
@@ -143,16 +240,12 @@ __device__ __forceinline__ void head_mma(uint32_t d, uint64_t a, uint64_t b, uin
 __device__ __forceinline__ void head_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(addr)
-        : "memory");
-#pragma unroll
-    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+// 32 lanes (a warp's quarter of the accumulator) by 16 or 32 columns; valid after tmem_ld_wait.
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -166,154 +259,241 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int
                  : "memory");
 }
 
-// ---- the product --------------------------------------------------------------------------------------------------------
+// ---- how the work is split ----------------------------------------------------------------------------------------------
+// A unit is one tile of the result and one block of 128 columns of K; unit u = tile * blocks + block.  Either every worker (a
+// CTA, or a pair of them) takes whole tiles in turn, or the units are cut into equal runs of neighbours (`split`), so that all
+// workers end together however many tiles there are.  Then a tile may lie in the runs of several workers: each leaves its
+// sums in the workspace, and the one that is done last adds them up in the order of the workers.
+struct HeadWork {
+    long long units;
+    int workers, blocks, tiles, split;
+    __host__ __device__ __forceinline__ long long start(int w) const { return units * w / workers; }
+    __device__ __forceinline__ int owner(long long u) const { return (int)(((u + 1) * workers - 1) / units); }
+};
+struct HeadWalk {      // one worker's segments, in order
+    const HeadWork& k;
+    const int worker;
+    long long u, u1;
+    int tile, b0, b1;
+    __device__ __forceinline__ HeadWalk(const HeadWork& kk, int w) : k(kk), worker(w), tile(w - kk.workers), b0(0), b1(0) {
+        u = k.start(w);
+        u1 = k.start(w + 1);
+    }
+    __device__ __forceinline__ bool next() {
+        if (!k.split) {
+            tile += k.workers;
+            b1 = k.blocks;
+            return tile < k.tiles;
+        }
+        if (u >= u1) return false;
+        tile = (int)(u / k.blocks);
+        b0 = (int)(u - (long long)tile * k.blocks);
+        b1 = (int)min((long long)k.blocks, b0 + (u1 - u));
+        u += b1 - b0;
+        return true;
+    }
+    __device__ __forceinline__ bool whole() const { return b1 - b0 == k.blocks; }
+};
+
 struct HeadParams {
     const float* sa;         // (blocks, pitch): the tokens' scales
     const float* sw;         // (V blocks, blocks): the weights'
     void* out;               // (M, V), rows ldo elements apart
     long long ldo;
-    int M, V, blocks, pitch;
-    int n;                   // tokens of a tile, a multiple of 16
-    int token_tiles, tiles;
+    HeadWork work;
+    int M, V, pitch;
+    int n;                   // few tokens: columns of the accumulator, 16 or 32
+    int token_tiles;         // more tokens: tiles of 128, or of 256 for pairs
     int stages;
+    int wide_store;          // more tokens: bytes of a store that the result's rows allow (32, 16, or 0: one by one)
+    float* partial;          // split work: two slots a CTA
+    int* arrived;            // split work: workers done with the tile that begins in a worker's run
     uint32_t polls;
     int *status, *mirror;
 };
 
+constexpr int kHeadMaxWorkers = 160;      // CTAs that the workspace has slots for
 constexpr int kHeadMaxStages = 12;
-__host__ __device__ constexpr int head_stage_bytes(int n) { return 128 * 128 + n * 128 + ((n * 4 + 1023) / 1024) * 1024; }
 
-struct HeadShared {
-    uint64_t full[kHeadMaxStages], empty[kHeadMaxStages], sum_full[2], sum_empty[2];
-    uint32_t tmem;
-    int gave_up;
+// One lane of a converged warp.  The copying and the multiplying warp run their loops with all lanes and only issue with one:
+// uniform control flow keeps descriptors and coordinates in uniform registers (a loop of one lane alone took 1200 cycles a unit).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
+// Bounded waits: the first that runs out reports, and everyone stops at the next wait.
+struct HeadWait {
+    const HeadParams& p;
+    volatile int* gave_up;
+    __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) const {
+        for (uint32_t i = 0; i < p.polls; i++) {
+            if (mbar_try_wait(bar, parity)) return true;
+            if (*gave_up) return false;
+        }
+        *gave_up = 1;
+        atomicExch(p.status, RS_ERR_TIMEOUT);
+        if (p.mirror) *reinterpret_cast<volatile int*>(p.mirror) = RS_ERR_TIMEOUT;
+        return false;
+    }
 };
+// Called by the adding threads (THREADS of them, barrier 1) after they have written their sums of a tile they share.
+// Returns whether this CTA is the last, and then sees the others' sums.
+template <int THREADS>
+__device__ __forceinline__ bool head_last(const HeadParams& p, int counter, int needed, int* flag) {
+    __threadfence();
+    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+    if (threadIdx.x == 0) *flag = atomicAdd(p.arrived + counter, 1) == needed - 1;
+    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+    const bool last = *(volatile int*)flag;
+    __threadfence();
+    return last;
+}
 
-// NT: most tokens of a tile (32, 64, 128, 256).  Warps 0 .. W-1 add the blocks' sums up, each thread one row of weights by
-// NT tokens (half of them at NT = 256); then one warp that copies and one that multiplies.
-template <int NT, typename OUT>
-__global__ void __launch_bounds__((NT > 128 ? 8 : 4) * 32 + 64, 1)
-    head_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ HeadParams p) {
-    constexpr int W = NT > 128 ? 8 : 4, COLS = NT > 128 ? NT / 2 : NT;
-    constexpr uint32_t kTmemCols = 2 * NT;
+// ---- few tokens -----------------------------------------------------------------------------------------------------------
+// 128 rows of weights are the accumulator's lanes and all tokens (at most 32) its columns, so that the tensor core's work is
+// small; the time is that of the weights' bytes.  Warps 0 .. 3 add the blocks' sums up, each thread one row by all tokens; then
+// one warp that copies and one that multiplies.  A ring of stages and four accumulators keep the three apart.  A step is two
+// blocks: waits and arrivals, about 150 cycles each between products, are paid once for both.
+constexpr int kFewTokens = 32, kFewBufs = 4;
+// weights of both blocks, tokens of both, the tokens' scales of both
+__host__ __device__ constexpr int head_few_stage(int n) { return 2 * 128 * 128 + 2 * n * 128 + 1024; }
+
+template <typename OUT>
+__global__ void __launch_bounds__(192, 1)
+    head_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ HeadParams p) {
+    constexpr int W = 4, NT = kFewTokens, BUFS = kFewBufs;
+    constexpr uint32_t kTmemCols = BUFS * 2 * NT;
     extern __shared__ uint8_t raw_smem[];
-    __shared__ HeadShared sh;
+    __shared__ uint64_t full_[kHeadMaxStages], empty_[kHeadMaxStages], sfull_[BUFS], sempty_[BUFS];
+    __shared__ uint32_t tmem_at;
+    __shared__ int gave_up, flag;
     const uint32_t base = (smem_addr(raw_smem) + 1023u) & ~1023u;
+    const uint8_t* const base_p = raw_smem + (base - smem_addr(raw_smem));
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t stage_bytes = (uint32_t)head_stage_bytes(p.n);
-    const uint32_t full = smem_addr(sh.full), empty = smem_addr(sh.empty), sfull = smem_addr(sh.sum_full), sempty = smem_addr(sh.sum_empty);
+    const uint32_t stage_bytes = (uint32_t)head_few_stage(p.n), stages = (uint32_t)p.stages, x_bytes = (uint32_t)p.n * 128u;
+    const uint32_t full = smem_addr(full_), empty = smem_addr(empty_), sfull = smem_addr(sfull_), sempty = smem_addr(sempty_);
     if (threadIdx.x == 0) {
-        for (int i = 0; i < p.stages; i++) {
+        for (uint32_t i = 0; i < stages; i++) {
             mbar_init(full + 8 * i, 1);
             mbar_init(empty + 8 * i, 1 + W);
         }
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < BUFS; i++) {
             mbar_init(sfull + 8 * i, 1);
             mbar_init(sempty + 8 * i, W);
         }
-        sh.gave_up = 0;
+        gave_up = 0;
         fence_mbar_init();
     }
     if (w == W + 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sh.tmem)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_at)), "r"(kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = sh.tmem;
+    const uint32_t tmem = tmem_at;
     grid_dependency_wait();                       // the tokens' codes and scales are another kernel's
-    const volatile int* gave_up = &sh.gave_up;
-    // A wait that runs out is reported; everyone stops at the next wait, and the copies in flight are waited for below.
-    auto wait = [&](uint32_t bar, uint32_t parity) {
-        for (uint32_t i = 0; i < p.polls; i++) {
-            if (mbar_try_wait(bar, parity)) return true;
-            if (*gave_up) return false;
-        }
-        sh.gave_up = 1;
-        atomicExch(p.status, RS_ERR_TIMEOUT);
-        if (p.mirror) *reinterpret_cast<volatile int*>(p.mirror) = RS_ERR_TIMEOUT;
-        return false;
-    };
+    const HeadWait wait = {p, &gave_up};
+    HeadWalk walk(p.work, blockIdx.x);
     if (w == W) {
-        if (lane == 0) {
-            uint32_t it = 0, s = 0, ph = 0;      // blocks so far, their stage, its phase
-            bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
-                const int vb = tile / p.token_tiles, m0 = (tile - vb * p.token_tiles) * p.n;
-                for (int b = 0; b < p.blocks; b++, it++) {
-                    if (it >= (uint32_t)p.stages && !wait(empty + 8 * s, ph ^ 1u)) { ok = false; break; }
-                    const uint32_t at = base + s * stage_bytes, bar = full + 8 * s;
-                    mbar_expect_tx(bar, 128u * 128u + (uint32_t)p.n * 132u);
-                    tma_2d(at, &map_w, b * kHeadBlock, vb * 128, bar);
-                    tma_2d(at + 16384u, &map_x, b * kHeadBlock, m0, bar);
-                    bulk_g2s(at + 16384u + (uint32_t)p.n * 128u, p.sa + (long long)b * p.pitch + m0, (uint32_t)p.n * 4u, bar);
-                    if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1u; }
+        uint32_t it = 0, s = 0, ph = 0;           // steps so far, their stage, its phase
+        bool ok = true;
+        while (ok && walk.next())
+            for (int b = walk.b0; b < walk.b1; b += 2, it++) {
+                if (it >= stages && !__all_sync(0xffffffffu, wait(empty + 8 * s, ph ^ 1u))) { ok = false; break; }
+                if (elect_one()) {
+                    const uint32_t at = base + s * stage_bytes, bar = full + 8 * s, n = (uint32_t)min(2, walk.b1 - b);
+                    mbar_expect_tx(bar, n * (128u * 128u + (uint32_t)p.n * 132u));
+                    for (uint32_t i = 0; i < n; i++) {
+                        tma_2d(at + i * 16384u, &map_w, (b + (int)i) * kHeadBlock, walk.tile * 128, bar);
+                        tma_2d(at + 32768u + i * x_bytes, &map_x, (b + (int)i) * kHeadBlock, 0, bar);
+                        bulk_g2s(at + 32768u + 2 * x_bytes + i * (uint32_t)p.n * 4u, p.sa + (long long)(b + i) * p.pitch, (uint32_t)p.n * 4u, bar);
+                    }
                 }
+                __syncwarp();
+                if (++s == stages) { s = 0; ph ^= 1u; }
             }
-            // nothing may still be on its way into shared memory when the CTA ends: neither a copy nor, in the ordinary
-            // case, the arrival that frees a stage
-            const uint32_t n = min(it, (uint32_t)p.stages);
-            for (uint32_t i = 0; i < n; i++) {
-                const uint32_t k = it - 1 - i, st = k % (uint32_t)p.stages, parity = (k / (uint32_t)p.stages) & 1u;
-                if (!ok || !wait(empty + 8 * st, parity)) {
-                    ok = false;
-                    mbar_wait_bounded(full + 8 * st, parity, p.polls);
-                }
+        // nothing may still be on its way into shared memory when the CTA ends: neither a copy nor, in the ordinary
+        // case, the arrival that frees a stage
+        const uint32_t n = min(it, stages);
+        for (uint32_t i = 0; i < n; i++) {
+            const uint32_t k = it - 1 - i, st = k % stages, parity = (k / stages) & 1u;
+            if (!ok || !wait(empty + 8 * st, parity)) {
+                ok = false;
+                mbar_wait_bounded(full + 8 * st, parity, p.polls);
             }
         }
     } else if (w == W + 1) {
-        if (lane == 0) {
-            const uint32_t idesc = head_idesc(p.n);
-            uint32_t it = 0, s = 0, ph = 0;
-            bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x)
-                for (int b = 0; b < p.blocks; b++, it++) {
-                    const uint32_t buf = it & 1u;
-                    if (it >= 2 && !wait(sempty + 8 * buf, ((it >> 1) & 1u) ^ 1u)) { ok = false; break; }
-                    if (!wait(full + 8 * s, ph)) { ok = false; break; }
-                    tmem_fence_after();
-                    const uint64_t da = head_desc(base + s * stage_bytes), db = head_desc(base + s * stage_bytes + 16384u);
-#pragma unroll
-                    for (int k = 0; k < 4; k++) head_mma(tmem + buf * NT, da + 2 * k, db + 2 * k, idesc, k > 0);
-                    head_commit(empty + 8 * s);
-                    head_commit(sfull + 8 * buf);
-                    if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1u; }
-                }
-            // (after a wait that ran out: the products in flight end by themselves)
-            if (!ok && it > 0) mbar_wait_bounded(sfull + 8 * ((it - 1) & 1u), ((it - 1) >> 1) & 1u, p.polls);
-        }
-    } else {
-        const int quad = w & 3, half = w >> 2, row = quad * 32 + lane, col0 = half * COLS;
-        uint32_t it = 0, s = 0;
+        const uint32_t idesc = head_idesc(128, p.n);
+        const uint64_t desc = head_desc(base);
+        uint32_t it = 0, s = 0, ph = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
-            const int vb = tile / p.token_tiles, m0 = (tile - vb * p.token_tiles) * p.n;
-            const float* sw = p.sw + (long long)vb * p.blocks;
-            float acc[COLS];
-#pragma unroll
-            for (int i = 0; i < COLS; i++) acc[i] = 0.f;
-            for (int b = 0; b < p.blocks; b++, it++) {
-                const uint32_t buf = it & 1u;
-                const float f = __ldg(sw + b);
-                ok = wait(sfull + 8 * buf, (it >> 1) & 1u);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        while (ok && walk.next())
+            for (int b = walk.b0; b < walk.b1; b += 2, it++) {
+                const uint32_t buf = it % BUFS;
+                if (it >= BUFS && !__all_sync(0xffffffffu, wait(sempty + 8 * buf, ((it / BUFS) & 1u) ^ 1u))) { ok = false; break; }
+                if (!__all_sync(0xffffffffu, wait(full + 8 * s, ph))) { ok = false; break; }
                 tmem_fence_after();
-                const float* sa = reinterpret_cast<const float*>(raw_smem + (base - smem_addr(raw_smem)) + s * stage_bytes + 16384u + (uint32_t)p.n * 128u) + col0;
+                if (elect_one()) {
+                    const uint64_t da = desc + ((s * stage_bytes) >> 4), db = da + (32768u >> 4);
 #pragma unroll
-                for (int q = 0; q < COLS; q += 16) {
-                    if (col0 + q < p.n) {
-                        float v[16];
-                        tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + buf * NT + col0 + q, v);
+                    for (int k = 0; k < 4; k++) head_mma(tmem + buf * 2 * NT, da + 2 * k, db + 2 * k, idesc, k > 0);
+                    if (b + 1 < walk.b1) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            head_mma(tmem + buf * 2 * NT + NT, da + (16384u >> 4) + 2 * k, db + (x_bytes >> 4) + 2 * k, idesc, k > 0);
+                    }
+                    head_commit(sfull + 8 * buf);
+                    head_commit(empty + 8 * s);
+                }
+                __syncwarp();
+                if (++s == stages) { s = 0; ph ^= 1u; }
+            }
+        // (after a wait that ran out: the products in flight end by themselves)
+        if (!ok && it > 0) mbar_wait_bounded(sfull + 8 * ((it - 1) % BUFS), ((it - 1) / BUFS) & 1u, p.polls);
+    } else {
+        const int row = w * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(w * 32) << 16);
+        uint32_t it = 0, s = 0;
+        bool dead = false;                        // after a wait that ran out: no more waits, but every barrier of the adding warps
+        float scale[2] = {0.f, 0.f};              // of the weights' blocks: these 32 and the next, one a lane
+        while (walk.next()) {
+            const float* sw = p.sw + (long long)walk.tile * p.work.blocks;
+            scale[0] = walk.b0 + lane < walk.b1 ? __ldg(sw + walk.b0 + lane) : 0.f;
+            uint64_t acc[NT / 2];
+#pragma unroll
+            for (int i = 0; i < NT / 2; i++) acc[i] = 0ull;
+            for (int b = walk.b0; b < walk.b1; b += 2, it++) {
+                const uint32_t buf = it % BUFS;
+                const int q = (b - walk.b0) & 31;
+                if (q == 0) {
+                    if (b > walk.b0) scale[0] = scale[1];
+                    scale[1] = b + 32 + lane < walk.b1 ? __ldg(sw + b + 32 + lane) : 0.f;
+                }
+                const float f0 = __shfl_sync(0xffffffffu, scale[0], q), f1 = __shfl_sync(0xffffffffu, scale[0], q + 1);
+                if (!dead) dead = !__all_sync(0xffffffffu, wait(sfull + 8 * buf, (it / BUFS) & 1u));
+                if (dead) break;
+                tmem_fence_after();
+                const ulonglong2* sa = reinterpret_cast<const ulonglong2*>(base_p + s * stage_bytes + 32768u + 2 * x_bytes);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if (b + h < walk.b1) {
+                        const uint64_t ff = h ? f2_pack(f1, f1) : f2_pack(f0, f0);
+                        uint32_t v[NT];
+                        tmem_ld32(lanes + buf * 2 * NT + h * NT, v);      // (columns behind the last token: not looked at)
                         tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            const float4 g = *reinterpret_cast<const float4*>(sa + q + i);
-                            acc[q + i] = fmaf(v[i], g.x * f, acc[q + i]);
-                            acc[q + i + 1] = fmaf(v[i + 1], g.y * f, acc[q + i + 1]);
-                            acc[q + i + 2] = fmaf(v[i + 2], g.z * f, acc[q + i + 2]);
-                            acc[q + i + 3] = fmaf(v[i + 3], g.w * f, acc[q + i + 3]);
-                        }
+                        for (int c = 0; c < NT; c += 16)
+                            if (c < p.n) {
+#pragma unroll
+                                for (int i = c; i < c + 16; i += 4) {
+                                    const ulonglong2 g = sa[(h * p.n + i) / 4];
+                                    acc[i / 2] = f2_fma(f2_pack(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), f2_mul(g.x, ff), acc[i / 2]);
+                                    acc[i / 2 + 1] = f2_fma(f2_pack(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), f2_mul(g.y, ff), acc[i / 2 + 1]);
+                                }
+                            }
                     }
                 }
                 tmem_fence_before();
@@ -322,18 +502,37 @@ __global__ void __launch_bounds__((NT > 128 ? 8 : 4) * 32 + 64, 1)
                     mbar_arrive(sempty + 8 * buf);
                     mbar_arrive(empty + 8 * s);
                 }
-                if (++s == (uint32_t)p.stages) s = 0;
+                if (++s == stages) s = 0;
             }
-            if (!ok) break;
-            const int v = vb * 128 + row;
-            if (v < p.V) {
-                OUT* o = (OUT*)p.out + (long long)(m0 + col0) * p.ldo + v;
-                const int cols = min(p.n, p.M - m0) - col0;
+            float y[NT];
 #pragma unroll
-                for (int i = 0; i < COLS; i++) {
-                    OUT y;
-                    head_to(y, acc[i]);
-                    if (i < cols) __stcs(o + i * p.ldo, y);
+            for (int i = 0; i < NT / 2; i++) f2_unpack(acc[i], y[2 * i], y[2 * i + 1]);
+            if (!walk.whole()) {
+                // slot 1: the tile begins in this run; slot 0: it began in an earlier one
+                float* mine = p.partial + (long long)(2 * (int)blockIdx.x + (walk.b0 == 0)) * 128 * p.n;
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+                    if (i < p.M) mine[i * 128 + row] = y[i];
+                const long long u = (long long)walk.tile * p.work.blocks;
+                const int c0 = p.work.owner(u), c1 = p.work.owner(u + p.work.blocks - 1);
+                if (!head_last<W * 32>(p, c0, c1 - c0 + 1, &flag)) continue;
+#pragma unroll
+                for (int i = 0; i < NT; i++) y[i] = 0.f;
+                for (int c = c0; c <= c1; c++) {
+                    const float* from = p.partial + (long long)(2 * c + (c == c0)) * 128 * p.n;
+#pragma unroll
+                    for (int i = 0; i < NT; i++)
+                        if (i < p.M) y[i] += __ldcg(from + i * 128 + row);
+                }
+            }
+            const int v = walk.tile * 128 + row;
+            if (v < p.V && !dead) {
+                OUT* o = (OUT*)p.out + v;
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    OUT z;
+                    head_to(z, y[i]);
+                    if (i < p.M) __stcs(o + i * p.ldo, z);
                 }
             }
         }
@@ -343,6 +542,292 @@ __global__ void __launch_bounds__((NT > 128 ? 8 : 4) * 32 + 64, 1)
     __syncthreads();
     tmem_fence_after();
     if (w == W + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+// ---- more tokens ------------------------------------------------------------------------------------------------------------
+// The tokens are the accumulator's lanes and 256 rows of weights its columns: a thread's sums of a block then share one scale,
+// its token's times the block's, where weights on the lanes need one of each token (reading those from shared memory cost a
+// quarter of the time at 64 tokens).  Up to 128 tokens a CTA has a tile to itself and the time is that of the weights' bytes.
+// Beyond, a pair of CTAs shares a tile of 256 tokens by 256 weight rows: each CTA brings 128 tokens and 128 weight rows, its
+// accumulator holds its 128 tokens by all 256 weight rows, and one thread of the first CTA issues the products of both; the
+// pair reads 64 KB for a unit where two CTAs of their own would read 96 KB.
+template <bool PAIR> __host__ __device__ constexpr int head_more_stage() { return 128 * 128 + (PAIR ? 128 : 256) * 128; }
+
+__device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void head_mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+// arrives at the barrier of the same address in both CTAs once the products issued so far are done
+__device__ __forceinline__ void head_commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+                 : "memory");
+}
+// (nothing in ordinary memory is handed over with these two: releasing it to the cluster would cost each arrival a fence)
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx_cluster(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+template <typename OUT>
+__device__ __forceinline__ uint32_t head_word(float a, float b);
+template <> __device__ __forceinline__ uint32_t head_word<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t head_word<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// COLS neighbours of a row: `wide` bytes a store where the rows allow it, else one by one
+template <int COLS, typename OUT>
+__device__ __forceinline__ void head_store(OUT* o, const uint64_t (&acc)[COLS / 2], int cols, int wide) {
+    constexpr int PER32 = 32 / (int)sizeof(OUT);
+    if (wide && cols >= COLS) {
+#pragma unroll
+        for (int i = 0; i < COLS; i += PER32) {
+            uint32_t x[8];
+            if constexpr (sizeof(OUT) == 4) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    float a, b;
+                    f2_unpack(acc[i / 2 + j], a, b);
+                    x[2 * j] = __float_as_uint(a);
+                    x[2 * j + 1] = __float_as_uint(b);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    float a, b;
+                    f2_unpack(acc[i / 2 + j], a, b);
+                    x[j] = head_word<OUT>(a, b);
+                }
+            }
+            if (wide == 32) {
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o + i), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]),
+                             "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+                             : "memory");
+            } else {
+                *reinterpret_cast<uint4*>(o + i) = make_uint4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<uint4*>(o + i + PER32 / 2) = make_uint4(x[4], x[5], x[6], x[7]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < COLS / 2; i++) {
+            float a, b;
+            f2_unpack(acc[i], a, b);
+            OUT z;
+            head_to(z, a);
+            if (2 * i < cols) o[2 * i] = z;
+            head_to(z, b);
+            if (2 * i + 1 < cols) o[2 * i + 1] = z;
+        }
+    }
+}
+
+template <bool PAIR, typename OUT>
+__global__ void __launch_bounds__(10 * 32, 1)
+    head_more_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ HeadParams p) {
+    constexpr int W = 8, COLS = 128, NT = 256, CTAS = PAIR ? 2 : 1;
+    constexpr uint32_t kTmemCols = 512, kStage = (uint32_t)head_more_stage<PAIR>();
+    extern __shared__ uint8_t raw_smem[];
+    __shared__ uint64_t full_[kHeadMaxStages], empty_[kHeadMaxStages], sfull_[2], sempty_[2];
+    __shared__ uint32_t tmem_at;
+    __shared__ int gave_up, flag;
+    const uint32_t base = (smem_addr(raw_smem) + 1023u) & ~1023u;
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = PAIR ? (int)cluster_ctarank() : 0, worker = (int)blockIdx.x / CTAS;
+    const uint32_t stages = (uint32_t)p.stages;
+    const uint32_t full = smem_addr(full_), empty = smem_addr(empty_), sfull = smem_addr(sfull_), sempty = smem_addr(sempty_);
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < stages; i++) {
+            mbar_init(full + 8 * i, CTAS);            // a pair's: those of the first CTA, both copying warps
+            mbar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(sfull + 8 * i, 1);
+            mbar_init(sempty + 8 * i, CTAS * W);      // a pair's: those of the first CTA, both CTAs' adding warps
+        }
+        gave_up = 0;
+        fence_mbar_init();
+    }
+    if (w == W + 1) {
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_at)), "r"(kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_at)), "r"(kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if constexpr (PAIR) {
+        cluster_arrive();
+        cluster_wait();                               // the other CTA's barriers are there
+    }
+    tmem_fence_after();
+    const uint32_t tmem = tmem_at;
+    grid_dependency_wait();
+    const HeadWait wait = {p, &gave_up};
+    HeadWalk walk(p.work, worker);
+    if (w == W) {
+        const uint32_t first_full = PAIR ? map_to_cta(full, 0) : full;
+        uint32_t it = 0, s = 0, ph = 0;
+        bool ok = true;
+        while (ok && walk.next()) {
+            const int vt = walk.tile / p.token_tiles, mt = walk.tile - vt * p.token_tiles;
+            const int v0 = vt * 256 + rank * 128, m0 = mt * 128 * CTAS + rank * 128;
+            for (int b = walk.b0; b < walk.b1; b++, it++) {
+                if (it >= stages && !__all_sync(0xffffffffu, wait(empty + 8 * s, ph ^ 1u))) { ok = false; break; }
+                if (elect_one()) {
+                    const uint32_t at = base + s * kStage, bar = first_full + 8 * s;
+                    if constexpr (PAIR) {
+                        mbar_expect_tx_cluster(bar, kStage);
+                        tma_2d_pair(at, &map_x, b * kHeadBlock, m0, bar);
+                        tma_2d_pair(at + 16384u, &map_w, b * kHeadBlock, v0, bar);
+                    } else {
+                        mbar_expect_tx(bar, kStage);
+                        tma_2d(at, &map_x, b * kHeadBlock, m0, bar);
+                        tma_2d(at + 16384u, &map_w, b * kHeadBlock, v0, bar);
+                    }
+                }
+                __syncwarp();
+                if (++s == stages) { s = 0; ph ^= 1u; }
+            }
+        }
+        const uint32_t n = min(it, stages);           // as in head_few_kernel; a pair's copies count on the first CTA's barriers
+        for (uint32_t i = 0; i < n; i++) {
+            const uint32_t k = it - 1 - i, st = k % stages, parity = (k / stages) & 1u;
+            if (!ok || !wait(empty + 8 * st, parity)) {
+                ok = false;
+                if (rank == 0) mbar_wait_bounded(full + 8 * st, parity, p.polls);
+            }
+        }
+    } else if (w == W + 1) {
+        if (rank == 0) {
+            const uint32_t idesc = head_idesc(128 * CTAS, NT);
+            const uint64_t desc = head_desc(base);
+            uint32_t it = 0, s = 0, ph = 0;
+            bool ok = true;
+            while (ok && walk.next())
+                for (int b = walk.b0; b < walk.b1; b++, it++) {
+                    const uint32_t buf = it & 1u;
+                    if (it >= 2 && !__all_sync(0xffffffffu, wait(sempty + 8 * buf, ((it >> 1) & 1u) ^ 1u))) { ok = false; break; }
+                    if (!__all_sync(0xffffffffu, wait(full + 8 * s, ph))) { ok = false; break; }
+                    tmem_fence_after();
+                    if (elect_one()) {
+                        const uint64_t da = desc + ((s * kStage) >> 4), db = da + (16384u >> 4);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            if constexpr (PAIR) head_mma_pair(tmem + buf * NT, da + 2 * k, db + 2 * k, idesc, k > 0);
+                            else head_mma(tmem + buf * NT, da + 2 * k, db + 2 * k, idesc, k > 0);
+                        }
+                        if constexpr (PAIR) {
+                            head_commit_pair(sfull + 8 * buf);
+                            head_commit_pair(empty + 8 * s);
+                        } else {
+                            head_commit(sfull + 8 * buf);
+                            head_commit(empty + 8 * s);
+                        }
+                    }
+                    __syncwarp();
+                    if (++s == stages) { s = 0; ph ^= 1u; }
+                }
+            if (!ok && it > 0) mbar_wait_bounded(sfull + 8 * ((it - 1) & 1u), ((it - 1) >> 1) & 1u, p.polls);
+        }
+    } else {
+        const int quad = w & 3, half = w >> 2, row = quad * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * COLS);
+        const uint32_t first_sempty = PAIR ? map_to_cta(sempty, 0) : sempty;
+        uint32_t it = 0;
+        bool dead = false;                            // as in head_few_kernel
+        while (walk.next()) {
+            const int vt = walk.tile / p.token_tiles, mt = walk.tile - vt * p.token_tiles;
+            const int m = mt * 128 * CTAS + rank * 128 + row, v0 = vt * 256 + half * 128;
+            // (weight rows and tokens behind the last one: any scale, their sums are not stored)
+            const float* sw = p.sw + (long long)min(vt * 2 + half, (p.V - 1) / 128) * p.work.blocks;
+            const float* sa = p.sa + m;
+            float next_a = __ldcg(sa + (long long)walk.b0 * p.pitch), next_w = __ldg(sw + walk.b0);
+            uint64_t acc[COLS / 2];
+#pragma unroll
+            for (int i = 0; i < COLS / 2; i++) acc[i] = 0ull;
+            for (int b = walk.b0; b < walk.b1; b++, it++) {
+                const uint32_t buf = it & 1u;
+                const float f = next_a * next_w;
+                if (b + 1 < walk.b1) {
+                    next_a = __ldcg(sa + (long long)(b + 1) * p.pitch);
+                    next_w = __ldg(sw + b + 1);
+                }
+                const uint64_t ff = f2_pack(f, f);
+                if (!dead) dead = !__all_sync(0xffffffffu, wait(sfull + 8 * buf, (it >> 1) & 1u));
+                if (dead) break;
+                tmem_fence_after();
+#pragma unroll
+                for (int c = 0; c < COLS; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(lanes + buf * NT + c, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        acc[c / 2 + i] = f2_fma(f2_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ff, acc[c / 2 + i]);
+                }
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (PAIR) mbar_arrive_cluster(first_sempty + 8 * buf);
+                    else mbar_arrive(sempty + 8 * buf);
+                }
+            }
+            if (!walk.whole()) {
+                float* mine = p.partial + (long long)(2 * (int)blockIdx.x + (walk.b0 == 0)) * 128 * 256 + (long long)half * COLS * 128 + row;
+#pragma unroll
+                for (int i = 0; i < COLS / 2; i++) {
+                    float a, b;
+                    f2_unpack(acc[i], a, b);
+                    mine[(2 * i) * 128] = a;
+                    mine[(2 * i + 1) * 128] = b;
+                }
+                const long long u = (long long)walk.tile * p.work.blocks;
+                const int c0 = p.work.owner(u), c1 = p.work.owner(u + p.work.blocks - 1);
+                // counted for each CTA of a pair apart: they share no row
+                if (!head_last<W * 32>(p, CTAS * c0 + rank, c1 - c0 + 1, &flag)) continue;
+#pragma unroll
+                for (int i = 0; i < COLS / 2; i++) acc[i] = 0ull;
+                for (int c = c0; c <= c1; c++) {
+                    const float* from = p.partial + (long long)(2 * (CTAS * c + rank) + (c == c0)) * 128 * 256 + (long long)half * COLS * 128 + row;
+#pragma unroll
+                    for (int i = 0; i < COLS / 2; i++) {
+                        float a, b;
+                        f2_unpack(acc[i], a, b);
+                        acc[i] = f2_pack(a + __ldcg(from + (2 * i) * 128), b + __ldcg(from + (2 * i + 1) * 128));
+                    }
+                }
+            }
+            if (m < p.M && !dead) head_store<COLS, OUT>((OUT*)p.out + (long long)m * p.ldo + v0, acc, p.V - v0, p.wide_store);
+        }
+    }
+    __syncwarp();
+    tmem_fence_before();
+    __syncthreads();
+    if constexpr (PAIR) {
+        cluster_arrive();
+        cluster_wait();                               // neither CTA leaves while the other's products, copies or arrivals may reach it
+    }
+    tmem_fence_after();
+    if (w == W + 1) {
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -369,12 +854,11 @@ static int head_map(CUtensorMap* m, const void* codes, long long rows, long long
     return e == CUDA_SUCCESS ? RS_OK : host_cuda_fail(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
 }
 
-template <int NT, typename OUT>
-static int head_launch(const CUtensorMap& w, const CUtensorMap& x, const HeadParams& p, int smem, int grid, cudaStream_t stream) {
-    auto kern = head_product_kernel<NT, OUT>;
+template <typename KERN>
+static int head_launch(KERN kern, const CUtensorMap& w, const CUtensorMap& x, const HeadParams& p, int threads, int smem, int grid, int cluster,
+                       cudaStream_t stream, bool (&done)[64]) {
     {
         static std::mutex mu;
-        static bool done[64] = {};      // per device
         int dev = 0;
         cudaError_t e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return host_cuda_fail(e, "cudaGetDevice");
@@ -393,39 +877,76 @@ static int head_launch(const CUtensorMap& w, const CUtensorMap& x, const HeadPar
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
     cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3((NT > 128 ? 8 : 4) * 32 + 64);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = stream;
     // starts while the tokens are still being quantized and waits for them itself
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, w, x, p);
     if (e != cudaSuccess) return host_cuda_fail(e, "cudaLaunchKernelEx(head)");
     host_count_launch();
     return RS_OK;
 }
 template <typename OUT>
-static int head_launch_n(const CUtensorMap& w, const CUtensorMap& x, const HeadParams& p, int smem, int grid, cudaStream_t stream) {
-    if (p.n <= 32) return head_launch<32, OUT>(w, x, p, smem, grid, stream);
-    if (p.n <= 64) return head_launch<64, OUT>(w, x, p, smem, grid, stream);
-    if (p.n <= 128) return head_launch<128, OUT>(w, x, p, smem, grid, stream);
-    return head_launch<256, OUT>(w, x, p, smem, grid, stream);
+static int head_run(const CUtensorMap& w, const CUtensorMap& x, const HeadParams& p, int smem, cudaStream_t stream) {
+    static bool done[3][64] = {};      // per device
+    const int n = p.work.workers;
+    if (p.M <= kFewTokens) return head_launch(head_few_kernel<OUT>, w, x, p, 192, smem, n, 1, stream, done[0]);
+    if (p.M <= 128) return head_launch(head_more_kernel<false, OUT>, w, x, p, 320, smem, n, 1, stream, done[1]);
+    return head_launch(head_more_kernel<true, OUT>, w, x, p, 320, smem, 2 * n, 2, stream, done[2]);
+}
+
+// Pairs of CTAs that the device runs at once.
+static int head_pairs(int* out) {
+    static std::mutex mu;
+    static int known[64] = {};         // per device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return host_cuda_fail(e, "cudaGetDevice");
+    std::lock_guard<std::mutex> lk(mu);
+    if (!known[dev & 63]) {
+        auto kern = head_more_kernel<true, float>;
+        const int smem = 6 * head_more_stage<true>() + 1024;
+        cudaLaunchConfig_t cfg;
+        memset(&cfg, 0, sizeof cfg);
+        cfg.gridDim = dim3(2);
+        cfg.blockDim = dim3(320);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = 2;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        int n = 0;
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+        if (e != cudaSuccess) return host_cuda_fail(e, "cudaOccupancyMaxActiveClusters");
+        known[dev & 63] = n < 1 ? 1 : n;
+    }
+    *out = known[dev & 63];
+    return RS_OK;
 }
 
 template <bool ROWS>
 static int head_quantize(const void* src, int dtype, long long stride, long long rows, long long K, uint8_t* codes, float* scales, int pitch,
-                         cudaStream_t st) {
+                         int* arrived, cudaStream_t st) {
     const int blocks = (int)((K + kHeadBlock - 1) / kHeadBlock);
     const uintptr_t size = dtype == RS_DTYPE_F32 ? 4 : 2;
-    const bool vec = ((uintptr_t)src & (4 * size - 1)) == 0 && stride % 4 == 0;
+    const bool vec = ROWS ? ((uintptr_t)src & (4 * size - 1)) == 0 && stride % 4 == 0 : ((uintptr_t)src & 15) == 0 && stride * size % 16 == 0;
     const long long ctas = ROWS ? (rows * blocks + 7) / 8 : (rows + kHeadBlock - 1) / kHeadBlock * blocks;
     if (ctas > 0x7fffffffLL) return RS_ERR_LIMIT;
     const unsigned grid = (unsigned)ctas;
 #define RS_HEAD_Q(DT, VEC)                                                                                                          \
-    if constexpr (ROWS) head_quantize_rows_kernel<DT, VEC><<<grid, 256, 0, st>>>(src, stride, (int)rows, (int)K, blocks, codes, scales, pitch); \
+    if constexpr (ROWS) head_quantize_rows_kernel<DT, VEC><<<grid, 256, 0, st>>>(src, stride, (int)rows, (int)K, blocks, codes, scales, pitch, arrived, \
+                                                                                2 * kHeadMaxWorkers); \
     else head_quantize_blocks_kernel<DT, VEC><<<grid, 256, 0, st>>>(src, stride, (int)rows, (int)K, blocks, codes, scales)
     if (dtype == RS_DTYPE_F32) { if (vec) { RS_HEAD_Q(RS_DTYPE_F32, true); } else { RS_HEAD_Q(RS_DTYPE_F32, false); } }
     else if (dtype == RS_DTYPE_F16) { if (vec) { RS_HEAD_Q(RS_DTYPE_F16, true); } else { RS_HEAD_Q(RS_DTYPE_F16, false); } }
@@ -439,6 +960,16 @@ static int head_quantize(const void* src, int dtype, long long stride, long long
 
 static bool head_dtype(int d) { return d == RS_DTYPE_F32 || d == RS_DTYPE_F16 || d == RS_DTYPE_BF16; }
 static int head_pitch(long long M) { return (int)((M + 255) / 256 * 256) + 256; }      // a tile's scales never end behind a row
+struct HeadLayout { size_t scales, arrived, partial, total; };
+static HeadLayout head_layout(long long M, long long K) {
+    HeadLayout l;
+    const size_t blocks = (size_t)((K + 127) / 128), n = M <= kFewTokens ? (size_t)(M + 15) / 16 * 16 : 256;
+    l.scales = ((size_t)M * (size_t)K + 255) / 256 * 256;
+    l.arrived = l.scales + blocks * (size_t)head_pitch(M) * 4;
+    l.partial = l.arrived + 2 * kHeadMaxWorkers * 4;
+    l.total = l.partial + (size_t)kHeadMaxWorkers * 2 * 128 * n * 4;
+    return l;
+}
 static int head_check(int64_t rows, int64_t K) {
     if (rows <= 0) return RS_ERR_BATCH;
     if (K <= 0 || K % 16 != 0 || K > RS_HEAD_MAX_K || rows > RS_HEAD_MAX_ROWS) return RS_ERR_LIMIT;
@@ -459,13 +990,12 @@ int rs_head_quantize(const void* weight, int32_t dtype, int64_t V, int64_t K, in
     if (!weight || !codes_device || !scales_device || ((uintptr_t)weight & (size - 1)) || ((uintptr_t)codes_device & 15) || ((uintptr_t)scales_device & 3))
         return RS_ERR_POINTER;
     if (row_stride < 0) return RS_ERR_LIMIT;
-    return head_quantize<false>(weight, dtype, row_stride, V, K, (uint8_t*)codes_device, scales_device, 0, (cudaStream_t)stream);
+    return head_quantize<false>(weight, dtype, row_stride, V, K, (uint8_t*)codes_device, scales_device, 0, nullptr, (cudaStream_t)stream);
 }
 
 size_t rs_head_workspace_bytes(int64_t M, int64_t K) {
     if (rs::head_check(M, K)) return 0;
-    const size_t blocks = (size_t)((K + 127) / 128), codes = ((size_t)M * (size_t)K + 255) / 256 * 256;
-    return codes + blocks * (size_t)rs::head_pitch(M) * 4;
+    return rs::head_layout(M, K).total;
 }
 
 int rs_head_logits(const void* hidden, int32_t hidden_dtype, int64_t M, int64_t K, int64_t hidden_stride, const void* codes_device,
@@ -487,36 +1017,53 @@ int rs_head_logits(const void* hidden, int32_t hidden_dtype, int64_t M, int64_t 
     HeadParams p;
     memset(&p, 0, sizeof p);
     if ((rc = host_status_word(&p.status))) return rc;
-    const size_t code_bytes = ((size_t)M * (size_t)K + 255) / 256 * 256;
-    uint8_t* a = (uint8_t*)workspace_device;
-    float* sa = (float*)(a + code_bytes);
+    const HeadLayout l = head_layout(M, K);
+    uint8_t* ws = (uint8_t*)workspace_device;
+    float* sa = (float*)(ws + l.scales);
     p.sa = sa;
     p.sw = scales_device;
     p.out = out_device;
     p.ldo = out_stride;
     p.M = (int)M;
     p.V = (int)V;
-    p.blocks = (int)((K + 127) / 128);
     p.pitch = head_pitch(M);
-    // tiles of at most 256 tokens, as equal as multiples of 16 allow
-    const long long most = (M + 255) / 256;
-    p.n = (int)(((M + most - 1) / most + 15) / 16 * 16);
-    p.token_tiles = (int)((M + p.n - 1) / p.n);
-    const long long tiles = (V + 127) / 128 * p.token_tiles;
-    if (tiles > 0x7fffffffLL) return RS_ERR_LIMIT;
-    p.tiles = (int)tiles;
-    const int room = dev.smem_optin - 2048 - 1024, per = head_stage_bytes(p.n);
-    p.stages = room / per > kHeadMaxStages ? kHeadMaxStages : room / per;
+    p.partial = (float*)(ws + l.partial);
+    p.arrived = (int*)(ws + l.arrived);
     p.polls = host_wait_polls();
     p.mirror = dev.mirror;
+    const bool few = M <= kFewTokens, pair = M > 128;
+    p.n = few ? (int)((M + 15) / 16 * 16) : 256;
+    p.token_tiles = pair ? (int)((M + 255) / 256) : 1;
+    const int tile_v = few ? 128 : 256;
+    HeadWork& k = p.work;
+    k.blocks = (int)((K + 127) / 128);
+    const long long tiles = (V + tile_v - 1) / tile_v * p.token_tiles;
+    if (tiles > 0x7fffffffLL) return RS_ERR_LIMIT;
+    k.tiles = (int)tiles;
+    k.units = tiles * k.blocks;
+    k.workers = dev.sms < kHeadMaxWorkers ? dev.sms : kHeadMaxWorkers;
+    if (pair) {
+        int pairs = 0;
+        if ((rc = head_pairs(&pairs))) return rc;
+        k.workers = k.workers / 2 < pairs ? k.workers / 2 : pairs;
+    }
+    // Whole tiles where the last round of them wastes little, for what a split tile costs: 256 KB written and read a pair.
+    const long long rounds = (tiles + k.workers - 1) / k.workers;
+    k.split = few || rounds * k.workers * 100 > tiles * 103;
+    if (k.split && k.units < 4LL * k.workers) k.workers = (int)((k.units + 3) / 4);
+    if (!k.split && tiles < k.workers) k.workers = (int)tiles;
+    const int per = few ? head_few_stage(p.n) : pair ? head_more_stage<true>() : head_more_stage<false>(), room = dev.smem_optin - 2048 - 1024;
+    p.stages = room / per > kHeadMaxStages ? kHeadMaxStages : room / per;
+    const uintptr_t step = (uintptr_t)out_device | (uintptr_t)out_stride * os;
+    p.wide_store = step % 32 == 0 ? 32 : step % 16 == 0 ? 16 : 0;
     CUtensorMap w, x;
-    if ((rc = head_map(&w, codes_device, V, K, 128)) || (rc = head_map(&x, a, M, K, p.n))) return rc;
-    if ((rc = head_quantize<true>(hidden, hidden_dtype, hidden_stride, M, K, a, sa, p.pitch, (cudaStream_t)stream))) return rc;
-    const int smem = p.stages * per + 1024, grid = p.tiles < dev.sms ? p.tiles : dev.sms;
+    if ((rc = head_map(&w, codes_device, V, K, few || pair ? 128 : 256)) || (rc = head_map(&x, ws, M, K, few ? p.n : 128))) return rc;
+    if ((rc = head_quantize<true>(hidden, hidden_dtype, hidden_stride, M, K, ws, sa, p.pitch, p.arrived, (cudaStream_t)stream))) return rc;
+    const int smem = p.stages * per + 1024;
     switch (out_dtype) {
-        case RS_DTYPE_F32: return head_launch_n<float>(w, x, p, smem, grid, (cudaStream_t)stream);
-        case RS_DTYPE_F16: return head_launch_n<__half>(w, x, p, smem, grid, (cudaStream_t)stream);
-        default: return head_launch_n<__nv_bfloat16>(w, x, p, smem, grid, (cudaStream_t)stream);
+        case RS_DTYPE_F32: return head_run<float>(w, x, p, smem, (cudaStream_t)stream);
+        case RS_DTYPE_F16: return head_run<__half>(w, x, p, smem, (cudaStream_t)stream);
+        default: return head_run<__nv_bfloat16>(w, x, p, smem, (cudaStream_t)stream);
     }
 }
 
