@@ -302,7 +302,7 @@ struct HeadParams {
     long long ldo;
     HeadWork work;
     int M, V, pitch;
-    int n;                   // few tokens: columns of the accumulator, 16 or 32
+    int n;                   // rows of tokens a stage holds, a multiple of 16
     int token_tiles;         // more tokens: tiles of 128, or of 256 for pairs
     int stages;
     int wide_store;          // more tokens: bytes of a store that the result's rows allow (32, 16, or 0: one by one)
@@ -551,7 +551,12 @@ __global__ void __launch_bounds__(192, 1)
 // Beyond, a pair of CTAs shares a tile of 256 tokens by 256 weight rows: each CTA brings 128 tokens and 128 weight rows, its
 // accumulator holds its 128 tokens by all 256 weight rows, and one thread of the first CTA issues the products of both; the
 // pair reads 64 KB for a unit where two CTAs of their own would read 96 KB.
-template <bool PAIR> __host__ __device__ constexpr int head_more_stage() { return 128 * 128 + (PAIR ? 128 : 256) * 128; }
+constexpr int kMoreAdders = 8, kMoreThreads = kMoreAdders * 32 + 64;      // warps that add, threads of a CTA
+// weights, then tokens; a CTA by itself brings only the `n` rows of tokens that there are (in steps of 16): what the other lanes
+// multiply is whatever lies behind, and nobody looks at their sums.  (The products read 128 rows all the same: behind the last
+// stage lies as much shared memory as they reach beyond it, head_more_tail.)
+__host__ __device__ constexpr int head_more_stage(bool pair, int n) { return (pair ? 128 + 128 : 256 + n) * 128; }
+__host__ __device__ constexpr int head_more_tail(bool pair, int n) { return pair ? 0 : (128 - n) * 128; }
 
 __device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
@@ -635,10 +640,11 @@ __device__ __forceinline__ void head_store(OUT* o, const uint64_t (&acc)[COLS / 
 }
 
 template <bool PAIR, typename OUT>
-__global__ void __launch_bounds__(10 * 32, 1)
+__global__ void __launch_bounds__(kMoreThreads, 1)
     head_more_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ HeadParams p) {
-    constexpr int W = 8, COLS = 128, NT = 256, CTAS = PAIR ? 2 : 1;
-    constexpr uint32_t kTmemCols = 512, kStage = (uint32_t)head_more_stage<PAIR>();
+    constexpr int W = kMoreAdders, COLS = 256 / (W / 4), NT = 256, CTAS = PAIR ? 2 : 1;
+    constexpr uint32_t kTmemCols = 512, kWeights = (PAIR ? 128 : 256) * 128;
+    const uint32_t stage_bytes = (uint32_t)head_more_stage(PAIR, p.n);
     extern __shared__ uint8_t raw_smem[];
     __shared__ uint64_t full_[kHeadMaxStages], empty_[kHeadMaxStages], sfull_[2], sempty_[2];
     __shared__ uint32_t tmem_at;
@@ -690,15 +696,15 @@ __global__ void __launch_bounds__(10 * 32, 1)
             for (int b = walk.b0; b < walk.b1; b++, it++) {
                 if (it >= stages && !__all_sync(0xffffffffu, wait(empty + 8 * s, ph ^ 1u))) { ok = false; break; }
                 if (elect_one()) {
-                    const uint32_t at = base + s * kStage, bar = first_full + 8 * s;
+                    const uint32_t at = base + s * stage_bytes, bar = first_full + 8 * s;
                     if constexpr (PAIR) {
-                        mbar_expect_tx_cluster(bar, kStage);
-                        tma_2d_pair(at, &map_x, b * kHeadBlock, m0, bar);
-                        tma_2d_pair(at + 16384u, &map_w, b * kHeadBlock, v0, bar);
+                        mbar_expect_tx_cluster(bar, stage_bytes);
+                        tma_2d_pair(at, &map_w, b * kHeadBlock, v0, bar);
+                        tma_2d_pair(at + kWeights, &map_x, b * kHeadBlock, m0, bar);
                     } else {
-                        mbar_expect_tx(bar, kStage);
-                        tma_2d(at, &map_x, b * kHeadBlock, m0, bar);
-                        tma_2d(at + 16384u, &map_w, b * kHeadBlock, v0, bar);
+                        mbar_expect_tx(bar, stage_bytes);
+                        tma_2d(at, &map_w, b * kHeadBlock, v0, bar);
+                        tma_2d(at + kWeights, &map_x, b * kHeadBlock, m0, bar);
                     }
                 }
                 __syncwarp();
@@ -726,7 +732,7 @@ __global__ void __launch_bounds__(10 * 32, 1)
                     if (!__all_sync(0xffffffffu, wait(full + 8 * s, ph))) { ok = false; break; }
                     tmem_fence_after();
                     if (elect_one()) {
-                        const uint64_t da = desc + ((s * kStage) >> 4), db = da + (16384u >> 4);
+                        const uint64_t db = desc + ((s * stage_bytes) >> 4), da = db + (kWeights >> 4);
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             if constexpr (PAIR) head_mma_pair(tmem + buf * NT, da + 2 * k, db + 2 * k, idesc, k > 0);
@@ -746,16 +752,16 @@ __global__ void __launch_bounds__(10 * 32, 1)
             if (!ok && it > 0) mbar_wait_bounded(sfull + 8 * ((it - 1) & 1u), ((it - 1) >> 1) & 1u, p.polls);
         }
     } else {
-        const int quad = w & 3, half = w >> 2, row = quad * 32 + lane;
-        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * COLS);
+        const int quad = w & 3, col0 = (w >> 2) * COLS, row = quad * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)col0;
         const uint32_t first_sempty = PAIR ? map_to_cta(sempty, 0) : sempty;
         uint32_t it = 0;
         bool dead = false;                            // as in head_few_kernel
         while (walk.next()) {
             const int vt = walk.tile / p.token_tiles, mt = walk.tile - vt * p.token_tiles;
-            const int m = mt * 128 * CTAS + rank * 128 + row, v0 = vt * 256 + half * 128;
+            const int m = mt * 128 * CTAS + rank * 128 + row, v0 = vt * 256 + col0;
             // (weight rows and tokens behind the last one: any scale, their sums are not stored)
-            const float* sw = p.sw + (long long)min(vt * 2 + half, (p.V - 1) / 128) * p.work.blocks;
+            const float* sw = p.sw + (long long)(min(v0, p.V - 1) / 128) * p.work.blocks;
             const float* sa = p.sa + m;
             float next_a = __ldcg(sa + (long long)walk.b0 * p.pitch), next_w = __ldg(sw + walk.b0);
             uint64_t acc[COLS / 2];
@@ -789,7 +795,7 @@ __global__ void __launch_bounds__(10 * 32, 1)
                 }
             }
             if (!walk.whole()) {
-                float* mine = p.partial + (long long)(2 * (int)blockIdx.x + (walk.b0 == 0)) * 128 * 256 + (long long)half * COLS * 128 + row;
+                float* mine = p.partial + (long long)(2 * (int)blockIdx.x + (walk.b0 == 0)) * 128 * 256 + (long long)col0 * 128 + row;
 #pragma unroll
                 for (int i = 0; i < COLS / 2; i++) {
                     float a, b;
@@ -804,7 +810,7 @@ __global__ void __launch_bounds__(10 * 32, 1)
 #pragma unroll
                 for (int i = 0; i < COLS / 2; i++) acc[i] = 0ull;
                 for (int c = c0; c <= c1; c++) {
-                    const float* from = p.partial + (long long)(2 * (CTAS * c + rank) + (c == c0)) * 128 * 256 + (long long)half * COLS * 128 + row;
+                    const float* from = p.partial + (long long)(2 * (CTAS * c + rank) + (c == c0)) * 128 * 256 + (long long)col0 * 128 + row;
 #pragma unroll
                     for (int i = 0; i < COLS / 2; i++) {
                         float a, b;
@@ -899,8 +905,8 @@ static int head_run(const CUtensorMap& w, const CUtensorMap& x, const HeadParams
     static bool done[3][64] = {};      // per device
     const int n = p.work.workers;
     if (p.M <= kFewTokens) return head_launch(head_few_kernel<OUT>, w, x, p, 192, smem, n, 1, stream, done[0]);
-    if (p.M <= 128) return head_launch(head_more_kernel<false, OUT>, w, x, p, 320, smem, n, 1, stream, done[1]);
-    return head_launch(head_more_kernel<true, OUT>, w, x, p, 320, smem, 2 * n, 2, stream, done[2]);
+    if (p.M <= 128) return head_launch(head_more_kernel<false, OUT>, w, x, p, kMoreThreads, smem, n, 1, stream, done[1]);
+    return head_launch(head_more_kernel<true, OUT>, w, x, p, kMoreThreads, smem, 2 * n, 2, stream, done[2]);
 }
 
 // Pairs of CTAs that the device runs at once.
@@ -913,11 +919,11 @@ static int head_pairs(int* out) {
     std::lock_guard<std::mutex> lk(mu);
     if (!known[dev & 63]) {
         auto kern = head_more_kernel<true, float>;
-        const int smem = 6 * head_more_stage<true>() + 1024;
+        const int smem = 6 * head_more_stage(true, 128) + 1024;
         cudaLaunchConfig_t cfg;
         memset(&cfg, 0, sizeof cfg);
         cfg.gridDim = dim3(2);
-        cfg.blockDim = dim3(320);
+        cfg.blockDim = dim3(kMoreThreads);
         cfg.dynamicSmemBytes = smem;
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeClusterDimension;
@@ -1032,7 +1038,7 @@ int rs_head_logits(const void* hidden, int32_t hidden_dtype, int64_t M, int64_t 
     p.polls = host_wait_polls();
     p.mirror = dev.mirror;
     const bool few = M <= kFewTokens, pair = M > 128;
-    p.n = few ? (int)((M + 15) / 16 * 16) : 256;
+    p.n = pair ? 128 : (int)((M + 15) / 16 * 16);
     p.token_tiles = pair ? (int)((M + 255) / 256) : 1;
     const int tile_v = few ? 128 : 256;
     HeadWork& k = p.work;
@@ -1052,14 +1058,15 @@ int rs_head_logits(const void* hidden, int32_t hidden_dtype, int64_t M, int64_t 
     k.split = few || rounds * k.workers * 100 > tiles * 103;
     if (k.split && k.units < 4LL * k.workers) k.workers = (int)((k.units + 3) / 4);
     if (!k.split && tiles < k.workers) k.workers = (int)tiles;
-    const int per = few ? head_few_stage(p.n) : pair ? head_more_stage<true>() : head_more_stage<false>(), room = dev.smem_optin - 2048 - 1024;
+    const int per = few ? head_few_stage(p.n) : head_more_stage(pair, p.n);
+    const int tail = few ? 0 : head_more_tail(pair, p.n), room = dev.smem_optin - 2048 - 1024 - tail;
     p.stages = room / per > kHeadMaxStages ? kHeadMaxStages : room / per;
     const uintptr_t step = (uintptr_t)out_device | (uintptr_t)out_stride * os;
     p.wide_store = step % 32 == 0 ? 32 : step % 16 == 0 ? 16 : 0;
     CUtensorMap w, x;
-    if ((rc = head_map(&w, codes_device, V, K, few || pair ? 128 : 256)) || (rc = head_map(&x, ws, M, K, few ? p.n : 128))) return rc;
+    if ((rc = head_map(&w, codes_device, V, K, few || pair ? 128 : 256)) || (rc = head_map(&x, ws, M, K, p.n))) return rc;
     if ((rc = head_quantize<true>(hidden, hidden_dtype, hidden_stride, M, K, ws, sa, p.pitch, p.arrived, (cudaStream_t)stream))) return rc;
-    const int smem = p.stages * per + 1024;
+    const int smem = p.stages * per + tail + 1024;
     switch (out_dtype) {
         case RS_DTYPE_F32: return head_run<float>(w, x, p, smem, (cudaStream_t)stream);
         case RS_DTYPE_F16: return head_run<__half>(w, x, p, smem, (cudaStream_t)stream);
