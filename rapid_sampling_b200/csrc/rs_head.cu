@@ -95,23 +95,6 @@ __global__ void __launch_bounds__(256) head_quantize_rows_kernel(const void* src
     if (lane == 0) scales[(long long)b * pitch + m] = s;
 }
 
-// Two fp32 at a time (the compiler does not pair scalar operations by itself).
-__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 // Codes of a pair by div_by's steps (a + b r with -s for the remainders).
 __device__ __forceinline__ uint32_t head_codes2(float a, float b, uint64_t minus_s, uint64_t r) {
     const uint64_t x = f2_pack(a, b);

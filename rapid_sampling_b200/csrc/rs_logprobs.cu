@@ -57,17 +57,45 @@ struct LpParams {
 };
 
 // ---- elements -----------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float max_nan(float a, float b) {      // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 16 bytes of logits: E elements, widened pair by pair.
 template <int DT> struct Elem;
 template <> struct Elem<RS_DTYPE_F32> {
     using T = float;
     static constexpr int E = 4;
     static constexpr uint32_t kNone = 0xFF800000u;      // a word of -inf
-    static __device__ __forceinline__ void wide(const uint4& v, float (&x)[4]) {
-        x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+    static __device__ __forceinline__ void pairs(const uint4& v, uint64_t (&x)[2]) {
+        x[0] = f2_pack(__uint_as_float(v.x), __uint_as_float(v.y));
+        x[1] = f2_pack(__uint_as_float(v.z), __uint_as_float(v.w));
+    }
+    template <int U> static __device__ __forceinline__ float largest(const uint4 (&v)[U]) {      // NaN if any element is
+        float m = __uint_as_float(v[0].x);
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            m = max3_nan(m, __uint_as_float(v[i].x), __uint_as_float(v[i].y));
+            m = max3_nan(m, __uint_as_float(v[i].z), __uint_as_float(v[i].w));
+        }
+        return m;
+    }
+    // elements of at least `from`
+    static __device__ __forceinline__ int reach(const uint4& v, float from) {
+        return (__uint_as_float(v.x) >= from) + (__uint_as_float(v.y) >= from) + (__uint_as_float(v.z) >= from) + (__uint_as_float(v.w) >= from);
     }
     static __device__ __forceinline__ float one(const T* p) { return *p; }
-    static __device__ __forceinline__ uint4 narrow(const float (&x)[4]) {
-        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    static __device__ __forceinline__ uint4 narrow(const uint64_t (&x)[2]) {
+        float a, b, c, d;
+        f2_unpack(x[0], a, b);
+        f2_unpack(x[1], c, d);
+        return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
     }
     static __device__ __forceinline__ T to(float x) { return x; }
 };
@@ -75,21 +103,35 @@ template <> struct Elem<RS_DTYPE_F16> {
     using T = __half;
     static constexpr int E = 8;
     static constexpr uint32_t kNone = 0xFC00FC00u;
-    static __device__ __forceinline__ void wide(const uint4& v, float (&x)[8]) {
+    static __device__ __forceinline__ __half2 h2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+    static __device__ __forceinline__ void pairs(const uint4& v, uint64_t (&x)[4]) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
+            const float2 f = __half22float2(h2(w[i]));
+            x[i] = f2_pack(f.x, f.y);
         }
     }
+    template <int U> static __device__ __forceinline__ float largest(const uint4 (&v)[U]) {
+        __half2 m = h2(v[0].x);
+#pragma unroll
+        for (int i = 0; i < U; i++) m = __hmax2_nan(__hmax2_nan(__hmax2_nan(__hmax2_nan(m, h2(v[i].x)), h2(v[i].y)), h2(v[i].z)), h2(v[i].w));
+        const float2 f = __half22float2(m);
+        return max_nan(f.x, f.y);
+    }
+    static __device__ __forceinline__ int reach(const uint4& v, float from) {      // `from` is a value of the type
+        const __half2 f = __float2half2_rn(from);
+        const __half2 n = __hadd2(__hadd2(__hge2(h2(v.x), f), __hge2(h2(v.y), f)), __hadd2(__hge2(h2(v.z), f), __hge2(h2(v.w), f)));
+        return (int)(__low2float(n) + __high2float(n));
+    }
     static __device__ __forceinline__ float one(const T* p) { return __half2float(*p); }
-    static __device__ __forceinline__ uint4 narrow(const float (&x)[8]) {
+    static __device__ __forceinline__ uint4 narrow(const uint64_t (&x)[4]) {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+            float a, b;
+            f2_unpack(x[i], a, b);
+            const __half2 h = __floats2half2_rn(a, b);
             w[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
@@ -100,36 +142,49 @@ template <> struct Elem<RS_DTYPE_BF16> {
     using T = __nv_bfloat16;
     static constexpr int E = 8;
     static constexpr uint32_t kNone = 0xFF80FF80u;
-    static __device__ __forceinline__ void wide(const uint4& v, float (&x)[8]) {
+    static __device__ __forceinline__ __nv_bfloat162 h2(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
+    static __device__ __forceinline__ void pairs(const uint4& v, uint64_t (&x)[4]) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
+        for (int i = 0; i < 4; i++) x[i] = f2_pack(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+    }
+    template <int U> static __device__ __forceinline__ float largest(const uint4 (&v)[U]) {
+        __nv_bfloat162 m = h2(v[0].x);
+#pragma unroll
+        for (int i = 0; i < U; i++) m = __hmax2_nan(__hmax2_nan(__hmax2_nan(__hmax2_nan(m, h2(v[i].x)), h2(v[i].y)), h2(v[i].z)), h2(v[i].w));
+        return max_nan(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ int reach(const uint4& v, float from) {
+        const __nv_bfloat162 f = __float2bfloat162_rn(from);
+        const __nv_bfloat162 n = __hadd2(__hadd2(__hge2(h2(v.x), f), __hge2(h2(v.y), f)), __hadd2(__hge2(h2(v.z), f), __hge2(h2(v.w), f)));
+        return (int)(__low2float(n) + __high2float(n));
     }
     static __device__ __forceinline__ float one(const T* p) { return __bfloat162float(*p); }
-    static __device__ __forceinline__ uint4 narrow(const float (&x)[8]) {
+    static __device__ __forceinline__ uint4 narrow(const uint64_t (&x)[4]) {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            float a, b;
+            f2_unpack(x[i], a, b);
+            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
             w[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
     static __device__ __forceinline__ T to(float x) { return __float2bfloat16_rn(x); }
 };
+template <int DT>
+__device__ __forceinline__ void widen(const uint4& v, float (&x)[Elem<DT>::E]) {
+    uint64_t p[Elem<DT>::E / 2];
+    Elem<DT>::pairs(v, p);
+#pragma unroll
+    for (int i = 0; i < Elem<DT>::E / 2; i++) f2_unpack(p[i], x[2 * i], x[2 * i + 1]);
+}
 
 __device__ __forceinline__ uint4 ld_stream(const uint4* p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {      // NaN if either is
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
 }
 __device__ __forceinline__ float warp_max_nan(float v) {
     float r;
@@ -150,6 +205,18 @@ __device__ __forceinline__ float of_key(uint32_t k) {
     return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
 }
 constexpr uint32_t kKeyNone = 0x007FFFFFu;      // key of -inf
+// The next larger value of the logits' type; of +inf a NaN, which nothing reaches.
+template <int DT>
+__device__ __forceinline__ float next_above(float x) {
+    constexpr uint32_t kStep = DT == RS_DTYPE_F32 ? 1u : DT == RS_DTYPE_F16 ? 0u : 0x10000u;
+    if constexpr (DT == RS_DTYPE_F16) {
+        const uint32_t u = __half_as_ushort(__float2half_rn(x + 0.0f));
+        return __half2float(__ushort_as_half((unsigned short)(u & 0x8000u ? (u == 0x8001u ? 0u : u - 1u) : u + 1u)));
+    } else {
+        const uint32_t u = __float_as_uint(x + 0.0f);
+        return __uint_as_float(u >> 31 ? (u == 0x80000000u + kStep ? 0u : u - kStep) : u + kStep);
+    }
+}
 
 // ---- one row's position, token and temperature --------------------------------------------------------------------
 struct LpRow {
@@ -192,22 +259,39 @@ __device__ __forceinline__ void stat_raise(Stat& a, float bm, float c) {
     a.u = f * fmaf(d, a.s, a.u);
     a.s *= f;
 }
-template <int N>
-__device__ __forceinline__ void stat_add(Stat& a, const float (&x)[N], float c) {
-    float bm = x[0];
+__device__ __forceinline__ void stat_one(Stat& a, float x, float c) {
+    stat_raise(a, x, c);
+    const float d = fmaxf((x - ref_of(a.mx)) * c, kFloor), e = ex2(d);
+    a.s += e;
+    a.u = fmaf(d, e, a.u);
+}
+// U vectors; the products and sums two at a time.
+template <int DT, int U>
+__device__ __forceinline__ void stat_add(Stat& a, const uint4 (&v)[U], float c) {
+    stat_raise(a, Elem<DT>::largest(v), c);
+    const float m = -ref_of(a.mx);
+    const uint64_t mm = f2_pack(m, m), cc = f2_pack(c, c);
+    uint64_t s = 0ull, u = 0ull;
 #pragma unroll
-    for (int i = 1; i < N; i++) bm = max_nan(bm, x[i]);
-    stat_raise(a, bm, c);
-    const float m = ref_of(a.mx);
-    float s = 0.f, u = 0.f;
+    for (int i = 0; i < U; i++) {
+        uint64_t x[Elem<DT>::E / 2];
+        Elem<DT>::pairs(v[i], x);
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const float d = fmaxf((x[i] - m) * c, kFloor), e = ex2(d);
-        s += e;
-        u = fmaf(d, e, u);
+        for (int k = 0; k < Elem<DT>::E / 2; k++) {
+            float d0, d1;
+            f2_unpack(f2_mul(f2_add(x[k], mm), cc), d0, d1);
+            d0 = fmaxf(d0, kFloor);
+            d1 = fmaxf(d1, kFloor);
+            const uint64_t e = f2_pack(ex2(d0), ex2(d1));
+            s = f2_add(s, e);
+            u = f2_fma(f2_pack(d0, d1), e, u);
+        }
     }
-    a.s += s;
-    a.u += u;
+    float s0, s1, u0, u1;
+    f2_unpack(s, s0, s1);
+    f2_unpack(u, u0, u1);
+    a.s += s0 + s1;
+    a.u += u0 + u1;
 }
 // The lanes' statistics as one, in every lane.  s comes and goes as the excess: the sum without the maximum's own 1 (-1: no
 // element above -inf).  Terms are added in a fixed order.
@@ -297,7 +381,7 @@ __device__ int top_count(const Span<DT>& sp, TopShared& sh, uint32_t at_least) {
     int n = 0;
     for (int v = sp.v0 + (int)threadIdx.x; v < sp.v1; v += kLpThreads) {
         float x[E];
-        Elem<DT>::wide(ld_stream(sp.vec + v), x);
+        widen<DT>(ld_stream(sp.vec + v), x);
 #pragma unroll
         for (int i = 0; i < E; i++) n += key_of(x[i]) >= at_least;
     }
@@ -323,7 +407,7 @@ __device__ void top_exact(const Span<DT>& sp, TopShared& sh, int n) {
     __syncthreads();
     for (int v = sp.v0 + t; v < sp.v1; v += kLpThreads) {
         float x[E];
-        Elem<DT>::wide(ld_stream(sp.vec + v), x);
+        widen<DT>(ld_stream(sp.vec + v), x);
 #pragma unroll
         for (int i = 0; i < E; i++)
             if (key_of(x[i]) > lo) top_push(sh, key_of(x[i]), sp.index(v) + i);
@@ -341,7 +425,7 @@ __device__ void top_exact(const Span<DT>& sp, TopShared& sh, int n) {
         if (have >= n) break;
         if (t < kStep && v + t < sp.v1) {
             float x[E];
-            Elem<DT>::wide(ld_stream(sp.vec + v + t), x);
+            widen<DT>(ld_stream(sp.vec + v + t), x);
 #pragma unroll
             for (int i = 0; i < E; i++)
                 if (key_of(x[i]) == lo) top_push(sh, lo, sp.index(v + t) + i);
@@ -363,20 +447,33 @@ __device__ int top_collect(const Span<DT>& sp, TopShared& sh, float mx, int n) {
     constexpr int E = Elem<DT>::E;
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
     const uint32_t mine = key_of(mx);
-    sh.key[t] = mine;
-    if (t == 0) { sh.nhot = 0; sh.ncand = 0; sh.tau = kKeyNone + 1; }
-    const int finite = __syncthreads_count(mine > kKeyNone);
-    if (finite >= n) {
-        int above = 0, reach = 0;
-#pragma unroll 8
-        for (int i = 0; i < kLpThreads / 4; i++) {
-            const uint4 k = reinterpret_cast<const uint4*>(sh.key)[i];
-            above += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
-            reach += (k.x >= mine) + (k.y >= mine) + (k.z >= mine) + (k.w >= mine);
+    // the n-th largest maximum: every warp sorts its own, a place among the others' by bisection
+    uint32_t k = mine;
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+        for (int step = size / 2; step > 0; step /= 2) {
+            const uint32_t o = __shfl_xor_sync(0xffffffffu, k, step);
+            const bool larger_first = (lane & size) == 0 || size == 32;
+            k = ((lane & step) == 0) == larger_first ? max(k, o) : min(k, o);
         }
-        if (above < n && n <= reach) sh.tau = mine;       // the same value from every thread that writes
-        __syncthreads();
+    sh.key[t] = k;
+    if (t == 0) { sh.nhot = 0; sh.ncand = 0; sh.tau = kKeyNone + 1u; }
+    __syncthreads();
+    if (lane < n) {
+        int rank = lane;
+#pragma unroll
+        for (int o = 0; o < kLpThreads / 32; o++) {
+            if (o == w) continue;
+            const uint32_t* list = sh.key + o * 32, least = o < w ? k : k + 1u;      // equal ones: the lower warp's first
+            int at = 0;
+#pragma unroll
+            for (int step = 16; step > 0; step /= 2) at += list[at + step - 1] >= least ? step : 0;
+            rank += at + (list[at] >= least);
+        }
+        if (rank == n - 1) sh.tau = max(k, kKeyNone + 1u);      // one thread; fewer than n with a logit left: all of those
     }
+    __syncthreads();
     const uint32_t tau = sh.tau;
     if (mine >= tau) {
         const int at = atomicAdd(&sh.nhot, 1);
@@ -389,7 +486,7 @@ __device__ int top_collect(const Span<DT>& sp, TopShared& sh, float mx, int n) {
             const int h = sh.hot[i];
             for (int v = sp.v0 + h + lane * kLpThreads; v < sp.v1; v += 32 * kLpThreads) {
                 float x[E];
-                Elem<DT>::wide(ld_stream(sp.vec + v), x);
+                widen<DT>(ld_stream(sp.vec + v), x);
 #pragma unroll
                 for (int k = 0; k < E; k++)
                     if (key_of(x[k]) >= tau) top_push(sh, key_of(x[k]), sp.index(v) + k);
@@ -434,38 +531,45 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
     const Span<DT> sp(p, row, part, parts);
     const int token = (int)row.token;
     const float xt = Elem<DT>::one(sp.row + token);
-    // rank: an element before the token counts from xt on, one behind it only above
-    const uint32_t kt = key_of(xt);
-    const float xt_above = of_key(kt + 1);
+    // rank: an element before the token counts from xt on, one behind it only from the type's next value on
+    const float xt_above = next_above<DT>(xt);
     int cnt = 0;
 
     Stat a = {-INFINITY, 0.f, 0.f};
     sp.singles(t, [&](int j, float x) {
-        const float one[1] = {x};
-        stat_add(a, one, c);
+        stat_one(a, x, c);
         if (TOP) cnt += j < token ? x >= xt : x > xt;
     });
-    for (int v = sp.v0 + t; v < sp.v1; v += kLpAhead * kLpThreads) {
-        uint4 raw[kLpAhead];
+    // the next vectors are on their way while these are added
+    uint4 raw[2][kLpAhead];
+    auto load = [&](uint4 (&to)[kLpAhead], int v) {
 #pragma unroll
         for (int i = 0; i < kLpAhead; i++) {
             const int at = v + i * kLpThreads;
-            raw[i] = at < sp.v1 ? ld_stream(sp.vec + at) : make_uint4(Elem<DT>::kNone, Elem<DT>::kNone, Elem<DT>::kNone, Elem<DT>::kNone);
+            to[i] = at < sp.v1 ? ld_stream(sp.vec + at) : make_uint4(Elem<DT>::kNone, Elem<DT>::kNone, Elem<DT>::kNone, Elem<DT>::kNone);
         }
-        float x[kLpAhead * E];
+    };
+    auto add = [&](const uint4 (&from)[kLpAhead], int v) {
+        stat_add<DT>(a, from, c);
+        if (TOP) {
 #pragma unroll
-        for (int i = 0; i < kLpAhead; i++) {
-            float y[E];
-            Elem<DT>::wide(raw[i], y);
-#pragma unroll
-            for (int k = 0; k < E; k++) x[i * E + k] = y[k];
-            if (TOP) {
-                const float from = sp.index(v + i * kLpThreads) < token ? xt : xt_above;
-#pragma unroll
-                for (int k = 0; k < E; k++) cnt += y[k] >= from;
+            for (int i = 0; i < kLpAhead; i++) {
+                const int at = v + i * kLpThreads;       // (a place behind the part holds -inf: nothing to count)
+                cnt += Elem<DT>::reach(from[i], at >= sp.v1 ? INFINITY : sp.index(at) < token ? xt : xt_above);
             }
         }
-        stat_add(a, x, c);
+    };
+    constexpr int kStep = kLpAhead * kLpThreads;
+    int v = sp.v0 + t;
+    if (v < sp.v1) load(raw[0], v);
+    while (v < sp.v1) {
+        if (v + kStep < sp.v1) load(raw[1], v + kStep);
+        add(raw[0], v);
+        v += kStep;
+        if (v >= sp.v1) break;
+        if (v + kStep < sp.v1) load(raw[0], v + kStep);
+        add(raw[1], v);
+        v += kStep;
     }
     const float my_mx = a.mx;
     a.s -= 1.f;
@@ -500,6 +604,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
         for (int i = t; i < nc; i += kLpThreads) {
             const unsigned long long e = top.cand[i];
             int at = 0;
+#pragma unroll 8
             for (int q = 0; q < nc; q++) at += top.cand[q] > e;
             if (at < n) st_cluster_u64(map_to_cta(smem_addr(&top.list[part * kTopMax + at]), 0), e);
         }
@@ -553,9 +658,16 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
             if (k >= top.list_n[q]) continue;
             const unsigned long long e = top.list[q * kTopMax + k];
             int at = k;                                   // the lists are in order: larger ones of its own come before
-            for (int o = 0; o < parts; o++)
-                if (o != q)
-                    for (int z = 0, zn = top.list_n[o]; z < zn && top.list[o * kTopMax + z] > e; z++) at++;
+            for (int o = 0; o < parts; o++) {
+                if (o == q) continue;
+                const unsigned long long* list = top.list + o * kTopMax;
+                int lo = 0, hi = top.list_n[o];           // entries above e
+                while (lo < hi) {
+                    const int mid = (lo + hi) / 2;
+                    if (list[mid] > e) lo = mid + 1; else hi = mid;
+                }
+                at += lo;
+            }
             if (at < n && !bad) {
                 p.top[r * n + at] = (of_key((uint32_t)(e >> 32)) - mx) * row.inv_t - logs;
                 p.top_ids[r * n + at] = (int)~(uint32_t)e;
@@ -569,8 +681,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
 }
 
 // ---- gradient -------------------------------------------------------------------------------------------------------
-// One element per step of arithmetic: with d = (x - m) c - log2 s, p = 2^d:  p (A + D d), plus g/T at the token itself,
-// where the two are taken together as -expm1(log p) so that a token of probability nearly one keeps its digits.
+// With d = (x - m) c - log2 s, p = 2^d, every element is p (A + D d); the token's own also has g/T, and the two are taken together
+// as -expm1(log p) so that a token of probability nearly one keeps its digits.  Logits and gradient pass once.
 template <int DT>
 __global__ void __launch_bounds__(kLpThreads, 4) lp_backward_kernel(const __grid_constant__ LpParams p) {
     constexpr int E = Elem<DT>::E;
@@ -580,55 +692,65 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_backward_kernel(const __grid
     const LpRow row = lp_row(p, r);
     const Span<DT> sp(p, row, part, p.chunks);
     T* const out = (T*)p.grad + r * p.V;
+    const bool together = (((uintptr_t)(out + sp.head)) & 15) == 0;      // logits and gradient: 16-byte boundaries at the same elements
+    const float2 st = p.stats[r];
+    uint4* const vec = reinterpret_cast<uint4*>(out + sp.head);
+    if (row.token < 0 || row.bad_token || st.x == -INFINITY) {
+        const T zero = Elem<DT>::to(0.f);
+        sp.singles(t, [&](int j, float) { out[j] = zero; });
+        if (together) {
+            for (int v = sp.v0 + t; v < sp.v1; v += kLpThreads) __stcs(vec + v, make_uint4(0u, 0u, 0u, 0u));
+        } else {
+            for (int j = sp.index(sp.v0) + t, j1 = sp.index(sp.v1); j < j1; j += kLpThreads) out[j] = zero;
+        }
+        return;
+    }
     const float g = p.g_logprob ? p.g_logprob[row.b * p.gl_sb + row.t * p.gl_st] : 0.f;
     const float h = p.g_entropy ? p.g_entropy[row.b * p.ge_sb + row.t * p.ge_st] : 0.f;
-    float2 st = p.stats[r];
-    const bool off = row.token < 0 || row.bad_token || st.x == -INFINITY;
-    const float nan = __int_as_float(0x7FC00000);
-    const float m = ref_of(st.x), c = row.c, H = p.entropy[r];
-    float A = -(g + h * H) * row.inv_t, D = -h * row.inv_t * 0.6931471805599453f;
-    if (!(st.x < INFINITY)) A = nan;
-    const int token = off ? -1 : (int)row.token;
+    const float nan = __int_as_float(0x7FC00000), m = ref_of(st.x), c = row.c, H = p.entropy[r], kLn2 = 0.6931471805599453f;
+    const float A = st.x < INFINITY ? -(g + h * H) * row.inv_t : nan, D = -h * row.inv_t * kLn2;
+    const int token = (int)row.token;
     auto grad = [&](float x) {
-        const float d = fmaxf(fmaf(x - m, c, -st.y), kFloor), e = ex2(d);
-        return e * fmaf(D, d, A);
+        const float d = fmaxf(fmaf(x - m, c, -st.y), kFloor);
+        return ex2(d) * fmaf(D, d, A);
     };
     auto grad_at = [&](float x) {      // the token's own
-        const float d = fmaxf(fmaf(x - m, c, -st.y), kFloor), e = ex2(d);
-        const float q = -expm1f(fmaxf((x - m) * row.inv_t - st.y * 0.6931471805599453f, -1e4f));
-        const float v = g * row.inv_t * q + e * fmaf(D, d, -h * H * row.inv_t);
+        const float d = fmaxf(fmaf(x - m, c, -st.y), kFloor);
+        const float q = -expm1f(fmaxf((x - m) * row.inv_t - st.y * kLn2, -1e4f));
+        const float v = g * row.inv_t * q + ex2(d) * fmaf(D, d, -h * H * row.inv_t);
         return st.x < INFINITY ? v : nan;
     };
-    const bool together = (((uintptr_t)(out + sp.head)) & 15) == 0;
-    sp.singles(t, [&](int j, float x) { out[j] = Elem<DT>::to(off ? 0.f : j == token ? grad_at(x) : grad(x)); });
+    sp.singles(t, [&](int j, float x) { out[j] = Elem<DT>::to(j == token ? grad_at(x) : grad(x)); });
     if (together) {
+        const uint64_t mm = f2_pack(-m, -m), cc = f2_pack(c, c), ll = f2_pack(-st.y, -st.y), AA = f2_pack(A, A), DD = f2_pack(D, D);
+        const int own = token >= sp.head && token < sp.tail() ? (token - sp.head) / E : -1;      // the vector that holds the token
         for (int v = sp.v0 + t; v < sp.v1; v += kLpAhead * kLpThreads) {
             uint4 raw[kLpAhead];
 #pragma unroll
+            for (int i = 0; i < kLpAhead; i++)
+                if (v + i * kLpThreads < sp.v1) raw[i] = ld_stream(sp.vec + v + i * kLpThreads);
+#pragma unroll
             for (int i = 0; i < kLpAhead; i++) {
                 const int at = v + i * kLpThreads;
-                raw[i] = at < sp.v1 && !off ? ld_stream(sp.vec + at) : make_uint4(0u, 0u, 0u, 0u);
-            }
+                if (at >= sp.v1) break;
+                uint64_t x[E / 2];
+                Elem<DT>::pairs(raw[i], x);
 #pragma unroll
-            for (int i = 0; i < kLpAhead; i++) {
-                const int at = v + i * kLpThreads, j0 = sp.index(at);
-                float x[E];
-                Elem<DT>::wide(raw[i], x);
-                if ((unsigned)(token - j0) < (unsigned)E) {
-#pragma unroll
-                    for (int k = 0; k < E; k++) x[k] = j0 + k == token ? grad_at(x[k]) : grad(x[k]);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < E; k++) x[k] = grad(x[k]);
+                for (int k = 0; k < E / 2; k++) {
+                    float d0, d1;
+                    f2_unpack(f2_fma(f2_add(x[k], mm), cc, ll), d0, d1);
+                    d0 = fmaxf(d0, kFloor);
+                    d1 = fmaxf(d1, kFloor);
+                    x[k] = f2_mul(f2_pack(ex2(d0), ex2(d1)), f2_fma(DD, f2_pack(d0, d1), AA));
                 }
-                if (at < sp.v1) __stcs(reinterpret_cast<uint4*>(out + sp.head) + at, off ? make_uint4(0u, 0u, 0u, 0u) : Elem<DT>::narrow(x));
+                __stcs(vec + at, Elem<DT>::narrow(x));
+                if (at == own) out[token] = Elem<DT>::to(grad_at(Elem<DT>::one(sp.row + token)));      // behind the vector's store, by the same thread
             }
         }
-    } else {                           // logits and gradient start at different places of their 16 bytes: element by element
-        const int j1 = sp.index(sp.v1);
-        for (int j = sp.index(sp.v0) + t; j < j1; j += kLpThreads) {
-            const float x = off ? 0.f : Elem<DT>::one(sp.row + j);
-            out[j] = Elem<DT>::to(off ? 0.f : j == token ? grad_at(x) : grad(x));
+    } else {                           // they start at different places of their 16 bytes: element by element
+        for (int j = sp.index(sp.v0) + t, j1 = sp.index(sp.v1); j < j1; j += kLpThreads) {
+            const float x = Elem<DT>::one(sp.row + j);
+            out[j] = Elem<DT>::to(j == token ? grad_at(x) : grad(x));
         }
     }
 }

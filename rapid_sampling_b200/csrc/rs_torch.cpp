@@ -275,9 +275,11 @@ static void check_logprobs(int rc) {
     if (rc != RS_OK) fail(rc, "");
 }
 
-// (log probabilities, entropies, statistics for the backward call or None)
-static pybind11::tuple token_logprobs(const at::Tensor& logits, const at::Tensor& tokens, double temperature,
-                                      const c10::optional<at::Tensor>& row_temperature, bool keep_stats) {
+struct Logprobs {
+    at::Tensor logprobs, entropy, stats;      // stats: for the backward call, or undefined
+};
+static Logprobs token_logprobs_run(const at::Tensor& logits, const at::Tensor& tokens, double temperature,
+                                   const c10::optional<at::Tensor>& row_temperature, bool keep_stats) {
     rs_logprob_call c = logprob_call(logits, tokens, temperature, row_temperature);
     c10::cuda::CUDAGuard guard(logits.device());
     raise_pending_logprobs(logits.get_device(), (cudaStream_t)c.stream);
@@ -286,7 +288,7 @@ static pybind11::tuple token_logprobs(const at::Tensor& logits, const at::Tensor
     if (keep_stats) stats = at::empty({c.B, c.T, 2}, f32);
     if (lp.numel() > 0)
         check_logprobs(rs_token_logprobs(&c, lp.data_ptr<float>(), ent.data_ptr<float>(), keep_stats ? stats.data_ptr<float>() : nullptr));
-    return pybind11::make_tuple(lp, ent, keep_stats ? pybind11::cast(stats) : pybind11::none());
+    return {lp, ent, stats};
 }
 
 static at::Tensor token_logprobs_backward(const at::Tensor& logits, const at::Tensor& tokens, double temperature,
@@ -316,6 +318,48 @@ static at::Tensor token_logprobs_backward(const at::Tensor& logits, const at::Te
         check_logprobs(rs_token_logprobs_backward(&c, entropy.data_ptr<float>(), stats.data_ptr<float>(), g[0], s[0][0], s[0][1], g[1],
                                                   s[1][0], s[1][1], grad.data_ptr()));
     return grad;
+}
+
+struct RowTemperature {      // no input of the graph
+    c10::optional<at::Tensor> t;
+};
+class TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
+  public:
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& tokens,
+                                                  double temperature, const RowTemperature& rows) {
+        Logprobs r = token_logprobs_run(logits, tokens, temperature, rows.t, true);
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["temperature"] = temperature;
+        torch::autograd::variable_list keep = {logits, tokens, r.entropy, r.stats};
+        if (rows.t.has_value()) keep.push_back(*rows.t);
+        ctx->save_for_backward(std::move(keep));
+        return {r.logprobs, r.entropy};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+        if (at::GradMode::is_enabled()) throw std::runtime_error("batch_token_logprobs is differentiable once: no create_graph !\n");
+        const auto saved = ctx->get_saved_variables();
+        at::Tensor grad;
+        if (g[0].defined() || g[1].defined()) {
+            auto maybe = [](const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
+            grad = token_logprobs_backward(saved[0], saved[1], ctx->saved_data["temperature"].toDouble(),
+                                           saved.size() > 4 ? c10::optional<at::Tensor>(saved[4]) : c10::nullopt, saved[2], saved[3], maybe(g[0]),
+                                           maybe(g[1]));
+        }
+        return {grad, at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+// (log probabilities, entropies); part of the autograd graph where the logits are
+static pybind11::tuple token_logprobs(const at::Tensor& logits, const at::Tensor& tokens, double temperature,
+                                      const c10::optional<at::Tensor>& row_temperature) {
+    if (row_temperature.has_value() && row_temperature->requires_grad())
+        throw std::invalid_argument("the temperature is not differentiated: it must not require a gradient !\n");
+    if (logits.requires_grad() && at::GradMode::is_enabled()) {
+        const auto r = TokenLogprobs::apply(logits, tokens, temperature, RowTemperature{row_temperature});
+        return pybind11::make_tuple(r[0], r[1]);
+    }
+    const Logprobs r = token_logprobs_run(logits, tokens, temperature, row_temperature, false);
+    return pybind11::make_tuple(r.logprobs, r.entropy);
 }
 
 // (log probabilities, ranks, entropies, top log probabilities, top ids); the first two None without tokens
@@ -439,10 +483,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("top_k") = py::none(), py::arg("top_p") = py::none(), py::arg("penalties") = py::none(),
           py::arg("presence_penalty") = 0.0, py::arg("repetition_penalty") = 0.0, py::arg("penalty_decay") = 0.0,
           py::arg("return_prob") = false);
-    m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("tokens"), py::arg("temperature"), py::arg("row_temperature"),
-          py::arg("keep_stats"));
-    m.def("token_logprobs_backward", &token_logprobs_backward, py::arg("logits"), py::arg("tokens"), py::arg("temperature"),
-          py::arg("row_temperature"), py::arg("entropy"), py::arg("stats"), py::arg("g_logprob"), py::arg("g_entropy"));
+    m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("tokens"), py::arg("temperature"), py::arg("row_temperature"));
     m.def("top_logprobs", &top_logprobs, py::arg("logits"), py::arg("top_n"), py::arg("tokens"), py::arg("temperature"),
           py::arg("row_temperature"));
     m.def("lm_head_quantize", &lm_head_quantize, py::arg("weight"));

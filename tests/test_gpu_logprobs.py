@@ -117,6 +117,25 @@ def test_masks(dtype):
     check_all(x, t, 100.0, top_n=20)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_masked_tokens_of_rows_shared_by_several_ctas(dtype):
+    """A masked token's rank counts every other id that is masked and lies before it, and nothing else."""
+    x, t = make((3,), 70003, dtype, 23)
+    x[:, 30000:60001] = -math.inf
+    t[:] = torch.tensor([30000, 45679, 60000], device="cuda")
+    x[2] = -math.inf
+    check_all(x, t, 1.0, top_n=20)
+
+
+def test_a_second_derivative_is_refused():
+    import rapid_sampling_b200 as rs
+    x, t = make((2,), 100, "f32", 24)
+    leaf = x.requires_grad_(True)
+    lp, _ = rs.batch_token_logprobs(leaf, t)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(lp.sum(), leaf, create_graph=True)
+
+
 def test_not_finite_rows():
     x, t = make((6,), 2050, "f32", 9)
     x[1, 5] = math.nan
