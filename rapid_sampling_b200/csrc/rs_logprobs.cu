@@ -53,7 +53,7 @@ struct LpParams {
     const float *g_logprob, *g_entropy;
     long long gl_sb, gl_st, ge_sb, ge_st;
     void* grad;                        // (rows, V) contiguous
-    int chunks;                        // CTAs per row
+    int chunks, piece;                 // CTAs per row, vectors of each
 };
 
 // ---- elements -----------------------------------------------------------------------------------------------------
@@ -224,10 +224,11 @@ struct LpRow {
     float inv_t, c;             // 1 / T, log2(e) / T
     bool bad_token, bad_temperature;
 };
-__device__ __forceinline__ LpRow lp_row(const LpParams& p, long long r) {
+__device__ __forceinline__ LpRow lp_row(const LpParams& p, uint32_t r) {
     LpRow o;
-    o.b = r / p.T;
-    o.t = r - o.b * p.T;
+    const uint32_t b = r / (uint32_t)p.T;
+    o.b = b;
+    o.t = r - b * (uint32_t)p.T;
     o.token = 0;
     if (p.tokens) {
         const long long at = o.b * p.tok_sb + o.t * p.tok_st;
@@ -321,7 +322,7 @@ struct Span {
     int head, nvec, V;       // of the row
     int v0, v1;              // this CTA's vectors
     bool first, last;
-    __device__ __forceinline__ Span(const LpParams& p, const LpRow& w, int part, int parts) {
+    __device__ __forceinline__ Span(const LpParams& p, const LpRow& w) {
         constexpr int E = Elem<DT>::E;
         row = (const T*)p.logits + w.b * p.sb + w.t * p.st;
         V = p.V;
@@ -329,8 +330,16 @@ struct Span {
         if (head > V) head = V;
         nvec = (V - head) / E;
         vec = reinterpret_cast<const uint4*>(row + head);
-        v0 = (int)((long long)nvec * part / parts);
-        v1 = (int)((long long)nvec * (part + 1) / parts);
+    }
+    __device__ __forceinline__ void share(int part, int log_parts) {      // one of 2^log_parts equal parts
+        v0 = (int)(((long long)nvec * part) >> log_parts);
+        v1 = (int)(((long long)nvec * (part + 1)) >> log_parts);
+        first = part == 0;
+        last = part == (1 << log_parts) - 1;
+    }
+    __device__ __forceinline__ void piece(int part, int size, int parts) {      // `size` vectors, the last part the rest
+        v0 = min(part * size, nvec);
+        v1 = part == parts - 1 ? nvec : min(v0 + size, nvec);
         first = part == 0;
         last = part == parts - 1;
     }
@@ -482,17 +491,29 @@ __device__ int top_collect(const Span<DT>& sp, TopShared& sh, float mx, int n) {
     __syncthreads();
     const int nhot = sh.nhot;
     if (nhot <= kTopHot) {
-        for (int i = w; i < nhot; i += kLpThreads / 32) {
-            const int h = sh.hot[i];
-            for (int v = sp.v0 + h + lane * kLpThreads; v < sp.v1; v += 32 * kLpThreads) {
-                float x[E];
-                widen<DT>(ld_stream(sp.vec + v), x);
+        // all (hot thread, vector) pairs spread over the CTA, four loads ahead
+        const int each = (sp.v1 - sp.v0 + kLpThreads - 1) / kLpThreads, lg = 32 - __clz(max(each, 1) - 1), pairs = nhot << lg;
+        for (int i0 = t; i0 < pairs; i0 += 4 * kLpThreads) {
+            uint4 raw[4];
+            int at[4];
 #pragma unroll
-                for (int k = 0; k < E; k++)
-                    if (key_of(x[k]) >= tau) top_push(sh, key_of(x[k]), sp.index(v) + k);
+            for (int q = 0; q < 4; q++) {
+                const int i = i0 + q * kLpThreads;
+                at[q] = sp.v1;
+                if (i < pairs) at[q] = sp.v0 + sh.hot[i >> lg] + (i & ((1 << lg) - 1)) * kLpThreads;
+                if (at[q] < sp.v1) raw[q] = ld_stream(sp.vec + at[q]);
             }
-            if (lane == 0) sp.singles(h, [&](int j, float x) { if (key_of(x) >= tau) top_push(sh, key_of(x), j); });
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if (at[q] >= sp.v1) continue;
+                float x[E];
+                widen<DT>(raw[q], x);
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (key_of(x[e]) >= tau) top_push(sh, key_of(x[e]), sp.index(at[q]) + e);
+            }
         }
+        if (t < nhot) sp.singles(sh.hot[t], [&](int j, float x) { if (key_of(x) >= tau) top_push(sh, key_of(x), j); });
         __syncthreads();
     }
     if (nhot > kTopHot || sh.ncand > kTopCap) top_exact(sp, sh, n);
@@ -501,14 +522,14 @@ __device__ int top_collect(const Span<DT>& sp, TopShared& sh, float mx, int n) {
 
 // One cluster of gridDim.x / rows CTAs per row (one CTA: no cluster).  Bound by HBM for many rows, by latency for few.
 template <int DT, bool TOP>
-__global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_constant__ LpParams p, int parts) {
+__global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_constant__ LpParams p, int log_parts) {
     constexpr int E = Elem<DT>::E;
     __shared__ LpShared sh;
     __shared__ typename std::conditional<TOP, TopShared, int>::type top;
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-    const int part = parts > 1 ? (int)cluster_ctarank() : 0;
-    const long long r = parts > 1 ? (long long)blockIdx.x / parts : (long long)blockIdx.x;
-    const LpRow row = lp_row(p, r);
+    const int parts = 1 << log_parts, part = parts > 1 ? (int)cluster_ctarank() : 0;
+    const long long r = blockIdx.x >> log_parts;
+    const LpRow row = lp_row(p, (uint32_t)r);
     if (row.token < 0 || row.bad_token) {         // not scored: the same for the whole cluster
         if (part == 0) {
             const float v = row.bad_token ? __int_as_float(0x7FC00000) : 0.f;
@@ -528,7 +549,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
     }
     if (parts > 1) cluster_arrive();
     const float c = row.c;
-    const Span<DT> sp(p, row, part, parts);
+    Span<DT> sp(p, row);
+    sp.share(part, log_parts);
     const int token = (int)row.token;
     const float xt = Elem<DT>::one(sp.row + token);
     // rank: an element before the token counts from xt on, one behind it only from the type's next value on
@@ -653,24 +675,33 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
         const bool bad = !(mx < INFINITY);
         int total = 0;
         for (int q = 0; q < parts; q++) total += top.list_n[q];
-        for (int i = t; i < parts * n; i += kLpThreads) {
-            const int q = i / n, k = i - q * n;
-            if (k >= top.list_n[q]) continue;
-            const unsigned long long e = top.list[q * kTopMax + k];
-            int at = k;                                   // the lists are in order: larger ones of its own come before
-            for (int o = 0; o < parts; o++) {
-                if (o == q) continue;
-                const unsigned long long* list = top.list + o * kTopMax;
-                int lo = 0, hi = top.list_n[o];           // entries above e
-                while (lo < hi) {
-                    const int mid = (lo + hi) / 2;
-                    if (list[mid] > e) lo = mid + 1; else hi = mid;
-                }
-                at += lo;
-            }
+        auto put = [&](unsigned long long e, int at) {
             if (at < n && !bad) {
                 p.top[r * n + at] = (of_key((uint32_t)(e >> 32)) - mx) * row.inv_t - logs;
                 p.top_ids[r * n + at] = (int)~(uint32_t)e;
+            }
+        };
+        if (parts == 1) {
+            if (t < total) put(top.list[t], t);      // in order already
+        } else {
+            // every list's first ceil(n / parts) entries are n in all: what lies below the least of those is not among the n largest
+            const int share = (n + parts - 1) >> log_parts;
+            unsigned long long least = ~0ull;
+            for (int q = 0; q < parts; q++) least = min(least, top.list_n[q] >= share ? top.list[q * kTopMax + share - 1] : 0ull);
+            if (t == 0) top.ncand = 0;
+            __syncthreads();
+            for (int i = t; i < parts * kTopMax; i += kLpThreads) {
+                const int q = i / kTopMax, k = i % kTopMax;
+                if (k < top.list_n[q] && top.list[i] >= least) top.cand[atomicAdd(&top.ncand, 1)] = top.list[i];
+            }
+            __syncthreads();
+            const int nc = top.ncand;
+            for (int i = t; i < nc; i += kLpThreads) {
+                const unsigned long long e = top.cand[i];
+                int at = 0;
+#pragma unroll 8
+                for (int q = 0; q < nc; q++) at += top.cand[q] > e;
+                put(e, at);
             }
         }
         if (t < n && (bad || t >= total)) {
@@ -687,10 +718,12 @@ template <int DT>
 __global__ void __launch_bounds__(kLpThreads, 4) lp_backward_kernel(const __grid_constant__ LpParams p) {
     constexpr int E = Elem<DT>::E;
     using T = typename Elem<DT>::T;
-    const long long r = blockIdx.x / (unsigned)p.chunks;
-    const int part = (int)(blockIdx.x - r * p.chunks), t = threadIdx.x;
-    const LpRow row = lp_row(p, r);
-    const Span<DT> sp(p, row, part, p.chunks);
+    const uint32_t r32 = blockIdx.x / (unsigned)p.chunks;
+    const int part = (int)(blockIdx.x - r32 * (unsigned)p.chunks), t = threadIdx.x;
+    const long long r = r32;
+    const LpRow row = lp_row(p, r32);
+    Span<DT> sp(p, row);
+    sp.piece(part, p.piece, p.chunks);
     T* const out = (T*)p.grad + r * p.V;
     const bool together = (((uintptr_t)(out + sp.head)) & 15) == 0;      // logits and gradient: 16-byte boundaries at the same elements
     const float2 st = p.stats[r];
@@ -723,30 +756,31 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_backward_kernel(const __grid
     sp.singles(t, [&](int j, float x) { out[j] = Elem<DT>::to(j == token ? grad_at(x) : grad(x)); });
     if (together) {
         const uint64_t mm = f2_pack(-m, -m), cc = f2_pack(c, c), ll = f2_pack(-st.y, -st.y), AA = f2_pack(A, A), DD = f2_pack(D, D);
-        const int own = token >= sp.head && token < sp.tail() ? (token - sp.head) / E : -1;      // the vector that holds the token
-        for (int v = sp.v0 + t; v < sp.v1; v += kLpAhead * kLpThreads) {
+        auto one = [&](const uint4& from, int at) {
+            uint64_t x[E / 2];
+            Elem<DT>::pairs(from, x);
+#pragma unroll
+            for (int k = 0; k < E / 2; k++) {
+                float d0, d1;
+                f2_unpack(f2_fma(f2_add(x[k], mm), cc, ll), d0, d1);
+                d0 = fmaxf(d0, kFloor);
+                d1 = fmaxf(d1, kFloor);
+                x[k] = f2_mul(f2_pack(ex2(d0), ex2(d1)), f2_fma(DD, f2_pack(d0, d1), AA));
+            }
+            __stcs(vec + at, Elem<DT>::narrow(x));
+        };
+        int v = sp.v0 + t;
+        for (; v + (kLpAhead - 1) * kLpThreads < sp.v1; v += kLpAhead * kLpThreads) {
             uint4 raw[kLpAhead];
 #pragma unroll
-            for (int i = 0; i < kLpAhead; i++)
-                if (v + i * kLpThreads < sp.v1) raw[i] = ld_stream(sp.vec + v + i * kLpThreads);
+            for (int i = 0; i < kLpAhead; i++) raw[i] = ld_stream(sp.vec + v + i * kLpThreads);
 #pragma unroll
-            for (int i = 0; i < kLpAhead; i++) {
-                const int at = v + i * kLpThreads;
-                if (at >= sp.v1) break;
-                uint64_t x[E / 2];
-                Elem<DT>::pairs(raw[i], x);
-#pragma unroll
-                for (int k = 0; k < E / 2; k++) {
-                    float d0, d1;
-                    f2_unpack(f2_fma(f2_add(x[k], mm), cc, ll), d0, d1);
-                    d0 = fmaxf(d0, kFloor);
-                    d1 = fmaxf(d1, kFloor);
-                    x[k] = f2_mul(f2_pack(ex2(d0), ex2(d1)), f2_fma(DD, f2_pack(d0, d1), AA));
-                }
-                __stcs(vec + at, Elem<DT>::narrow(x));
-                if (at == own) out[token] = Elem<DT>::to(grad_at(Elem<DT>::one(sp.row + token)));      // behind the vector's store, by the same thread
-            }
+            for (int i = 0; i < kLpAhead; i++) one(raw[i], v + i * kLpThreads);
         }
+        for (; v < sp.v1; v += kLpThreads) one(ld_stream(sp.vec + v), v);
+        // the token's own, behind the store of its vector by the same thread
+        const int own = token >= sp.head && token < sp.tail() ? (token - sp.head) / E : -1;
+        if (own >= sp.v0 && own < sp.v1 && (own - sp.v0) % kLpThreads == t) out[token] = Elem<DT>::to(grad_at(Elem<DT>::one(sp.row + token)));
     } else {                           // they start at different places of their 16 bytes: element by element
         for (int j = sp.index(sp.v0) + t, j1 = sp.index(sp.v1); j < j1; j += kLpThreads) {
             const float x = Elem<DT>::one(sp.row + j);
@@ -807,6 +841,7 @@ static int lp_launch(const LpParams& p, int parts, cudaStream_t stream) {
     }
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
+    const int log_parts = 31 - __builtin_clz((unsigned)parts);
     cfg.gridDim = dim3((unsigned)(p.rows * parts));
     cfg.blockDim = dim3(kLpThreads);
     cfg.stream = stream;
@@ -816,7 +851,7 @@ static int lp_launch(const LpParams& p, int parts, cudaStream_t stream) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;      // a cluster of one too: its shared memory is addressed as the cluster's
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, parts);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, log_parts);
     if (e != cudaSuccess) return host_cuda_fail(e, "cudaLaunchKernelEx(logprobs)");
     host_count_launch();
     return RS_OK;
@@ -893,10 +928,13 @@ int rs_token_logprobs_backward(const rs_logprob_call* call, const float* entropy
     p.ge_sb = ge_stride_b;
     p.ge_st = ge_stride_t;
     p.grad = grad_device;
-    // about 16 KB of logits a CTA, fewer where the grid would pass what a launch takes
-    const long long bytes = p.V * (long long)size;
-    long long chunks = (bytes + 16383) / 16384;
-    while (chunks > 1 && p.rows * chunks > 0x7fffffffLL) chunks = (chunks + 1) / 2;
+    // 64 KB of logits a CTA, so that its row's few numbers cost little; down to 8 KB where that leaves multiprocessors idle
+    const long long vectors = p.V * (long long)size / 16 + 1;
+    long long piece = 4096;
+    while (piece > 512 && p.rows * ((vectors + piece - 1) / piece) < 4LL * dev.sms) piece /= 2;
+    while (p.rows * ((vectors + piece - 1) / piece) > 0x7fffffffLL) piece *= 2;
+    const long long chunks = (vectors + piece - 1) / piece;
+    p.piece = (int)piece;
     p.chunks = (int)chunks;
     const unsigned grid = (unsigned)(p.rows * chunks);
     cudaStream_t st = (cudaStream_t)call->stream;
