@@ -25,7 +25,8 @@ constexpr int kLpThreads = 256;
 constexpr int kLpAhead = 4;            // 16-byte loads in flight per thread
 constexpr int kTopMax = 64;            // longest list of alternatives
 constexpr int kTopCap = 1024;          // candidates for a list, per CTA
-constexpr int kTopHot = 128;           // threads whose logits are looked at again
+constexpr int kTopHot = 128;           // pieces of a row that are looked at again
+constexpr int kTopPieces = 128;        // steps that the maxima of pieces are kept of
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFloor = -160.f;       // exponent from which on exp2f is zero; keeps 0 * inf out of the second sum
 
@@ -268,8 +269,9 @@ __device__ __forceinline__ void stat_one(Stat& a, float x, float c) {
 }
 // U vectors; the products and sums two at a time.
 template <int DT, int U>
-__device__ __forceinline__ void stat_add(Stat& a, const uint4 (&v)[U], float c) {
-    stat_raise(a, Elem<DT>::largest(v), c);
+__device__ __forceinline__ float stat_add(Stat& a, const uint4 (&v)[U], float c) {      // returns their maximum
+    const float most = Elem<DT>::largest(v);
+    stat_raise(a, most, c);
     const float m = -ref_of(a.mx);
     const uint64_t mm = f2_pack(m, m), cc = f2_pack(c, c);
     uint64_t s = 0ull, u = 0ull;
@@ -293,6 +295,7 @@ __device__ __forceinline__ void stat_add(Stat& a, const uint4 (&v)[U], float c) 
     f2_unpack(u, u0, u1);
     a.s += s0 + s1;
     a.u += u0 + u1;
+    return most;
 }
 // The lanes' statistics as one, in every lane.  s comes and goes as the excess: the sum without the maximum's own 1 (-1: no
 // element above -inf).  Terms are added in a fixed order.
@@ -362,10 +365,10 @@ struct LpShared {
     int c_cnt[16];
 };
 struct TopShared {
-    uint32_t key[kLpThreads];
+    alignas(16) uint32_t key[kLpThreads / 2];
     unsigned long long cand[kTopCap];
-    unsigned long long list[16 * kTopMax];     // the cluster's lists, in the first CTA
-    int list_n[16];
+    unsigned long long list[16 * kTopMax];     // the cluster's lists of top_n entries, in the first CTA; 0: none
+    uint32_t piece[kTopPieces * kLpThreads / 8];
     short hot[kTopHot];
     int nhot, nfinite, ncand, count;
     uint32_t tau;
@@ -376,6 +379,17 @@ __device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
 
+// The maxima of pieces, eight threads' vectors of a step or, in long parts, of 2^shift steps: where a list's entries are.
+__device__ __forceinline__ int top_shift_of(int steps) { return steps <= kTopPieces ? 0 : 32 - __clz((steps - 1) / kTopPieces); }
+__device__ __forceinline__ void top_note(TopShared& sh, int step, int shift, float most) {
+    uint32_t k = key_of(most);
+#pragma unroll
+    for (int o = 1; o < 8; o *= 2) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
+    if ((threadIdx.x & 7) == 0) {
+        uint32_t* at = sh.piece + (step >> shift) * (kLpThreads / 8) + threadIdx.x / 8;
+        *at = (step & ((1 << shift) - 1)) ? max(*at, k) : k;
+    }
+}
 __device__ __forceinline__ void top_push(TopShared& sh, uint32_t key, int j) {
     const int at = atomicAdd(&sh.ncand, 1);
     if (at < kTopCap) sh.cand[at] = ((unsigned long long)key << 32) | (uint32_t)~j;
@@ -449,58 +463,58 @@ __device__ void top_exact(const Span<DT>& sp, TopShared& sh, int n) {
     __syncthreads();
 }
 // The n largest elements of the CTA's part (larger key first, then lower index), unordered, among sh.cand[0 .. result).
-// At least n of the threads have a maximum that reaches the n-th largest maximum, so the list lies within the elements that
-// reach it too, and those are in the few threads whose maximum does: only their elements are read again.
+// At least n threads have a maximum that reaches the n-th largest maximum of the groups, so the list lies within the elements
+// that reach it too, and those are in the few pieces whose maximum does: only they are read again.
 template <int DT>
 __device__ int top_collect(const Span<DT>& sp, TopShared& sh, float mx, int n) {
     constexpr int E = Elem<DT>::E;
-    const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+    const int t = threadIdx.x;
     const uint32_t mine = key_of(mx);
-    // the n-th largest maximum: every warp sorts its own, a place among the others' by bisection
-    uint32_t k = mine;
-#pragma unroll
-    for (int size = 2; size <= 32; size *= 2)
-#pragma unroll
-        for (int step = size / 2; step > 0; step /= 2) {
-            const uint32_t o = __shfl_xor_sync(0xffffffffu, k, step);
-            const bool larger_first = (lane & size) == 0 || size == 32;
-            k = ((lane & step) == 0) == larger_first ? max(k, o) : min(k, o);
-        }
-    sh.key[t] = k;
-    if (t == 0) { sh.nhot = 0; sh.ncand = 0; sh.tau = kKeyNone + 1u; }
+    // the n-th largest of the maxima of equal groups of threads, at least 1.6 n of them: exact enough (about 1.5 n threads
+    // reach it) and a quarter of the time that the n-th largest of all threads' takes
+    const int lg = n <= 5 ? 5 : n <= 10 ? 4 : n <= 20 ? 3 : n <= 40 ? 2 : 1, groups = kLpThreads >> lg;
+    uint32_t of_group = mine;
+    for (int step = 1; step < (1 << lg); step *= 2) of_group = max(of_group, __shfl_xor_sync(0xffffffffu, of_group, step));
+    if ((t & ((1 << lg) - 1)) == 0) sh.key[t >> lg] = of_group;
+    if (t == 0) { sh.nhot = 0; sh.ncand = 0; sh.tau = kKeyNone + 1u; }      // (fewer than n groups with a logit left: all those logits)
     __syncthreads();
-    if (lane < n) {
-        int rank = lane;
-#pragma unroll
-        for (int o = 0; o < kLpThreads / 32; o++) {
-            if (o == w) continue;
-            const uint32_t* list = sh.key + o * 32, least = o < w ? k : k + 1u;      // equal ones: the lower warp's first
-            int at = 0;
-#pragma unroll
-            for (int step = 16; step > 0; step /= 2) at += list[at + step - 1] >= least ? step : 0;
-            rank += at + (list[at] >= least);
+    if (t < groups) {
+        const uint32_t k = sh.key[t];
+        int rank = 0;
+#pragma unroll 4
+        for (int i = 0; i < groups; i += 4) {
+            const uint4 o = *reinterpret_cast<const uint4*>(sh.key + i);
+            rank += (o.x > k || (o.x == k && i < t)) + (o.y > k || (o.y == k && i + 1 < t)) + (o.z > k || (o.z == k && i + 2 < t)) +
+                    (o.w > k || (o.w == k && i + 3 < t));
         }
-        if (rank == n - 1) sh.tau = max(k, kKeyNone + 1u);      // one thread; fewer than n with a logit left: all of those
+        if (rank == n - 1) sh.tau = max(k, kKeyNone + 1u);                   // one thread
     }
     __syncthreads();
     const uint32_t tau = sh.tau;
-    if (mine >= tau) {
-        const int at = atomicAdd(&sh.nhot, 1);
-        if (at < kTopHot) sh.hot[at] = (short)t;
-    }
+    constexpr int kStep = kLpAhead * kLpThreads, kGroups = kLpThreads / 8;
+    const int steps = (sp.v1 - sp.v0 + kStep - 1) / kStep, shift = top_shift_of(steps), pieces = ((steps + (1 << shift) - 1) >> shift) * kGroups;
+    for (int i = t; i < pieces; i += kLpThreads)
+        if (sh.piece[i] >= tau) {
+            const int at = atomicAdd(&sh.nhot, 1);
+            if (at < kTopHot) sh.hot[at] = (short)i;
+        }
+    sp.singles(t, [&](int j, float x) { if (key_of(x) >= tau) top_push(sh, key_of(x), j); });
     __syncthreads();
     const int nhot = sh.nhot;
     if (nhot <= kTopHot) {
-        // all (hot thread, vector) pairs spread over the CTA, four loads ahead
-        const int each = (sp.v1 - sp.v0 + kLpThreads - 1) / kLpThreads, lg = 32 - __clz(max(each, 1) - 1), pairs = nhot << lg;
-        for (int i0 = t; i0 < pairs; i0 += 4 * kLpThreads) {
+        // the hot pieces' vectors spread over the CTA, four loads ahead
+        const int le = 5 + shift, all = nhot << le;
+        for (int i0 = t; i0 < all; i0 += 4 * kLpThreads) {
             uint4 raw[4];
             int at[4];
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 const int i = i0 + q * kLpThreads;
                 at[q] = sp.v1;
-                if (i < pairs) at[q] = sp.v0 + sh.hot[i >> lg] + (i & ((1 << lg) - 1)) * kLpThreads;
+                if (i < all) {
+                    const int piece = sh.hot[i >> le], k = i & ((1 << le) - 1), step = ((piece / kGroups) << shift) + (k >> 5);
+                    at[q] = sp.v0 + step * kStep + ((k >> 3) & 3) * kLpThreads + (piece % kGroups) * 8 + (k & 7);
+                }
                 if (at[q] < sp.v1) raw[q] = ld_stream(sp.vec + at[q]);
             }
 #pragma unroll
@@ -513,7 +527,6 @@ __device__ int top_collect(const Span<DT>& sp, TopShared& sh, float mx, int n) {
                     if (key_of(x[e]) >= tau) top_push(sh, key_of(x[e]), sp.index(at[q]) + e);
             }
         }
-        if (t < nhot) sp.singles(sh.hot[t], [&](int j, float x) { if (key_of(x) >= tau) top_push(sh, key_of(x), j); });
         __syncthreads();
     }
     if (nhot > kTopHot || sh.ncand > kTopCap) top_exact(sp, sh, n);
@@ -562,28 +575,46 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
         stat_one(a, x, c);
         if (TOP) cnt += j < token ? x >= xt : x > xt;
     });
-    // the next vectors are on their way while these are added
+    // steps of kLpAhead vectors a thread, the next step's on their way while one is added; the last one may be a part of one
+    constexpr int kStep = kLpAhead * kLpThreads;
     uint4 raw[2][kLpAhead];
     auto load = [&](uint4 (&to)[kLpAhead], int v) {
 #pragma unroll
-        for (int i = 0; i < kLpAhead; i++) {
-            const int at = v + i * kLpThreads;
-            to[i] = at < sp.v1 ? ld_stream(sp.vec + at) : make_uint4(Elem<DT>::kNone, Elem<DT>::kNone, Elem<DT>::kNone, Elem<DT>::kNone);
-        }
+        for (int i = 0; i < kLpAhead; i++)
+            if (v + i * kLpThreads + t < sp.v1) to[i] = ld_stream(sp.vec + v + i * kLpThreads + t);
     };
-    auto add = [&](const uint4 (&from)[kLpAhead], int v) {
-        stat_add<DT>(a, from, c);
-        if (TOP) {
+    const int top_shift = TOP ? top_shift_of((sp.v1 - sp.v0 + kStep - 1) / kStep) : 0;
+    auto from = [&](int v) { return sp.index(v) < token ? xt : xt_above; };
+    auto add = [&](const uint4 (&x)[kLpAhead], int v) {
+        float most = -INFINITY;
+        if (v + kStep <= sp.v1) {
+            most = stat_add<DT>(a, x, c);
+            if (TOP) {
 #pragma unroll
-            for (int i = 0; i < kLpAhead; i++) {
-                const int at = v + i * kLpThreads;       // (a place behind the part holds -inf: nothing to count)
-                cnt += Elem<DT>::reach(from[i], at >= sp.v1 ? INFINITY : sp.index(at) < token ? xt : xt_above);
+                for (int i = 0; i < kLpAhead; i++) cnt += Elem<DT>::reach(x[i], from(v + i * kLpThreads + t));
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLpAhead; i++)
+                if (v + i * kLpThreads + t < sp.v1) {
+                    const uint4 one[1] = {x[i]};
+                    most = fmaxf(most, stat_add<DT>(a, one, c));
+                    if (TOP) cnt += Elem<DT>::reach(x[i], from(v + i * kLpThreads + t));
+                }
         }
+        if constexpr (TOP) top_note(top, (v - sp.v0) / kStep, top_shift, most);
     };
-    constexpr int kStep = kLpAhead * kLpThreads;
-    int v = sp.v0 + t;
+    int v = sp.v0;
     if (v < sp.v1) load(raw[0], v);
+    if (TOP && p.tokens) {             // the token's own vector, if it begins before the token, is counted from xt on throughout
+        const int own = token >= sp.head && token < sp.tail() ? (token - sp.head) / E : -1;
+        if (own >= sp.v0 && own < sp.v1 && (own - sp.v0) % kLpThreads == t && sp.index(own) < token) {
+            float x[E];
+            widen<DT>(ld_stream(sp.vec + own), x);
+#pragma unroll
+            for (int i = 0; i < E; i++) cnt -= sp.index(own) + i >= token && x[i] == xt;
+        }
+    }
     while (v < sp.v1) {
         if (v + kStep < sp.v1) load(raw[1], v + kStep);
         add(raw[0], v);
@@ -628,9 +659,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
             int at = 0;
 #pragma unroll 8
             for (int q = 0; q < nc; q++) at += top.cand[q] > e;
-            if (at < n) st_cluster_u64(map_to_cta(smem_addr(&top.list[part * kTopMax + at]), 0), e);
+            if (at < n) st_cluster_u64(map_to_cta(smem_addr(&top.list[part * n + at]), 0), e);
         }
-        if (t == 0) st_cluster_u32(map_to_cta(smem_addr(&top.list_n[part]), 0), (uint32_t)min(nc, n));
+        if (t >= nc && t < n) st_cluster_u64(map_to_cta(smem_addr(&top.list[part * n + t]), 0), 0ull);      // no entry
     }
     if (parts > 1) {
         cluster_arrive();
@@ -656,13 +687,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
             if (p.stats) p.stats[r] = make_float2(b.mx, logs * kLog2e);
             if (row.bad_temperature) lp_report(p, RS_ERR_TEMPERATURE);
             if (TOP) {
-                if (p.rank) {
-                    // the token's own vector was counted from xt on if it begins before the token
-                    const int v = (token - sp.head) / E, j0 = sp.index(v);
-                    if (token >= sp.head && v < sp.nvec && j0 < token)
-                        for (int j = token; j < j0 + E; j++) above -= Elem<DT>::one(sp.row + j) == xt;
-                    p.rank[r] = bad ? 0 : above + 1;
-                }
+                if (p.rank) p.rank[r] = bad ? 0 : above + 1;
                 sh.r_mx = b.mx;
                 sh.r_logs = logs;
             }
@@ -673,27 +698,30 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
         const int n = p.top_n;
         const float mx = sh.r_mx, logs = sh.r_logs;
         const bool bad = !(mx < INFINITY);
-        int total = 0;
-        for (int q = 0; q < parts; q++) total += top.list_n[q];
-        auto put = [&](unsigned long long e, int at) {
-            if (at < n && !bad) {
-                p.top[r * n + at] = (of_key((uint32_t)(e >> 32)) - mx) * row.inv_t - logs;
-                p.top_ids[r * n + at] = (int)~(uint32_t)e;
-            }
+        auto put = [&](unsigned long long e, int at) {      // e = 0: a slot that stays empty
+            p.top[r * n + at] = bad ? __int_as_float(0x7FC00000) : e ? (of_key((uint32_t)(e >> 32)) - mx) * row.inv_t - logs : -INFINITY;
+            p.top_ids[r * n + at] = bad || !e ? -1 : (int)~(uint32_t)e;
         };
+        const int all = parts * n;
         if (parts == 1) {
-            if (t < total) put(top.list[t], t);      // in order already
+            if (t < n) put(top.list[t], t);          // in order already
+        } else if (all <= kLpThreads / 2) {
+            if (t < all) {
+                const unsigned long long e = top.list[t];
+                int at = 0;
+#pragma unroll 8
+                for (int q = 0; q < all; q++) at += top.list[q] > e || (top.list[q] == e && q < t);      // (equal: both empty)
+                if (at < n) put(e, at);
+            }
         } else {
             // every list's first ceil(n / parts) entries are n in all: what lies below the least of those is not among the n largest
             const int share = (n + parts - 1) >> log_parts;
             unsigned long long least = ~0ull;
-            for (int q = 0; q < parts; q++) least = min(least, top.list_n[q] >= share ? top.list[q * kTopMax + share - 1] : 0ull);
+            for (int q = 0; q < parts; q++) least = min(least, top.list[q * n + share - 1]);
             if (t == 0) top.ncand = 0;
             __syncthreads();
-            for (int i = t; i < parts * kTopMax; i += kLpThreads) {
-                const int q = i / kTopMax, k = i % kTopMax;
-                if (k < top.list_n[q] && top.list[i] >= least) top.cand[atomicAdd(&top.ncand, 1)] = top.list[i];
-            }
+            for (int i = t; i < all; i += kLpThreads)
+                if (top.list[i] && top.list[i] >= least) top.cand[atomicAdd(&top.ncand, 1)] = top.list[i];
             __syncthreads();
             const int nc = top.ncand;
             for (int i = t; i < nc; i += kLpThreads) {
@@ -701,12 +729,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
                 int at = 0;
 #pragma unroll 8
                 for (int q = 0; q < nc; q++) at += top.cand[q] > e;
-                put(e, at);
+                if (at < n) put(e, at);
             }
-        }
-        if (t < n && (bad || t >= total)) {
-            p.top[r * n + t] = bad ? __int_as_float(0x7FC00000) : -INFINITY;
-            p.top_ids[r * n + t] = -1;
+            if (t >= nc && t < n) put(0ull, t);
         }
     }
 }
