@@ -242,7 +242,7 @@ int rs_vp_tile_max(const rs_vp_call* call, const float* tile_device, int64_t ld,
  * (float32) is not NULL, else `temperature`.  With z = logits / temperature:
  *   log probability  z_token - logsumexp(z)
  *   entropy          of softmax(z), in nats
- * A negative token marks a position that is not scored: its logits are not read, log probability and entropy are 0, the
+ * A negative token marks a position that is not scored: whatever its logits hold: log probability and entropy are 0, the
  * gradient is 0.  Unlike the samplers, which always have to name a token, these calls do not replace what is not finite:
  *   -inf             a masked token: probability 0
  *   nothing but -inf log probability -inf, entropy 0, gradient 0

@@ -75,7 +75,7 @@ def batch_token_logprobs(logits, tokens, temperature=1.0):
     V up to 1048576.  tokens: int32 or int64, the logits' shape without V.  temperature: a number, or a float32 CUDA tensor
     of one value, one per row, or one per sequence; not differentiated.
 
-    A negative token marks a position that is not scored (padding): 0, 0 and no gradient, and its logits are not read.
+    A negative token marks a position that is not scored (padding): 0, 0 and no gradient, whatever its logits hold.
     Unlike the sampling calls, nothing is replaced: -inf masks a token; a row of nothing but -inf has log probability -inf,
     entropy 0 and gradient 0; NaN or +inf makes its row NaN.  A token >= V gives NaN and no gradient, a temperature outside
     [0.001, 1000] in a tensor counts as 1, and either raises ValueError from the next call on the device."""

@@ -543,6 +543,18 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
     const int parts = 1 << log_parts, part = parts > 1 ? (int)cluster_ctarank() : 0;
     const long long r = blockIdx.x >> log_parts;
     const LpRow row = lp_row(p, (uint32_t)r);
+    Span<DT> sp(p, row);
+    sp.share(part, log_parts);
+    // steps of kLpAhead vectors a thread, the next step's on their way while one is added; the last one may be a part of one.
+    // The first is asked for before the token is known, whose load takes as long.
+    constexpr int kStep = kLpAhead * kLpThreads;
+    uint4 raw[2][kLpAhead];
+    auto load = [&](uint4 (&to)[kLpAhead], int v) {
+#pragma unroll
+        for (int i = 0; i < kLpAhead; i++)
+            if (v + i * kLpThreads + t < sp.v1) to[i] = ld_stream(sp.vec + v + i * kLpThreads + t);
+    };
+    load(raw[0], sp.v0);
     if (row.token < 0 || row.bad_token) {         // not scored: the same for the whole cluster
         if (part == 0) {
             const float v = row.bad_token ? __int_as_float(0x7FC00000) : 0.f;
@@ -562,8 +574,6 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
     }
     if (parts > 1) cluster_arrive();
     const float c = row.c;
-    Span<DT> sp(p, row);
-    sp.share(part, log_parts);
     const int token = (int)row.token;
     const float xt = Elem<DT>::one(sp.row + token);
     // rank: an element before the token counts from xt on, one behind it only from the type's next value on
@@ -575,14 +585,6 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
         stat_one(a, x, c);
         if (TOP) cnt += j < token ? x >= xt : x > xt;
     });
-    // steps of kLpAhead vectors a thread, the next step's on their way while one is added; the last one may be a part of one
-    constexpr int kStep = kLpAhead * kLpThreads;
-    uint4 raw[2][kLpAhead];
-    auto load = [&](uint4 (&to)[kLpAhead], int v) {
-#pragma unroll
-        for (int i = 0; i < kLpAhead; i++)
-            if (v + i * kLpThreads + t < sp.v1) to[i] = ld_stream(sp.vec + v + i * kLpThreads + t);
-    };
     const int top_shift = TOP ? top_shift_of((sp.v1 - sp.v0 + kStep - 1) / kStep) : 0;
     auto from = [&](int v) { return sp.index(v) < token ? xt : xt_above; };
     auto add = [&](const uint4 (&x)[kLpAhead], int v) {
@@ -605,7 +607,6 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
         if constexpr (TOP) top_note(top, (v - sp.v0) / kStep, top_shift, most);
     };
     int v = sp.v0;
-    if (v < sp.v1) load(raw[0], v);
     if (TOP && p.tokens) {             // the token's own vector, if it begins before the token, is counted from xt on throughout
         const int own = token >= sp.head && token < sp.tail() ? (token - sp.head) / E : -1;
         if (own >= sp.v0 && own < sp.v1 && (own - sp.v0) % kLpThreads == t && sp.index(own) < token) {

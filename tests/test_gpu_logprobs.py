@@ -150,7 +150,7 @@ def test_padded_positions():
     x, t = make((4, 9), 777, "bf16", 10)
     t[1, 4:] = -1
     t[2] = -100
-    x[2] = math.nan                                                    # never read
+    x[2] = math.nan                                                    # does not matter
     check_all(x, t, 1.0, top_n=3)
 
 
