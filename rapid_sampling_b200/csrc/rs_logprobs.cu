@@ -795,15 +795,30 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_backward_kernel(const __grid
             }
             __stcs(vec + at, Elem<DT>::narrow(x));
         };
-        int v = sp.v0 + t;
-        for (; v + (kLpAhead - 1) * kLpThreads < sp.v1; v += kLpAhead * kLpThreads) {
-            uint4 raw[kLpAhead];
+        // as in the forward pass: the next step's loads are on their way while one is computed and stored
+        constexpr int kStep = kLpAhead * kLpThreads;
+        uint4 raw[2][kLpAhead];
+        auto load = [&](uint4 (&to)[kLpAhead], int v) {
 #pragma unroll
-            for (int i = 0; i < kLpAhead; i++) raw[i] = ld_stream(sp.vec + v + i * kLpThreads);
+            for (int i = 0; i < kLpAhead; i++)
+                if (v + i * kLpThreads + t < sp.v1) to[i] = ld_stream(sp.vec + v + i * kLpThreads + t);
+        };
+        auto step = [&](const uint4 (&x)[kLpAhead], int v) {
 #pragma unroll
-            for (int i = 0; i < kLpAhead; i++) one(raw[i], v + i * kLpThreads);
+            for (int i = 0; i < kLpAhead; i++)
+                if (v + i * kLpThreads + t < sp.v1) one(x[i], v + i * kLpThreads + t);
+        };
+        int v = sp.v0;
+        load(raw[0], v);
+        while (v < sp.v1) {
+            if (v + kStep < sp.v1) load(raw[1], v + kStep);
+            step(raw[0], v);
+            v += kStep;
+            if (v >= sp.v1) break;
+            if (v + kStep < sp.v1) load(raw[0], v + kStep);
+            step(raw[1], v);
+            v += kStep;
         }
-        for (; v < sp.v1; v += kLpThreads) one(ld_stream(sp.vec + v), v);
         // the token's own, behind the store of its vector by the same thread
         const int own = token >= sp.head && token < sp.tail() ? (token - sp.head) / E : -1;
         if (own >= sp.v0 && own < sp.v1 && (own - sp.v0) % kLpThreads == t) out[token] = Elem<DT>::to(grad_at(Elem<DT>::one(sp.row + token)));
