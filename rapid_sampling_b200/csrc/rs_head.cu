@@ -288,7 +288,8 @@ struct HeadParams {
     int n;                   // rows of tokens a stage holds, a multiple of 16
     int token_tiles;         // more tokens: tiles of 128, or of 256 for pairs
     int stages;
-    int wide_store;          // more tokens: bytes of a store that the result's rows allow (32, 16, or 0: one by one)
+    int boxes;               // pairs: the copy engine stores the result
+    int wide_store;          // more tokens, else: bytes of a store that the result's rows allow (32, 16, or 0: one by one)
     float* partial;          // split work: two slots a CTA
     int* arrived;            // split work: workers done with the tile that begins in a worker's run
     uint32_t polls;
@@ -622,9 +623,53 @@ __device__ __forceinline__ void head_store(OUT* o, const uint64_t (&acc)[COLS / 
     }
 }
 
+// The same by way of shared memory, 8 KB a warp, for the warp's 32 rows: two boxes of 128 bytes by 32 rows at a time, which the
+// copy engine stores (and cuts off behind the last row and column) while the warp goes on with the next tile.  All CTAs end
+// their tiles at about the same time: stores by the threads themselves waited 3.6 us a tile for one another (16 % of the time at
+// 2048 tokens).  128-byte swizzle: the 16-byte column c of row r lies at c ^ (r % 8).
+constexpr int kStoreBytes = 8192;
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
+}
+template <int COLS, typename OUT>
+__device__ __forceinline__ void head_store_box(const CUtensorMap* map, uint32_t buf, const uint64_t (&acc)[COLS / 2], int lane, int m, int v0, int V) {
+    constexpr int PER = 128 / (int)sizeof(OUT);       // columns of a box
+#pragma unroll
+    for (int c0 = 0; c0 < COLS; c0 += 2 * PER) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the boxes before have been read
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 16; i++) {                // 16 bytes each
+            const int col = c0 + i * (16 / (int)sizeof(OUT));
+            uint32_t x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float a, b;
+                if constexpr (sizeof(OUT) == 4) {
+                    f2_unpack(acc[(col + j) / 2], a, b);
+                    x[j] = __float_as_uint(j & 1 ? b : a);
+                } else {
+                    f2_unpack(acc[col / 2 + j], a, b);
+                    x[j] = head_word<OUT>(a, b);
+                }
+            }
+            const uint32_t at = buf + (uint32_t)(i / 8) * 4096u + (uint32_t)lane * 128u + (uint32_t)(((i & 7) ^ (lane & 7)) * 16);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+            if (v0 + c0 < V) tma_store_2d(map, buf, v0 + c0, m);
+            if (v0 + c0 + PER < V) tma_store_2d(map, buf + 4096u, v0 + c0 + PER, m);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+    }
+}
+
 template <bool PAIR, typename OUT>
 __global__ void __launch_bounds__(kMoreThreads, 1)
-    head_more_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ HeadParams p) {
+    head_more_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_out,
+                     const __grid_constant__ HeadParams p) {
     constexpr int W = kMoreAdders, COLS = 256 / (W / 4), NT = 256, CTAS = PAIR ? 2 : 1;
     constexpr uint32_t kTmemCols = 512, kWeights = (PAIR ? 128 : 256) * 128;
     const uint32_t stage_bytes = (uint32_t)head_more_stage(PAIR, p.n);
@@ -746,16 +791,23 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
             // (weight rows and tokens behind the last one: any scale, their sums are not stored)
             const float* sw = p.sw + (long long)(min(v0, p.V - 1) / 128) * p.work.blocks;
             const float* sa = p.sa + m;
-            float next_a = __ldcg(sa + (long long)walk.b0 * p.pitch), next_w = __ldg(sw + walk.b0);
+            // two blocks ahead: a load from L2 takes longer than a block's products
+            float a1 = __ldcg(sa + (long long)walk.b0 * p.pitch), w1 = __ldg(sw + walk.b0), a2 = 0.f, w2 = 0.f;
+            if (walk.b0 + 1 < walk.b1) {
+                a2 = __ldcg(sa + (long long)(walk.b0 + 1) * p.pitch);
+                w2 = __ldg(sw + walk.b0 + 1);
+            }
             uint64_t acc[COLS / 2];
 #pragma unroll
             for (int i = 0; i < COLS / 2; i++) acc[i] = 0ull;
             for (int b = walk.b0; b < walk.b1; b++, it++) {
                 const uint32_t buf = it & 1u;
-                const float f = next_a * next_w;
-                if (b + 1 < walk.b1) {
-                    next_a = __ldcg(sa + (long long)(b + 1) * p.pitch);
-                    next_w = __ldg(sw + b + 1);
+                const float f = a1 * w1;
+                a1 = a2;
+                w1 = w2;
+                if (b + 2 < walk.b1) {
+                    a2 = __ldcg(sa + (long long)(b + 2) * p.pitch);
+                    w2 = __ldg(sw + b + 2);
                 }
                 const uint64_t ff = f2_pack(f, f);
                 if (!dead) dead = !__all_sync(0xffffffffu, wait(sfull + 8 * buf, (it >> 1) & 1u));
@@ -802,8 +854,14 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
                     }
                 }
             }
-            if (m < p.M && !dead) head_store<COLS, OUT>((OUT*)p.out + (long long)m * p.ldo + v0, acc, p.V - v0, p.wide_store);
+            if (PAIR && p.boxes) {
+                if (!dead && m - lane < p.M && v0 < p.V)
+                    head_store_box<COLS, OUT>(&map_out, base + stages * stage_bytes + (uint32_t)(w * kStoreBytes), acc, lane, m - lane, v0, p.V);
+            } else if (m < p.M && !dead) {
+                head_store<COLS, OUT>((OUT*)p.out + (long long)m * p.ldo + v0, acc, p.V - v0, p.wide_store);
+            }
         }
+        if (PAIR && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncwarp();
     tmem_fence_before();
@@ -832,20 +890,19 @@ static EncodeTiled head_encoder() {
     }();
     return fn;
 }
-// (rows, K) codes in tiles of box_rows x 128; what lies outside reads as zero
-static int head_map(CUtensorMap* m, const void* codes, long long rows, long long K, int box_rows) {
+// (rows, cols) elements, rows `pitch` bytes apart, in boxes of box_rows rows by 128 bytes; what lies outside reads as zero
+static int head_map(CUtensorMap* m, CUtensorMapDataType type, int size, const void* at, long long rows, long long cols, long long pitch, int box_rows) {
     EncodeTiled enc = head_encoder();
     if (!enc) return host_cuda_fail(cudaErrorSymbolNotFound, "cuTensorMapEncodeTiled");
-    const cuuint64_t dim[2] = {(cuuint64_t)K, (cuuint64_t)rows}, stride[1] = {(cuuint64_t)K};
-    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, step[2] = {1, 1};
-    const CUresult e = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dim, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const cuuint64_t dim[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, stride[1] = {(cuuint64_t)pitch};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows}, step[2] = {1, 1};
+    const CUresult e = enc(m, type, 2, const_cast<void*>(at), dim, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return e == CUDA_SUCCESS ? RS_OK : host_cuda_fail(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
 }
 
-template <typename KERN>
-static int head_launch(KERN kern, const CUtensorMap& w, const CUtensorMap& x, const HeadParams& p, int threads, int smem, int grid, int cluster,
-                       cudaStream_t stream, bool (&done)[64]) {
+template <typename KERN, typename... ARGS>
+static int head_launch(KERN kern, int threads, int smem, int grid, int cluster, cudaStream_t stream, bool (&done)[64], const ARGS&... args) {
     {
         static std::mutex mu;
         int dev = 0;
@@ -878,18 +935,18 @@ static int head_launch(KERN kern, const CUtensorMap& w, const CUtensorMap& x, co
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, w, x, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
     if (e != cudaSuccess) return host_cuda_fail(e, "cudaLaunchKernelEx(head)");
     host_count_launch();
     return RS_OK;
 }
 template <typename OUT>
-static int head_run(const CUtensorMap& w, const CUtensorMap& x, const HeadParams& p, int smem, cudaStream_t stream) {
+static int head_run(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& out, const HeadParams& p, int smem, cudaStream_t stream) {
     static bool done[3][64] = {};      // per device
     const int n = p.work.workers;
-    if (p.M <= kFewTokens) return head_launch(head_few_kernel<OUT>, w, x, p, 192, smem, n, 1, stream, done[0]);
-    if (p.M <= 128) return head_launch(head_more_kernel<false, OUT>, w, x, p, kMoreThreads, smem, n, 1, stream, done[1]);
-    return head_launch(head_more_kernel<true, OUT>, w, x, p, kMoreThreads, smem, 2 * n, 2, stream, done[2]);
+    if (p.M <= kFewTokens) return head_launch(head_few_kernel<OUT>, 192, smem, n, 1, stream, done[0], w, x, p);
+    if (p.M <= 128) return head_launch(head_more_kernel<false, OUT>, kMoreThreads, smem, n, 1, stream, done[1], w, x, out, p);
+    return head_launch(head_more_kernel<true, OUT>, kMoreThreads, smem, 2 * n, 2, stream, done[2], w, x, out, p);
 }
 
 // Pairs of CTAs that the device runs at once.
@@ -1042,18 +1099,28 @@ int rs_head_logits(const void* hidden, int32_t hidden_dtype, int64_t M, int64_t 
     if (k.split && k.units < 4LL * k.workers) k.workers = (int)((k.units + 3) / 4);
     if (!k.split && tiles < k.workers) k.workers = (int)tiles;
     const int per = few ? head_few_stage(p.n) : head_more_stage(pair, p.n);
-    const int tail = few ? 0 : head_more_tail(pair, p.n), room = dev.smem_optin - 2048 - 1024 - tail;
-    p.stages = room / per > kHeadMaxStages ? kHeadMaxStages : room / per;
     const uintptr_t step = (uintptr_t)out_device | (uintptr_t)out_stride * os;
     p.wide_store = step % 32 == 0 ? 32 : step % 16 == 0 ? 16 : 0;
-    CUtensorMap w, x;
-    if ((rc = head_map(&w, codes_device, V, K, few || pair ? 128 : 256)) || (rc = head_map(&x, ws, M, K, p.n))) return rc;
+    p.boxes = pair && p.wide_store;
+    const int tail = few ? 0 : p.boxes ? kMoreAdders * kStoreBytes : head_more_tail(pair, p.n), room = dev.smem_optin - 2048 - 1024 - tail;
+    p.stages = room / per > kHeadMaxStages ? kHeadMaxStages : room / per;
+    CUtensorMap w, x, out;
+    if ((rc = head_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes_device, V, K, K, few || pair ? 128 : 256)) ||
+        (rc = head_map(&x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, ws, M, K, K, p.n)))
+        return rc;
+    memset(&out, 0, sizeof out);
+    if (p.boxes) {
+        const CUtensorMapDataType type = out_dtype == RS_DTYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                         : out_dtype == RS_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        if ((rc = head_map(&out, type, (int)os, out_device, M, V, (long long)(out_stride * (int64_t)os), 32))) return rc;
+    }
     if ((rc = head_quantize<true>(hidden, hidden_dtype, hidden_stride, M, K, ws, sa, p.pitch, p.arrived, (cudaStream_t)stream))) return rc;
     const int smem = p.stages * per + tail + 1024;
     switch (out_dtype) {
-        case RS_DTYPE_F32: return head_run<float>(w, x, p, smem, (cudaStream_t)stream);
-        case RS_DTYPE_F16: return head_run<__half>(w, x, p, smem, (cudaStream_t)stream);
-        default: return head_run<__nv_bfloat16>(w, x, p, smem, (cudaStream_t)stream);
+        case RS_DTYPE_F32: return head_run<float>(w, x, out, p, smem, (cudaStream_t)stream);
+        case RS_DTYPE_F16: return head_run<__half>(w, x, out, p, smem, (cudaStream_t)stream);
+        default: return head_run<__nv_bfloat16>(w, x, out, p, smem, (cudaStream_t)stream);
     }
 }
 

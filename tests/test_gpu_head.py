@@ -139,6 +139,22 @@ def test_whole_numbers(spread):
     assert bool(((got - want).abs() <= 4 * 2.0 ** -24 * partial).all())
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_many_tokens_into_rows_of_any_alignment(dtype):
+    """Results stored in boxes, in vectors and one by one; nothing beside them is touched."""
+    import rapid_sampling_b200 as rs
+    K, V, M = 256, 1000, 333
+    codes, scales = rs.lm_head_quantize(make(V, K, "bf16", 1, 0.02))
+    hidden = make(M, K, "bf16", 2)
+    got = rs.lm_head_logits(hidden, codes, scales, dtype=DT[dtype])
+    check(hidden, codes, scales, got)
+    for pad, first in ((24, 8), (24, 1), (9, 0), (9, 3)):
+        buf = torch.full((M, V + pad), 7.0, device="cuda", dtype=DT[dtype])
+        rs.lm_head_logits(hidden, codes, scales, out=buf[:, first:first + V])
+        assert torch.equal(buf[:, first:first + V], got), (pad, first)
+        assert bool((buf[:, :first] == 7).all()) and bool((buf[:, first + V:] == 7).all())
+
+
 def test_shapes_strides_and_out():
     import rapid_sampling_b200 as rs
     K, V = 256, 300
