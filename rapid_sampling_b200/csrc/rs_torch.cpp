@@ -51,6 +51,11 @@ volatile int* mirror_for(int device) {
     }
     return m.word.data_ptr<int>();
 }
+bool mirror_known(int device) {
+    std::lock_guard<std::mutex> lk(g_mirror_mu);
+    const auto it = g_mirror.find(device);
+    return it != g_mirror.end() && it->second.word.defined();
+}
 [[noreturn]] void throw_status(const char* what, int device, int v) {
     std::string msg = std::string(what) + " on cuda:" + std::to_string(device) + " reported: " + rs_status_string(v) + " !\n";
     if (v == RS_ERR_TEMPERATURE || v == RS_ERR_TOKEN) throw std::invalid_argument(msg);
@@ -211,10 +216,11 @@ at::Tensor sample_repetition_any(at::Tensor& logits, at::Tensor& penalties, at::
 // The same for the calls that have no workspace.  A call that is being captured neither raises nor creates the mirror:
 // both would touch the device outside the graph.
 static void raise_pending_logprobs(int device, cudaStream_t stream) {
-    if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) return;
+    auto capturing = [] { return at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None; };
+    if (!mirror_known(device) && capturing()) return;
     volatile int* w = mirror_for(device);
     const int v = *w;
-    if (v == 0) return;
+    if (v == 0 || capturing()) return;
     *w = 0;
     rs_logprobs_status(stream);      // clears the device's word
     throw_status("an earlier call", device, v);

@@ -147,6 +147,36 @@ class VocabParallelSampler:
     def push_tile(self, tile, col_begin):
         self.compute.tile_max(tile, col_begin)
 
+    def project(self, hidden, codes, scales, states, temperature, top_k, top_p, penalties=None, presence_penalty=0.0,
+                repetition_penalty=0.0, penalty_decay=0.0, out=None):
+        """This rank's logits (B, V_local) from hidden states (B, K), the same on every rank, and this rank's rows of an fp8
+        lm_head (`lm_head_quantize` of its V_local weight rows).  The product is made in column slabs small enough for L2 and
+        each slab's row maxima are handed over at once, so that `sample(logits, ..., max_from_tiles=True)` with the same
+        arguments needs no pass for them.  `out`: a contiguous float32 buffer to use again."""
+        from . import lm_head_logits
+        if self.T != 1:
+            raise ValueError("project makes one position per row, but this sampler was made for T=%d" % self.T)
+        if tuple(codes.shape) != (self.V_local, hidden.shape[-1]) or tuple(hidden.shape[:-1]) != (self.B,):
+            raise ValueError("project takes hidden states (B, K) and codes (V_local, K)")
+        if out is None:
+            out = torch.empty((self.B, self.V_local), dtype=torch.float32, device=hidden.device)
+        elif tuple(out.shape) != (self.B, self.V_local) or out.dtype != torch.float32 or not out.is_contiguous():
+            raise ValueError("out must be a contiguous float32 tensor (B, V_local)")
+        self.begin_tiles(out, states, temperature, top_k, top_p, penalties, presence_penalty, repetition_penalty, penalty_decay)
+        cols = max(128, (1 << 23) // self.B // 128 * 128)          # 32 MB a slab; whole blocks of the codes' scales
+        for col in range(0, self.V_local, cols):
+            tile = out[:, col:col + cols]
+            lm_head_logits(hidden, codes[col:col + cols], scales[col // 128:(col + cols) // 128], out=tile)
+            self.push_tile(tile, col)
+        return out
+
+    def sample_hidden(self, hidden, codes, scales, states, temperature, top_k, top_p, penalties=None, presence_penalty=0.0,
+                      repetition_penalty=0.0, penalty_decay=0.0, out=None):
+        """`project` and `sample` in one: token ids (B,) from hidden states, identical on every rank."""
+        rest = (states, temperature, top_k, top_p, penalties, presence_penalty, repetition_penalty, penalty_decay)
+        logits = self.project(hidden, codes, scales, *rest, out=out)
+        return self.sample(logits, *rest, max_from_tiles=True)
+
     def _fast_stages(self, penalties):
         """The device side of the fast protocol: four kernels, four collectives, then the state advance and the penalty
         update, which the device applies only if every row was settled."""

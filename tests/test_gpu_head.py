@@ -264,3 +264,31 @@ def test_from_hidden_states_to_a_scored_token():
         want = torch.log_softmax(wide(*quantized(hidden, 1), 1) @ wide(codes, scales, 128).t() / 0.8, -1)
         # logits to 2e-5 of their size (the bound of the products above), so differences to twice that over the temperature
         assert float((lp.double() - want.gather(1, ids.long()[:, None])[:, 0]).abs().max()) < 1e-3
+
+
+@pytest.mark.parametrize("B,V_local,penalised", [(3, 4100, False), (40, 16384, True), (70, 151936, False)])
+def test_vocab_parallel_sampling_from_hidden_states(B, V_local, penalised):
+    """The vocab-parallel sampler's own path from hidden states: the product, whatever its slabs, and the ids and states of a
+    plain call on its logits."""
+    import rapid_sampling_b200 as rs
+    from rapid_sampling_b200.vocab_parallel import VocabParallelSampler
+    K = 256
+    codes, scales = rs.lm_head_quantize(make(V_local, K, "bf16", 1, 0.2))
+    hidden = make(B, K, "bf16", 2)
+    a, b = VocabParallelSampler(B, V_local, 0, 1), VocabParallelSampler(B, V_local, 0, 1)
+    st_a, st_b = rs.setup_rand(5, B), rs.setup_rand(5, B)
+    pen_a, pen_b = (torch.zeros(B, V_local, device="cuda"), torch.zeros(B, V_local, device="cuda")) if penalised else (None, None)
+    buf = torch.empty(B, V_local, device="cuda")
+    for step in range(3):
+        got = a.sample_hidden(hidden, codes, scales, st_a, 0.8, 50, 0.9, pen_a, 0.1, 0.1, 0.95, out=buf)
+        check(hidden, codes, scales, buf)
+        want = b.sample(buf, st_b, 0.8, 50, 0.9, pen_b, 0.1, 0.1, 0.95)
+        assert torch.equal(got, want) and torch.equal(st_a, st_b)
+        if penalised:
+            assert torch.equal(pen_a, pen_b)
+    assert a.project(hidden, codes, scales, st_a, 0.8, 50, 0.9).shape == (B, V_local)
+    for bad in (lambda: a.project(hidden[:1], codes, scales, st_a, 0.8, 50, 0.9), lambda: a.project(hidden, codes[:128], scales, st_a, 0.8, 50, 0.9),
+                lambda: a.project(hidden, codes, scales, st_a, 0.8, 50, 0.9, out=buf.half()),
+                lambda: VocabParallelSampler(B, V_local, 0, 1, T=2).project(hidden, codes, scales, st_a, 0.8, 50, 0.9)):
+        with pytest.raises(ValueError):
+            bad()
