@@ -831,12 +831,14 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
             }
             if (!walk.whole()) {
                 float* mine = p.partial + (long long)(2 * (int)blockIdx.x + (walk.b0 == 0)) * 128 * 256 + (long long)col0 * 128 + row;
+                if (m < p.M) {
 #pragma unroll
-                for (int i = 0; i < COLS / 2; i++) {
-                    float a, b;
-                    f2_unpack(acc[i], a, b);
-                    mine[(2 * i) * 128] = a;
-                    mine[(2 * i + 1) * 128] = b;
+                    for (int i = 0; i < COLS / 2; i++) {
+                        float a, b;
+                        f2_unpack(acc[i], a, b);
+                        mine[(2 * i) * 128] = a;
+                        mine[(2 * i + 1) * 128] = b;
+                    }
                 }
                 const long long u = (long long)walk.tile * p.work.blocks;
                 const int c0 = p.work.owner(u), c1 = p.work.owner(u + p.work.blocks - 1);
@@ -844,7 +846,7 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
                 if (!head_last<W * 32>(p, CTAS * c0 + rank, c1 - c0 + 1, &flag)) continue;
 #pragma unroll
                 for (int i = 0; i < COLS / 2; i++) acc[i] = 0ull;
-                for (int c = c0; c <= c1; c++) {
+                for (int c = c0; c <= c1 && m < p.M; c++) {
                     const float* from = p.partial + (long long)(2 * (CTAS * c + rank) + (c == c0)) * 128 * 256 + (long long)col0 * 128 + row;
 #pragma unroll
                     for (int i = 0; i < COLS / 2; i++) {
