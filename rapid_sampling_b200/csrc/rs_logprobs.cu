@@ -21,12 +21,9 @@
 
 namespace rs {
 
-constexpr int kLpThreads = 256;
 constexpr int kLpAhead = 4;            // 16-byte loads in flight per thread
 constexpr int kTopMax = 64;            // longest list of alternatives
-constexpr int kTopCap = 1024;          // candidates for a list, per CTA
 constexpr int kTopHot = 128;           // pieces of a row that are looked at again
-constexpr int kTopPieces = 128;        // steps that the maxima of pieces are kept of
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFloor = -160.f;       // exponent from which on exp2f is zero; keeps 0 * inf out of the second sum
 
@@ -87,10 +84,13 @@ template <> struct Elem<RS_DTYPE_F32> {
         }
         return m;
     }
-    // elements of at least `from`
-    static __device__ __forceinline__ int reach(const uint4& v, float from) {
-        return (__uint_as_float(v.x) >= from) + (__uint_as_float(v.y) >= from) + (__uint_as_float(v.z) >= from) + (__uint_as_float(v.w) >= from);
+    // counts the elements of at least `from`, a value of the type
+    using Count = int;
+    static __device__ __forceinline__ Count none() { return 0; }
+    static __device__ __forceinline__ void reach(Count& n, const uint4& v, float from) {
+        n += (__uint_as_float(v.x) >= from) + (__uint_as_float(v.y) >= from) + (__uint_as_float(v.z) >= from) + (__uint_as_float(v.w) >= from);
     }
+    static __device__ __forceinline__ int whole(Count n) { return n; }
     static __device__ __forceinline__ float one(const T* p) { return *p; }
     static __device__ __forceinline__ uint4 narrow(const uint64_t (&x)[2]) {
         float a, b, c, d;
@@ -120,11 +120,13 @@ template <> struct Elem<RS_DTYPE_F16> {
         const float2 f = __half22float2(m);
         return max_nan(f.x, f.y);
     }
-    static __device__ __forceinline__ int reach(const uint4& v, float from) {      // `from` is a value of the type
+    using Count = __half2;             // exact up to 2048 in each half
+    static __device__ __forceinline__ Count none() { return __float2half2_rn(0.f); }
+    static __device__ __forceinline__ void reach(Count& n, const uint4& v, float from) {
         const __half2 f = __float2half2_rn(from);
-        const __half2 n = __hadd2(__hadd2(__hge2(h2(v.x), f), __hge2(h2(v.y), f)), __hadd2(__hge2(h2(v.z), f), __hge2(h2(v.w), f)));
-        return (int)(__low2float(n) + __high2float(n));
+        n = __hadd2(__hadd2(__hadd2(__hge2(h2(v.x), f), __hge2(h2(v.y), f)), __hadd2(__hge2(h2(v.z), f), __hge2(h2(v.w), f))), n);
     }
+    static __device__ __forceinline__ int whole(Count n) { return (int)(__low2float(n) + __high2float(n)); }
     static __device__ __forceinline__ float one(const T* p) { return __half2float(*p); }
     static __device__ __forceinline__ uint4 narrow(const uint64_t (&x)[4]) {
         uint32_t w[4];
@@ -155,11 +157,13 @@ template <> struct Elem<RS_DTYPE_BF16> {
         for (int i = 0; i < U; i++) m = __hmax2_nan(__hmax2_nan(__hmax2_nan(__hmax2_nan(m, h2(v[i].x)), h2(v[i].y)), h2(v[i].z)), h2(v[i].w));
         return max_nan(__low2float(m), __high2float(m));
     }
-    static __device__ __forceinline__ int reach(const uint4& v, float from) {
+    using Count = __nv_bfloat162;      // exact up to 256 in each half
+    static __device__ __forceinline__ Count none() { return __float2bfloat162_rn(0.f); }
+    static __device__ __forceinline__ void reach(Count& n, const uint4& v, float from) {
         const __nv_bfloat162 f = __float2bfloat162_rn(from);
-        const __nv_bfloat162 n = __hadd2(__hadd2(__hge2(h2(v.x), f), __hge2(h2(v.y), f)), __hadd2(__hge2(h2(v.z), f), __hge2(h2(v.w), f)));
-        return (int)(__low2float(n) + __high2float(n));
+        n = __hadd2(__hadd2(__hadd2(__hge2(h2(v.x), f), __hge2(h2(v.y), f)), __hadd2(__hge2(h2(v.z), f), __hge2(h2(v.w), f))), n);
     }
+    static __device__ __forceinline__ int whole(Count n) { return (int)(__low2float(n) + __high2float(n)); }
     static __device__ __forceinline__ float one(const T* p) { return __bfloat162float(*p); }
     static __device__ __forceinline__ uint4 narrow(const uint64_t (&x)[4]) {
         uint32_t w[4];
@@ -316,7 +320,7 @@ __device__ __forceinline__ Stat stat_warp(Stat a, float c) {
 
 // ---- the part of a row that a CTA reads ----------------------------------------------------------------------------
 // Elements up to the first 16-byte boundary and behind the last whole vector are single ones, taken by the first and the
-// last CTA of the row; the vectors between are split evenly.  Vector v of the CTA belongs to thread v % kLpThreads.
+// last CTA of the row; the vectors between are split evenly.  Vector v of the CTA belongs to thread v % NT.
 template <int DT>
 struct Span {
     using T = typename Elem<DT>::T;
@@ -364,11 +368,15 @@ struct LpShared {
     float c_mx[16], c_s[16], c_u[16];
     int c_cnt[16];
 };
+// (Rows of CTAs with fewer than 256 threads are short and not shared.)
+template <int NT>
 struct TopShared {
-    alignas(16) uint32_t key[kLpThreads / 2];
-    unsigned long long cand[kTopCap];
-    unsigned long long list[16 * kTopMax];     // the cluster's lists of top_n entries, in the first CTA; 0: none
-    uint32_t piece[kTopPieces * kLpThreads / 8];
+    static constexpr int kCap = NT == 256 ? 1024 : 640;            // candidates for a list
+    static constexpr int kPieces = NT == 256 ? 128 : 16;           // steps that the maxima of pieces are kept of
+    alignas(16) uint32_t key[NT];
+    unsigned long long cand[kCap];
+    unsigned long long list[(NT == 256 ? 16 : 1) * kTopMax];       // the cluster's lists of top_n entries, in the first CTA; 0: none
+    uint32_t piece[kPieces * NT / 8];
     short hot[kTopHot];
     int nhot, nfinite, ncand, count;
     uint32_t tau;
@@ -380,29 +388,35 @@ __device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long
 }
 
 // The maxima of pieces, eight threads' vectors of a step or, in long parts, of 2^shift steps: where a list's entries are.
-__device__ __forceinline__ int top_shift_of(int steps) { return steps <= kTopPieces ? 0 : 32 - __clz((steps - 1) / kTopPieces); }
-__device__ __forceinline__ void top_note(TopShared& sh, int step, int shift, float most) {
+template <int NT>
+__device__ __forceinline__ int top_shift_of(int steps) {
+    constexpr int most = TopShared<NT>::kPieces;
+    return steps <= most ? 0 : 32 - __clz((steps - 1) / most);
+}
+template <int NT>
+__device__ __forceinline__ void top_note(TopShared<NT>& sh, int step, int shift, float most) {
     uint32_t k = key_of(most);
 #pragma unroll
     for (int o = 1; o < 8; o *= 2) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
     if ((threadIdx.x & 7) == 0) {
-        uint32_t* at = sh.piece + (step >> shift) * (kLpThreads / 8) + threadIdx.x / 8;
+        uint32_t* at = sh.piece + (step >> shift) * (NT / 8) + threadIdx.x / 8;
         *at = (step & ((1 << shift) - 1)) ? max(*at, k) : k;
     }
 }
-__device__ __forceinline__ void top_push(TopShared& sh, uint32_t key, int j) {
+template <int NT>
+__device__ __forceinline__ void top_push(TopShared<NT>& sh, uint32_t key, int j) {
     const int at = atomicAdd(&sh.ncand, 1);
-    if (at < kTopCap) sh.cand[at] = ((unsigned long long)key << 32) | (uint32_t)~j;
+    if (at < TopShared<NT>::kCap) sh.cand[at] = ((unsigned long long)key << 32) | (uint32_t)~j;
 }
 // Elements of the CTA's part with a key of at least `at_least`.
-template <int DT>
-__device__ int top_count(const Span<DT>& sp, TopShared& sh, uint32_t at_least) {
+template <int DT, int NT>
+__device__ int top_count(const Span<DT>& sp, TopShared<NT>& sh, uint32_t at_least) {
     constexpr int E = Elem<DT>::E;
     __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
     int n = 0;
-    for (int v = sp.v0 + (int)threadIdx.x; v < sp.v1; v += kLpThreads) {
+    for (int v = sp.v0 + (int)threadIdx.x; v < sp.v1; v += NT) {
         float x[E];
         widen<DT>(ld_stream(sp.vec + v), x);
 #pragma unroll
@@ -417,8 +431,8 @@ __device__ int top_count(const Span<DT>& sp, TopShared& sh, uint32_t at_least) {
 // order of their indices.  For parts whose n largest elements are not told apart by the threads' maxima: long runs of equal
 // logits, or large ones that crowd in few threads.  About 32 passes over the part at worst, 2 where the threads' n-th
 // largest maximum is the key, as with a mask of the type's lowest value.
-template <int DT>
-__device__ void top_exact(const Span<DT>& sp, TopShared& sh, int n) {
+template <int DT, int NT>
+__device__ void top_exact(const Span<DT>& sp, TopShared<NT>& sh, int n) {
     constexpr int E = Elem<DT>::E;
     const int t = threadIdx.x;
     uint32_t lo = sh.tau, hi = 0xFF800001u;        // count(lo) >= n > count(hi): nothing lies above +inf's key
@@ -428,7 +442,7 @@ __device__ void top_exact(const Span<DT>& sp, TopShared& sh, int n) {
     __syncthreads();
     if (t == 0) sh.ncand = 0;
     __syncthreads();
-    for (int v = sp.v0 + t; v < sp.v1; v += kLpThreads) {
+    for (int v = sp.v0 + t; v < sp.v1; v += NT) {
         float x[E];
         widen<DT>(ld_stream(sp.vec + v), x);
 #pragma unroll
@@ -465,14 +479,17 @@ __device__ void top_exact(const Span<DT>& sp, TopShared& sh, int n) {
 // The n largest elements of the CTA's part (larger key first, then lower index), unordered, among sh.cand[0 .. result).
 // At least n threads have a maximum that reaches the n-th largest maximum of the groups, so the list lies within the elements
 // that reach it too, and those are in the few pieces whose maximum does: only they are read again.
-template <int DT>
-__device__ int top_collect(const Span<DT>& sp, TopShared& sh, float mx, int n) {
+template <int DT, int NT>
+__device__ int top_collect(const Span<DT>& sp, TopShared<NT>& sh, float mx, int n) {
     constexpr int E = Elem<DT>::E;
     const int t = threadIdx.x;
     const uint32_t mine = key_of(mx);
     // the n-th largest of the maxima of equal groups of threads, at least 1.6 n of them: exact enough (about 1.5 n threads
     // reach it) and a quarter of the time that the n-th largest of all threads' takes
-    const int lg = n <= 5 ? 5 : n <= 10 ? 4 : n <= 20 ? 3 : n <= 40 ? 2 : 1, groups = kLpThreads >> lg;
+    const int busy = min(NT, sp.v1 - sp.v0);      // threads that have vectors
+    int lg = 0;
+    while (lg < 5 && (busy >> (lg + 1)) * 5 >= n * 8) lg++;
+    const int groups = NT >> lg;
     uint32_t of_group = mine;
     for (int step = 1; step < (1 << lg); step *= 2) of_group = max(of_group, __shfl_xor_sync(0xffffffffu, of_group, step));
     if ((t & ((1 << lg) - 1)) == 0) sh.key[t >> lg] = of_group;
@@ -491,9 +508,9 @@ __device__ int top_collect(const Span<DT>& sp, TopShared& sh, float mx, int n) {
     }
     __syncthreads();
     const uint32_t tau = sh.tau;
-    constexpr int kStep = kLpAhead * kLpThreads, kGroups = kLpThreads / 8;
-    const int steps = (sp.v1 - sp.v0 + kStep - 1) / kStep, shift = top_shift_of(steps), pieces = ((steps + (1 << shift) - 1) >> shift) * kGroups;
-    for (int i = t; i < pieces; i += kLpThreads)
+    constexpr int kStep = kLpAhead * NT, kGroups = NT / 8;
+    const int steps = (sp.v1 - sp.v0 + kStep - 1) / kStep, shift = top_shift_of<NT>(steps), pieces = ((steps + (1 << shift) - 1) >> shift) * kGroups;
+    for (int i = t; i < pieces; i += NT)
         if (sh.piece[i] >= tau) {
             const int at = atomicAdd(&sh.nhot, 1);
             if (at < kTopHot) sh.hot[at] = (short)i;
@@ -504,16 +521,16 @@ __device__ int top_collect(const Span<DT>& sp, TopShared& sh, float mx, int n) {
     if (nhot <= kTopHot) {
         // the hot pieces' vectors spread over the CTA, four loads ahead
         const int le = 5 + shift, all = nhot << le;
-        for (int i0 = t; i0 < all; i0 += 4 * kLpThreads) {
+        for (int i0 = t; i0 < all; i0 += 4 * NT) {
             uint4 raw[4];
             int at[4];
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                const int i = i0 + q * kLpThreads;
+                const int i = i0 + q * NT;
                 at[q] = sp.v1;
                 if (i < all) {
                     const int piece = sh.hot[i >> le], k = i & ((1 << le) - 1), step = ((piece / kGroups) << shift) + (k >> 5);
-                    at[q] = sp.v0 + step * kStep + ((k >> 3) & 3) * kLpThreads + (piece % kGroups) * 8 + (k & 7);
+                    at[q] = sp.v0 + step * kStep + ((k >> 3) & 3) * NT + (piece % kGroups) * 8 + (k & 7);
                 }
                 if (at[q] < sp.v1) raw[q] = ld_stream(sp.vec + at[q]);
             }
@@ -529,16 +546,16 @@ __device__ int top_collect(const Span<DT>& sp, TopShared& sh, float mx, int n) {
         }
         __syncthreads();
     }
-    if (nhot > kTopHot || sh.ncand > kTopCap) top_exact(sp, sh, n);
-    return min(sh.ncand, kTopCap);      // (a row with NaN may offer more; its list is not used)
+    if (nhot > kTopHot || sh.ncand > TopShared<NT>::kCap) top_exact(sp, sh, n);
+    return min(sh.ncand, TopShared<NT>::kCap);      // (a row with NaN may offer more; its list is not used)
 }
 
 // One cluster of gridDim.x / rows CTAs per row (one CTA: no cluster).  Bound by HBM for many rows, by latency for few.
-template <int DT, bool TOP>
-__global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_constant__ LpParams p, int log_parts) {
+template <int DT, bool TOP, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) lp_rows_kernel(const __grid_constant__ LpParams p, int log_parts) {
     constexpr int E = Elem<DT>::E;
     __shared__ LpShared sh;
-    __shared__ typename std::conditional<TOP, TopShared, int>::type top;
+    __shared__ typename std::conditional<TOP, TopShared<NT>, int>::type top;
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
     const int parts = 1 << log_parts, part = parts > 1 ? (int)cluster_ctarank() : 0;
     const long long r = blockIdx.x >> log_parts;
@@ -547,12 +564,12 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
     sp.share(part, log_parts);
     // steps of kLpAhead vectors a thread, the next step's on their way while one is added; the last one may be a part of one.
     // The first is asked for before the token is known, whose load takes as long.
-    constexpr int kStep = kLpAhead * kLpThreads;
+    constexpr int kStep = kLpAhead * NT;
     uint4 raw[2][kLpAhead];
     auto load = [&](uint4 (&to)[kLpAhead], int v) {
 #pragma unroll
         for (int i = 0; i < kLpAhead; i++)
-            if (v + i * kLpThreads + t < sp.v1) to[i] = ld_stream(sp.vec + v + i * kLpThreads + t);
+            if (v + i * NT + t < sp.v1) to[i] = ld_stream(sp.vec + v + i * NT + t);
     };
     load(raw[0], sp.v0);
     if (row.token < 0 || row.bad_token) {         // not scored: the same for the whole cluster
@@ -585,23 +602,29 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
         stat_one(a, x, c);
         if (TOP) cnt += j < token ? x >= xt : x > xt;
     });
-    const int top_shift = TOP ? top_shift_of((sp.v1 - sp.v0 + kStep - 1) / kStep) : 0;
+    const int top_shift = TOP ? top_shift_of<NT>((sp.v1 - sp.v0 + kStep - 1) / kStep) : 0;
     auto from = [&](int v) { return sp.index(v) < token ? xt : xt_above; };
     auto add = [&](const uint4 (&x)[kLpAhead], int v) {
         float most = -INFINITY;
         if (v + kStep <= sp.v1) {
             most = stat_add<DT>(a, x, c);
             if (TOP) {
+                typename Elem<DT>::Count n = Elem<DT>::none();
 #pragma unroll
-                for (int i = 0; i < kLpAhead; i++) cnt += Elem<DT>::reach(x[i], from(v + i * kLpThreads + t));
+                for (int i = 0; i < kLpAhead; i++) Elem<DT>::reach(n, x[i], from(v + i * NT + t));
+                cnt += Elem<DT>::whole(n);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < kLpAhead; i++)
-                if (v + i * kLpThreads + t < sp.v1) {
+                if (v + i * NT + t < sp.v1) {
                     const uint4 one[1] = {x[i]};
                     most = fmaxf(most, stat_add<DT>(a, one, c));
-                    if (TOP) cnt += Elem<DT>::reach(x[i], from(v + i * kLpThreads + t));
+                    if (TOP) {
+                        typename Elem<DT>::Count n = Elem<DT>::none();
+                        Elem<DT>::reach(n, x[i], from(v + i * NT + t));
+                        cnt += Elem<DT>::whole(n);
+                    }
                 }
         }
         if constexpr (TOP) top_note(top, (v - sp.v0) / kStep, top_shift, most);
@@ -609,7 +632,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
     int v = sp.v0;
     if (TOP && p.tokens) {             // the token's own vector, if it begins before the token, is counted from xt on throughout
         const int own = token >= sp.head && token < sp.tail() ? (token - sp.head) / E : -1;
-        if (own >= sp.v0 && own < sp.v1 && (own - sp.v0) % kLpThreads == t && sp.index(own) < token) {
+        if (own >= sp.v0 && own < sp.v1 && (own - sp.v0) % NT == t && sp.index(own) < token) {
             float x[E];
             widen<DT>(ld_stream(sp.vec + own), x);
 #pragma unroll
@@ -637,9 +660,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
     if (parts > 1) cluster_wait();                // every CTA of the cluster runs: its shared memory may be written
     if (w == 0) {
         Stat b = {-INFINITY, -1.f, 0.f};
-        if (lane < kLpThreads / 32) b = {sh.mx[lane], sh.s[lane], sh.u[lane]};
+        if (lane < NT / 32) b = {sh.mx[lane], sh.s[lane], sh.u[lane]};
         b = stat_warp(b, c);
-        int n = TOP ? (int)warp_sum_u32(lane < kLpThreads / 32 ? (uint32_t)sh.cnt[lane] : 0u) : 0;
+        int n = TOP ? (int)warp_sum_u32(lane < NT / 32 ? (uint32_t)sh.cnt[lane] : 0u) : 0;
         if (parts > 1) {
             if (lane == 0) {
                 st_cluster_f32(map_to_cta(smem_addr(&sh.c_mx[part]), 0), b.mx);
@@ -655,7 +678,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
     if constexpr (TOP) {
         const int n = p.top_n;
         const int nc = top_collect(sp, top, my_mx, n);
-        for (int i = t; i < nc; i += kLpThreads) {
+        for (int i = t; i < nc; i += NT) {
             const unsigned long long e = top.cand[i];
             int at = 0;
 #pragma unroll 8
@@ -706,7 +729,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
         const int all = parts * n;
         if (parts == 1) {
             if (t < n) put(top.list[t], t);          // in order already
-        } else if (all <= kLpThreads / 2) {
+        } else if (all <= NT / 2) {
             if (t < all) {
                 const unsigned long long e = top.list[t];
                 int at = 0;
@@ -721,11 +744,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
             for (int q = 0; q < parts; q++) least = min(least, top.list[q * n + share - 1]);
             if (t == 0) top.ncand = 0;
             __syncthreads();
-            for (int i = t; i < all; i += kLpThreads)
+            for (int i = t; i < all; i += NT)
                 if (top.list[i] && top.list[i] >= least) top.cand[atomicAdd(&top.ncand, 1)] = top.list[i];
             __syncthreads();
             const int nc = top.ncand;
-            for (int i = t; i < nc; i += kLpThreads) {
+            for (int i = t; i < nc; i += NT) {
                 const unsigned long long e = top.cand[i];
                 int at = 0;
 #pragma unroll 8
@@ -740,8 +763,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_rows_kernel(const __grid_con
 // ---- gradient -------------------------------------------------------------------------------------------------------
 // With d = (x - m) c - log2 s, p = 2^d, every element is p (A + D d); the token's own also has g/T, and the two are taken together
 // as -expm1(log p) so that a token of probability nearly one keeps its digits.  Logits and gradient pass once.
-template <int DT>
-__global__ void __launch_bounds__(kLpThreads, 4) lp_backward_kernel(const __grid_constant__ LpParams p) {
+template <int DT, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) lp_backward_kernel(const __grid_constant__ LpParams p) {
     constexpr int E = Elem<DT>::E;
     using T = typename Elem<DT>::T;
     const uint32_t r32 = blockIdx.x / (unsigned)p.chunks;
@@ -758,9 +781,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_backward_kernel(const __grid
         const T zero = Elem<DT>::to(0.f);
         sp.singles(t, [&](int j, float) { out[j] = zero; });
         if (together) {
-            for (int v = sp.v0 + t; v < sp.v1; v += kLpThreads) __stcs(vec + v, make_uint4(0u, 0u, 0u, 0u));
+            for (int v = sp.v0 + t; v < sp.v1; v += NT) __stcs(vec + v, make_uint4(0u, 0u, 0u, 0u));
         } else {
-            for (int j = sp.index(sp.v0) + t, j1 = sp.index(sp.v1); j < j1; j += kLpThreads) out[j] = zero;
+            for (int j = sp.index(sp.v0) + t, j1 = sp.index(sp.v1); j < j1; j += NT) out[j] = zero;
         }
         return;
     }
@@ -796,17 +819,17 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_backward_kernel(const __grid
             __stcs(vec + at, Elem<DT>::narrow(x));
         };
         // as in the forward pass: the next step's loads are on their way while one is computed and stored
-        constexpr int kStep = kLpAhead * kLpThreads;
+        constexpr int kStep = kLpAhead * NT;
         uint4 raw[2][kLpAhead];
         auto load = [&](uint4 (&to)[kLpAhead], int v) {
 #pragma unroll
             for (int i = 0; i < kLpAhead; i++)
-                if (v + i * kLpThreads + t < sp.v1) to[i] = ld_stream(sp.vec + v + i * kLpThreads + t);
+                if (v + i * NT + t < sp.v1) to[i] = ld_stream(sp.vec + v + i * NT + t);
         };
         auto step = [&](const uint4 (&x)[kLpAhead], int v) {
 #pragma unroll
             for (int i = 0; i < kLpAhead; i++)
-                if (v + i * kLpThreads + t < sp.v1) one(x[i], v + i * kLpThreads + t);
+                if (v + i * NT + t < sp.v1) one(x[i], v + i * NT + t);
         };
         int v = sp.v0;
         load(raw[0], v);
@@ -821,9 +844,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_backward_kernel(const __grid
         }
         // the token's own, behind the store of its vector by the same thread
         const int own = token >= sp.head && token < sp.tail() ? (token - sp.head) / E : -1;
-        if (own >= sp.v0 && own < sp.v1 && (own - sp.v0) % kLpThreads == t) out[token] = Elem<DT>::to(grad_at(Elem<DT>::one(sp.row + token)));
+        if (own >= sp.v0 && own < sp.v1 && (own - sp.v0) % NT == t) out[token] = Elem<DT>::to(grad_at(Elem<DT>::one(sp.row + token)));
     } else {                           // they start at different places of their 16 bytes: element by element
-        for (int j = sp.index(sp.v0) + t, j1 = sp.index(sp.v1); j < j1; j += kLpThreads) {
+        for (int j = sp.index(sp.v0) + t, j1 = sp.index(sp.v1); j < j1; j += NT) {
             const float x = Elem<DT>::one(sp.row + j);
             out[j] = Elem<DT>::to(j == token ? grad_at(x) : grad(x));
         }
@@ -864,9 +887,9 @@ static int lp_params(const rs_logprob_call* k, bool needs_tokens, LpParams* p, H
     return RS_OK;
 }
 
-template <int DT, bool TOP>
+template <int DT, bool TOP, int NT>
 static int lp_launch(const LpParams& p, int parts, cudaStream_t stream) {
-    auto kern = lp_rows_kernel<DT, TOP>;
+    auto kern = lp_rows_kernel<DT, TOP, NT>;
     if (parts > 8) {
         static std::mutex mu;
         static bool done[64] = {};      // per device
@@ -884,7 +907,7 @@ static int lp_launch(const LpParams& p, int parts, cudaStream_t stream) {
     memset(&cfg, 0, sizeof cfg);
     const int log_parts = 31 - __builtin_clz((unsigned)parts);
     cfg.gridDim = dim3((unsigned)(p.rows * parts));
-    cfg.blockDim = dim3(kLpThreads);
+    cfg.blockDim = dim3(NT);
     cfg.stream = stream;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -904,15 +927,38 @@ static int lp_parts(long long rows, int V, int sms) {
     while (parts < 16 && rows * parts < 2LL * sms && V / (2 * parts) >= 4096) parts *= 2;
     return parts;
 }
+// Threads of a CTA that has a row to itself.  A row's fixed costs, about 3 us, are hidden by the other rows on its
+// multiprocessor, and the fewer threads a row has the more of them there are (16 of 64, 8 of 128, 4 of 256); long rows need
+// the loads in flight of many threads.  us at 64 / 128 / 256 threads, bf16, statistics and a list of 20:
+//   16384 rows of 1024: 35 / 37 / 64 and 113 / 124 / more;  of 4096: 46 / 43 / 74 and 159 / 134 / 217;
+//   7629 of 65536: 175 / 153 / 158 and 426 / 283 / 287;  3290 of 151936: 179 / 155 / 155 and 489 / 297 / 249.
+static int lp_threads(int V, int size, int top_n) {
+    const int bytes = V * size;
+    if (bytes <= 4096) return top_n > 40 ? 128 : 64;
+    return bytes <= 131072 ? 128 : 256;
+}
 
+template <bool TOP, int NT>
+static int lp_typed(const LpParams& p, int dtype, int parts, cudaStream_t stream) {
+    switch (dtype) {
+        case RS_DTYPE_F32: return lp_launch<RS_DTYPE_F32, TOP, NT>(p, parts, stream);
+        case RS_DTYPE_F16: return lp_launch<RS_DTYPE_F16, TOP, NT>(p, parts, stream);
+        default: return lp_launch<RS_DTYPE_BF16, TOP, NT>(p, parts, stream);
+    }
+}
 template <bool TOP>
 static int lp_dispatch(const LpParams& p, int dtype, int sms, cudaStream_t stream) {
     const int parts = lp_parts(p.rows, p.V, sms);
-    switch (dtype) {
-        case RS_DTYPE_F32: return lp_launch<RS_DTYPE_F32, TOP>(p, parts, stream);
-        case RS_DTYPE_F16: return lp_launch<RS_DTYPE_F16, TOP>(p, parts, stream);
-        default: return lp_launch<RS_DTYPE_BF16, TOP>(p, parts, stream);
-    }
+    const int threads = parts > 1 ? 256 : lp_threads(p.V, dtype == RS_DTYPE_F32 ? 4 : 2, TOP ? p.top_n : 0);
+    if (threads == 64) return lp_typed<TOP, 64>(p, dtype, parts, stream);
+    if (threads == 128) return lp_typed<TOP, 128>(p, dtype, parts, stream);
+    return lp_typed<TOP, 256>(p, dtype, parts, stream);
+}
+template <int DT>
+static void lp_backward(const LpParams& p, int threads, unsigned grid, cudaStream_t st) {
+    if (threads == 64) lp_backward_kernel<DT, 64><<<grid, 64, 0, st>>>(p);
+    else if (threads == 128) lp_backward_kernel<DT, 128><<<grid, 128, 0, st>>>(p);
+    else lp_backward_kernel<DT, 256><<<grid, 256, 0, st>>>(p);
 }
 
 int host_status_word(int** out) {
@@ -977,12 +1023,13 @@ int rs_token_logprobs_backward(const rs_logprob_call* call, const float* entropy
     const long long chunks = (vectors + piece - 1) / piece;
     p.piece = (int)piece;
     p.chunks = (int)chunks;
+    const int threads = rs::lp_threads((int)call->V, (int)size, 0);
     const unsigned grid = (unsigned)(p.rows * chunks);
     cudaStream_t st = (cudaStream_t)call->stream;
     switch (call->dtype) {
-        case RS_DTYPE_F32: rs::lp_backward_kernel<RS_DTYPE_F32><<<grid, rs::kLpThreads, 0, st>>>(p); break;
-        case RS_DTYPE_F16: rs::lp_backward_kernel<RS_DTYPE_F16><<<grid, rs::kLpThreads, 0, st>>>(p); break;
-        default: rs::lp_backward_kernel<RS_DTYPE_BF16><<<grid, rs::kLpThreads, 0, st>>>(p);
+        case RS_DTYPE_F32: rs::lp_backward<RS_DTYPE_F32>(p, threads, grid, st); break;
+        case RS_DTYPE_F16: rs::lp_backward<RS_DTYPE_F16>(p, threads, grid, st); break;
+        default: rs::lp_backward<RS_DTYPE_BF16>(p, threads, grid, st);
     }
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return rs::host_cuda_fail(e, "launch(logprobs backward)");

@@ -182,6 +182,19 @@ def test_large_logits_crowded_in_few_threads(dtype, E):
     check_all(x, t, 1.0, top_n=64, grads=False)
 
 
+@pytest.mark.parametrize("V,rows", [(1000, 3), (9000, 300), (70000, 300)])
+def test_large_logits_crowded_in_rows_of_one_cta(V, rows):
+    """The same where a row has one CTA, of each size; most rows ordinary, so that other CTAs run beside."""
+    x, t = make((rows,), V, "f32", 25, sigma=0.1)
+    j = torch.arange(V, device="cuda")
+    for r, (every, width) in enumerate([(1024, 64), (2048, 300), (512, 8)]):
+        crowd = (j % every) < width
+        x[r, crowd] = 5 + torch.rand(int(crowd.sum()), device="cuda")
+    x[rows - 1] = 1.0
+    check_all(x, t, 1.0, top_n=64, grads=False)
+    check_all(x, t, 1.0, top_n=3, grads=False)
+
+
 def test_confident_rows_keep_their_digits():
     """log p = -log1p(the rest) where p is nearly 1: relative, not absolute, accuracy (three roundings and the sum's error).
     The rest's terms are added apart from the maximum's own 1 but for those of the one thread that holds it, in which they
