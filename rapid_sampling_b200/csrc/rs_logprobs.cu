@@ -371,12 +371,12 @@ struct LpShared {
 // (Rows of CTAs with fewer than 256 threads are short and not shared.)
 template <int NT>
 struct TopShared {
-    static constexpr int kCap = NT == 256 ? 1024 : 640;            // candidates for a list
-    static constexpr int kPieces = NT == 256 ? 128 : 16;           // steps that the maxima of pieces are kept of
+    static constexpr int kCap = 640;                               // candidates for a list
+    static constexpr int kPieces = NT == 256 ? 32 : NT == 128 ? 16 : 2;      // steps that the maxima of pieces are kept of
     alignas(16) uint32_t key[NT];
     unsigned long long cand[kCap];
     unsigned long long list[(NT == 256 ? 16 : 1) * kTopMax];       // the cluster's lists of top_n entries, in the first CTA; 0: none
-    uint32_t piece[kPieces * NT / 8];
+    alignas(16) uint32_t piece[kPieces * NT];
     short hot[kTopHot];
     int nhot, nfinite, ncand, count;
     uint32_t tau;
@@ -387,7 +387,7 @@ __device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
 
-// The maxima of pieces, eight threads' vectors of a step or, in long parts, of 2^shift steps: where a list's entries are.
+// The maxima of pieces, a thread's vectors of a step or, in long parts, of 2^shift steps: where a list's entries are.
 template <int NT>
 __device__ __forceinline__ int top_shift_of(int steps) {
     constexpr int most = TopShared<NT>::kPieces;
@@ -395,13 +395,9 @@ __device__ __forceinline__ int top_shift_of(int steps) {
 }
 template <int NT>
 __device__ __forceinline__ void top_note(TopShared<NT>& sh, int step, int shift, float most) {
-    uint32_t k = key_of(most);
-#pragma unroll
-    for (int o = 1; o < 8; o *= 2) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
-    if ((threadIdx.x & 7) == 0) {
-        uint32_t* at = sh.piece + (step >> shift) * (NT / 8) + threadIdx.x / 8;
-        *at = (step & ((1 << shift) - 1)) ? max(*at, k) : k;
-    }
+    uint32_t* at = sh.piece + (step >> shift) * NT + threadIdx.x;
+    const uint32_t k = key_of(most);
+    *at = (step & ((1 << shift) - 1)) ? max(*at, k) : k;
 }
 template <int NT>
 __device__ __forceinline__ void top_push(TopShared<NT>& sh, uint32_t key, int j) {
@@ -508,19 +504,21 @@ __device__ int top_collect(const Span<DT>& sp, TopShared<NT>& sh, float mx, int 
     }
     __syncthreads();
     const uint32_t tau = sh.tau;
-    constexpr int kStep = kLpAhead * NT, kGroups = NT / 8;
-    const int steps = (sp.v1 - sp.v0 + kStep - 1) / kStep, shift = top_shift_of<NT>(steps), pieces = ((steps + (1 << shift) - 1) >> shift) * kGroups;
-    for (int i = t; i < pieces; i += NT)
-        if (sh.piece[i] >= tau) {
-            const int at = atomicAdd(&sh.nhot, 1);
-            if (at < kTopHot) sh.hot[at] = (short)i;
-        }
+    constexpr int kStep = kLpAhead * NT;
+    const int steps = (sp.v1 - sp.v0 + kStep - 1) / kStep, shift = top_shift_of<NT>(steps), pieces = ((steps + (1 << shift) - 1) >> shift) * NT;
+    if (mine >= tau)                               // a thread's own pieces
+        for (int i = t; i < pieces; i += NT)
+            if (sh.piece[i] >= tau) {
+                const int at = atomicAdd(&sh.nhot, 1);
+                if (at < kTopHot) sh.hot[at] = (short)i;
+            }
     sp.singles(t, [&](int j, float x) { if (key_of(x) >= tau) top_push(sh, key_of(x), j); });
     __syncthreads();
     const int nhot = sh.nhot;
     if (nhot <= kTopHot) {
         // the hot pieces' vectors spread over the CTA, four loads ahead
-        const int le = 5 + shift, all = nhot << le;
+        static_assert(kLpAhead == 4, "vectors of a piece");
+        const int le = 2 + shift, all = nhot << le;
         for (int i0 = t; i0 < all; i0 += 4 * NT) {
             uint4 raw[4];
             int at[4];
@@ -529,8 +527,8 @@ __device__ int top_collect(const Span<DT>& sp, TopShared<NT>& sh, float mx, int 
                 const int i = i0 + q * NT;
                 at[q] = sp.v1;
                 if (i < all) {
-                    const int piece = sh.hot[i >> le], k = i & ((1 << le) - 1), step = ((piece / kGroups) << shift) + (k >> 5);
-                    at[q] = sp.v0 + step * kStep + ((k >> 3) & 3) * NT + (piece % kGroups) * 8 + (k & 7);
+                    const int piece = sh.hot[i >> le], k = i & ((1 << le) - 1), step = ((piece / NT) << shift) + (k >> 2);
+                    at[q] = sp.v0 + step * kStep + (k & 3) * NT + piece % NT;
                 }
                 if (at[q] < sp.v1) raw[q] = ld_stream(sp.vec + at[q]);
             }
@@ -740,19 +738,20 @@ __global__ void __launch_bounds__(NT, 1024 / NT) lp_rows_kernel(const __grid_con
         } else {
             // every list's first ceil(n / parts) entries are n in all: what lies below the least of those is not among the n largest
             const int share = (n + parts - 1) >> log_parts;
+            unsigned long long* left = reinterpret_cast<unsigned long long*>(top.piece);      // up to parts * top_n; the pieces have served
             unsigned long long least = ~0ull;
             for (int q = 0; q < parts; q++) least = min(least, top.list[q * n + share - 1]);
             if (t == 0) top.ncand = 0;
             __syncthreads();
             for (int i = t; i < all; i += NT)
-                if (top.list[i] && top.list[i] >= least) top.cand[atomicAdd(&top.ncand, 1)] = top.list[i];
+                if (top.list[i] && top.list[i] >= least) left[atomicAdd(&top.ncand, 1)] = top.list[i];
             __syncthreads();
             const int nc = top.ncand;
             for (int i = t; i < nc; i += NT) {
-                const unsigned long long e = top.cand[i];
+                const unsigned long long e = left[i];
                 int at = 0;
 #pragma unroll 8
-                for (int q = 0; q < nc; q++) at += top.cand[q] > e;
+                for (int q = 0; q < nc; q++) at += left[q] > e;
                 if (at < n) put(e, at);
             }
             if (t >= nc && t < n) put(0ull, t);
