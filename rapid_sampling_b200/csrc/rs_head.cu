@@ -298,6 +298,7 @@ struct HeadParams {
 
 constexpr int kHeadMaxWorkers = 160;      // CTAs that the workspace has slots for
 constexpr int kHeadMaxStages = 12;
+constexpr uint32_t kHeadDrainPolls = 1u << 16;      // limit of the waits for what is in flight after a wait ran out, whatever its own limit
 
 // One lane of a converged warp.  The copying and the multiplying warp run their loops with all lanes and only issue with one:
 // uniform control flow keeps descriptors and coordinates in uniform registers (a loop of one lane alone took 1200 cycles a unit).
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(192, 1)
             const uint32_t k = it - 1 - i, st = k % stages, parity = (k / stages) & 1u;
             if (!ok || !wait(empty + 8 * st, parity)) {
                 ok = false;
-                mbar_wait_bounded(full + 8 * st, parity, p.polls);
+                mbar_wait_bounded(full + 8 * st, parity, kHeadDrainPolls);
             }
         }
     } else if (w == W + 1) {
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(192, 1)
                 if (++s == stages) { s = 0; ph ^= 1u; }
             }
         // (after a wait that ran out: the products in flight end by themselves)
-        if (!ok && it > 0) mbar_wait_bounded(sfull + 8 * ((it - 1) % BUFS), ((it - 1) / BUFS) & 1u, p.polls);
+        if (!ok && it > 0) mbar_wait_bounded(sfull + 8 * ((it - 1) % BUFS), ((it - 1) / BUFS) & 1u, kHeadDrainPolls);
     } else {
         const int row = w * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(w * 32) << 16);
@@ -744,7 +745,7 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
             const uint32_t k = it - 1 - i, st = k % stages, parity = (k / stages) & 1u;
             if (!ok || !wait(empty + 8 * st, parity)) {
                 ok = false;
-                if (rank == 0) mbar_wait_bounded(full + 8 * st, parity, p.polls);
+                if (rank == 0) mbar_wait_bounded(full + 8 * st, parity, kHeadDrainPolls);
             }
         }
     } else if (w == W + 1) {
@@ -777,7 +778,7 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
                     __syncwarp();
                     if (++s == stages) { s = 0; ph ^= 1u; }
                 }
-            if (!ok && it > 0) mbar_wait_bounded(sfull + 8 * ((it - 1) & 1u), ((it - 1) >> 1) & 1u, p.polls);
+            if (!ok && it > 0) mbar_wait_bounded(sfull + 8 * ((it - 1) & 1u), ((it - 1) >> 1) & 1u, kHeadDrainPolls);
         }
     } else {
         const int quad = w & 3, col0 = (w >> 2) * COLS, row = quad * 32 + lane;

@@ -68,6 +68,7 @@ void raise_pending_status(int device, at::Tensor& ws, cudaStream_t stream) {
     if (v == 0) return;
     *w = 0;
     rs_clear_status(ws.data_ptr(), stream);
+    if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) rs_logprobs_status(stream);
     throw_status("an earlier sampling call", device, v);
 }
 

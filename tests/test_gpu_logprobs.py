@@ -413,3 +413,65 @@ def test_follows_a_sampling_call():
     # the sampler's probability is a 32-bit softmax of its own: 2e-6 relative
     assert bool(((lp.exp() - prob).abs() <= 2e-5 * prob).all())
     assert bool((rank <= 40).all()) and torch.equal(top_ids.gather(1, (rank.long() - 1)[:, None])[:, 0], ids)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_subnormal_logits_are_ordered(dtype):
+    """Values below the smallest normal one differ and are counted and listed in their order."""
+    V = 2500
+    step = {"f32": 2.0 ** -149, "f16": 2.0 ** -24, "bf16": 2.0 ** -133}[dtype]
+    k = torch.arange(V, device="cuda") * 37 % 101 - 50
+    x = (k.double() * step).to(DT[dtype])[None].repeat(3, 1)
+    assert len(x.float().unique()) == 101
+    check_all(x, torch.tensor([0, 1200, 2499], device="cuda"), 1.0, top_n=64)
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    """Nothing needs a call outside a capture first."""
+    import subprocess
+    import sys
+    code = """
+import torch, rapid_sampling_b200 as rs
+x = torch.randn(6, 5000, device="cuda"); t = torch.randint(0, 5000, (6,), device="cuda")
+w = torch.randn(5000, 256, device="cuda"); h = {m: torch.randn(m, 256, device="cuda") for m in (4, 50, 200)}
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a = rs.batch_token_logprobs(x, t) + rs.batch_top_logprobs(x, 5, t)
+    codes, scales = rs.lm_head_quantize(w)
+    b = [rs.lm_head_logits(v, codes, scales) for v in h.values()]
+g.replay(); torch.cuda.synchronize()
+want = rs.batch_token_logprobs(x, t) + rs.batch_top_logprobs(x, 5, t)
+assert all(torch.equal(p, q) for p, q in zip(a, want))
+c2, s2 = rs.lm_head_quantize(w)
+assert torch.equal(codes.float(), c2.float()) and torch.equal(scales, s2)
+assert all(torch.equal(p, rs.lm_head_logits(v, c2, s2)) for p, v in zip(b, h.values()))
+print("fine")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+def test_calls_from_several_threads():
+    """Two host threads with streams of their own."""
+    import threading
+    import rapid_sampling_b200 as rs
+    codes, scales = rs.lm_head_quantize(torch.randn(3000, 512, device="cuda") * 0.05)
+    data = [(make((9,), 20000, "bf16", 40 + i), torch.randn(70 * (i + 1), 512, device="cuda")) for i in range(2)]
+    want = [(rs.batch_top_logprobs(x, 10, t), rs.lm_head_logits(h, codes, scales)) for (x, t), h in data]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        (x, t), h = data[i]
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(50):
+                a, b = rs.batch_top_logprobs(x, 10, t), rs.lm_head_logits(h, codes, scales)
+            st.synchronize()
+            if not (all(torch.equal(p, q) for p, q in zip(a, want[i][0])) and torch.equal(b, want[i][1])):
+                wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [th.start() for th in threads]
+    [th.join() for th in threads]
+    assert not wrong
