@@ -289,7 +289,8 @@ struct HeadParams {
     int token_tiles;         // more tokens: tiles of 128, or of 256 for pairs
     int stages;
     int boxes;               // pairs: the copy engine stores the result
-    int wide_store;          // more tokens, else: bytes of a store that the result's rows allow (32, 16, or 0: one by one)
+    int wide_store;          // more tokens, else: bytes of a store that the result's rows allow (32, 16, or 0)
+    int turn_at;             // offset in shared memory of what head_store_turned needs
     float* partial;          // split work: two slots a CTA
     int* arrived;            // split work: workers done with the tile that begins in a worker's run
     uint32_t polls;
@@ -577,50 +578,71 @@ template <> __device__ __forceinline__ uint32_t head_word<__nv_bfloat16>(float a
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// COLS neighbours of a row: `wide` bytes a store where the rows allow it, else one by one
+// COLS neighbours of a row, or the first `cols` of them, 32 or 16 bytes a store.
 template <int COLS, typename OUT>
 __device__ __forceinline__ void head_store(OUT* o, const uint64_t (&acc)[COLS / 2], int cols, int wide) {
     constexpr int PER32 = 32 / (int)sizeof(OUT);
-    if (wide && cols >= COLS) {
 #pragma unroll
-        for (int i = 0; i < COLS; i += PER32) {
-            uint32_t x[8];
-            if constexpr (sizeof(OUT) == 4) {
+    for (int i = 0; i < COLS; i += PER32) {
+        uint32_t x[8];
+        if constexpr (sizeof(OUT) == 4) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    float a, b;
-                    f2_unpack(acc[i / 2 + j], a, b);
-                    x[2 * j] = __float_as_uint(a);
-                    x[2 * j + 1] = __float_as_uint(b);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    float a, b;
-                    f2_unpack(acc[i / 2 + j], a, b);
-                    x[j] = head_word<OUT>(a, b);
-                }
+            for (int j = 0; j < 4; j++) {
+                float a, b;
+                f2_unpack(acc[i / 2 + j], a, b);
+                x[2 * j] = __float_as_uint(a);
+                x[2 * j + 1] = __float_as_uint(b);
             }
-            if (wide == 32) {
-                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o + i), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]),
-                             "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
-                             : "memory");
-            } else {
-                *reinterpret_cast<uint4*>(o + i) = make_uint4(x[0], x[1], x[2], x[3]);
-                *reinterpret_cast<uint4*>(o + i + PER32 / 2) = make_uint4(x[4], x[5], x[6], x[7]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                float a, b;
+                f2_unpack(acc[i / 2 + j], a, b);
+                x[j] = head_word<OUT>(a, b);
             }
         }
-    } else {
+        if (i + PER32 > cols) {
 #pragma unroll
-        for (int i = 0; i < COLS / 2; i++) {
+            for (int j = 0; j < PER32; j++) {
+                float a, b;
+                f2_unpack(acc[(i + j) / 2], a, b);
+                OUT z;
+                head_to(z, j & 1 ? b : a);
+                if (i + j < cols) o[i + j] = z;
+            }
+        } else if (wide == 32) {
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o + i), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]),
+                         "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+                         : "memory");
+        } else {
+            *reinterpret_cast<uint4*>(o + i) = make_uint4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<uint4*>(o + i + PER32 / 2) = make_uint4(x[4], x[5], x[6], x[7]);
+        }
+    }
+}
+// A warp's 32 rows by COLS columns where the rows allow no wide stores (a store of one element a row each took 50 us for 1293
+// rows of 2931 fp16, the products 5): 32 columns at a time by way of shared memory (rows of 33 words: no bank twice), then row by row, neighbours of a row from neighbouring lanes.
+constexpr int kTurnBytes = 32 * 33 * 4;
+template <int COLS, typename OUT>
+__device__ __forceinline__ void head_store_turned(OUT* o, long long ldo, float* buf, const uint64_t (&acc)[COLS / 2], int lane, int rows, int cols) {
+#pragma unroll
+    for (int c0 = 0; c0 < COLS; c0 += 32) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
             float a, b;
-            f2_unpack(acc[i], a, b);
-            OUT z;
-            head_to(z, a);
-            if (2 * i < cols) o[2 * i] = z;
-            head_to(z, b);
-            if (2 * i + 1 < cols) o[2 * i + 1] = z;
+            f2_unpack(acc[c0 / 2 + i], a, b);
+            buf[lane * 33 + 2 * i] = a;
+            buf[lane * 33 + 2 * i + 1] = b;
         }
+        __syncwarp();
+        if (c0 + lane < cols)
+#pragma unroll 8
+            for (int r = 0; r < min(rows, 32); r++) {
+                OUT z;
+                head_to(z, buf[r * 33 + lane]);
+                __stcs(o + r * ldo + c0 + lane, z);
+            }
+        __syncwarp();
     }
 }
 
@@ -860,8 +882,14 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
             if (PAIR && p.boxes) {
                 if (!dead && m - lane < p.M && v0 < p.V)
                     head_store_box<COLS, OUT>(&map_out, base + stages * stage_bytes + (uint32_t)(w * kStoreBytes), acc, lane, m - lane, v0, p.V);
-            } else if (m < p.M && !dead) {
-                head_store<COLS, OUT>((OUT*)p.out + (long long)m * p.ldo + v0, acc, p.V - v0, p.wide_store);
+            } else if (!dead && m - lane < p.M && v0 < p.V) {
+                OUT* o = (OUT*)p.out + (long long)(m - lane) * p.ldo + v0;
+                if (p.wide_store) {
+                    if (m < p.M) head_store<COLS, OUT>(o + lane * p.ldo, acc, p.V - v0, p.wide_store);
+                } else {
+                    float* buf = reinterpret_cast<float*>(raw_smem + (base - smem_addr(raw_smem)) + p.turn_at + (uint32_t)(w * kTurnBytes));
+                    head_store_turned<COLS, OUT>(o, p.ldo, buf, acc, lane, p.M - (m - lane), p.V - v0);
+                }
             }
         }
         if (PAIR && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -1105,7 +1133,9 @@ int rs_head_logits(const void* hidden, int32_t hidden_dtype, int64_t M, int64_t 
     const uintptr_t step = (uintptr_t)out_device | (uintptr_t)out_stride * os;
     p.wide_store = step % 32 == 0 ? 32 : step % 16 == 0 ? 16 : 0;
     p.boxes = pair && p.wide_store;
-    const int tail = few ? 0 : p.boxes ? kMoreAdders * kStoreBytes : head_more_tail(pair, p.n), room = dev.smem_optin - 2048 - 1024 - tail;
+    // behind the stages: the boxes to store, or what the products read beyond the last stage and the rows to turn
+    const int tail = few ? 0 : p.boxes ? kMoreAdders * kStoreBytes : head_more_tail(pair, p.n) + (p.wide_store ? 0 : kMoreAdders * kTurnBytes);
+    const int room = dev.smem_optin - 2048 - 1024 - tail;
     p.stages = room / per > kHeadMaxStages ? kHeadMaxStages : room / per;
     CUtensorMap w, x, out;
     if ((rc = head_map(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes_device, V, K, K, few || pair ? 128 : 256)) ||
@@ -1119,6 +1149,7 @@ int rs_head_logits(const void* hidden, int32_t hidden_dtype, int64_t M, int64_t 
         if ((rc = head_map(&out, type, (int)os, out_device, M, V, (long long)(out_stride * (int64_t)os), 32))) return rc;
     }
     if ((rc = head_quantize<true>(hidden, hidden_dtype, hidden_stride, M, K, ws, sa, p.pitch, p.arrived, (cudaStream_t)stream))) return rc;
+    p.turn_at = p.stages * per + (few ? 0 : head_more_tail(pair, p.n));
     const int smem = p.stages * per + tail + 1024;
     switch (out_dtype) {
         case RS_DTYPE_F32: return head_run<float>(w, x, out, p, smem, (cudaStream_t)stream);
