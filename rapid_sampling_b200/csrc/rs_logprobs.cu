@@ -920,10 +920,13 @@ static int lp_launch(const LpParams& p, int parts, cudaStream_t stream) {
     return RS_OK;
 }
 
-// CTAs per row: enough of them that every multiprocessor has two, as long as each keeps 4096 logits to read.
+// CTAs per row: enough of them that every multiprocessor has two, as long as each keeps 4096 logits to read; clusters of 16, which
+// the device places less freely, only for up to 18 rows.  us for statistics / a list of 20, V = 151936, f32, at 1, 2, 4, 8 CTAs:
+// 100 rows 34 / 44, 22 / 31, 16 / 24, 19 / 29; 300 rows 40 / 52, 42 / 57; 32 rows bf16 at 1, 8, 16: 16 / 30, 8 / 15, 11 / 19.
 static int lp_parts(long long rows, int V, int sms) {
+    const int most = rows * 16 <= 2LL * sms ? 16 : 8;
     int parts = 1;
-    while (parts < 16 && rows * parts < 2LL * sms && V / (2 * parts) >= 4096) parts *= 2;
+    while (parts < most && rows * parts < 2LL * sms && V / (2 * parts) >= 4096) parts *= 2;
     return parts;
 }
 // Threads of a CTA that has a row to itself.  A row's fixed costs, about 3 us, are hidden by the other rows on its
