@@ -324,6 +324,66 @@ struct HeadWait {
         return false;
     }
 };
+// A thread's sums of one row and `cols` tokens in a slot of the workspace: four tokens of 128 rows together, so that both the
+// threads' 16 bytes and a warp's 512 are contiguous.
+template <int COLS>
+__device__ __forceinline__ void head_leave(float* slot, int row, int col0, int cols, const uint64_t (&acc)[COLS / 2]) {
+#pragma unroll
+    for (int i = 0; i < COLS; i += 4) {
+        float4 v;
+        f2_unpack(acc[i / 2], v.x, v.y);
+        f2_unpack(acc[i / 2 + 1], v.z, v.w);
+        if (i < cols) __stcg(reinterpret_cast<float4*>(slot + ((col0 + i) / 4 * 128 + row) * 4), v);
+    }
+}
+template <int COLS>
+__device__ __forceinline__ void head_fetch(const float* slot, int row, int col0, int cols, uint64_t (&acc)[COLS / 2]) {      // adds
+#pragma unroll
+    for (int i = 0; i < COLS; i += 4) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < cols) v = __ldcg(reinterpret_cast<const float4*>(slot + ((col0 + i) / 4 * 128 + row) * 4));
+        acc[i / 2] = f2_add(acc[i / 2], f2_pack(v.x, v.y));
+        acc[i / 2 + 1] = f2_add(acc[i / 2 + 1], f2_pack(v.z, v.w));
+    }
+}
+// Ends a shared tile's segment (few tokens), called by all adding threads (THREADS of them, barrier 1): returns whether this
+// worker was the tile's last, and then its sums are the whole tile's.  Slot 1 of a worker is for the tile that begins in its
+// run, slot 0 for the one that began in an earlier one.  Of two workers the last keeps its own sums in registers, and does not
+// write them if the other's are there already, as they nearly always are (64 tokens: 152 -> 145 us); of more than two, all are
+// added in their order.  (Not inlined: the loop around it needs the registers.)
+template <int THREADS, int COLS>
+__device__ __noinline__ bool head_share(const HeadParams& p, int slot_floats, int tile, int worker, bool begins, int row, int col0, int cols,
+                                        uint64_t (&acc)[COLS / 2], int* flag) {
+    const long long u = (long long)tile * p.work.blocks;
+    const int first = p.work.owner(u), last = p.work.owner(u + p.work.blocks - 1), needed = last - first + 1;
+    int* const counter = p.arrived + first;
+    auto slot = [&](int w) { return p.partial + (long long)(2 * w + (w == first)) * slot_floats; };
+    auto vote = [&](bool mine) {                  // thread 0's word, to all
+        if (threadIdx.x == 0) *flag = mine;
+        asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+        const bool v = *(volatile int*)flag;
+        asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+        return v;
+    };
+    bool end = needed == 2 && vote(threadIdx.x == 0 && atomicAdd(counter, 0) == 1);
+    if (!end) {
+        head_leave<COLS>(p.partial + (long long)(2 * worker + begins) * slot_floats, row, col0, cols, acc);
+        __threadfence();
+        asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+        end = vote(threadIdx.x == 0 && atomicAdd(counter, 1) == needed - 1);
+        if (!end) return false;
+    }
+    __threadfence();
+    if (needed == 2) {
+        head_fetch<COLS>(slot(worker == first ? last : first), row, col0, cols, acc);
+    } else {
+#pragma unroll
+        for (int i = 0; i < COLS / 2; i++) acc[i] = 0ull;
+        for (int w = first; w <= last; w++) head_fetch<COLS>(slot(w), row, col0, cols, acc);
+    }
+    return true;
+}
+
 // Called by the adding threads (THREADS of them, barrier 1) after they have written their sums of a tile they share.
 // Returns whether this CTA is the last, and then sees the others' sums.
 template <int THREADS>
@@ -338,18 +398,18 @@ __device__ __forceinline__ bool head_last(const HeadParams& p, int counter, int 
 }
 
 // ---- few tokens -----------------------------------------------------------------------------------------------------------
-// 128 rows of weights are the accumulator's lanes and all tokens (at most 32) its columns, so that the tensor core's work is
-// small; the time is that of the weights' bytes.  Warps 0 .. 3 add the blocks' sums up, each thread one row by all tokens; then
+// 128 rows of weights are the accumulator's lanes and all tokens (at most 64) its columns, so that the tensor core's work is
+// small; the time is that of the weights' bytes.  Warps 0 .. W-1 add the blocks' sums up, each thread one row by 32 tokens; then
 // one warp that copies and one that multiplies.  A ring of stages and four accumulators keep the three apart.  A step is two
 // blocks: waits and arrivals, about 150 cycles each between products, are paid once for both.
-constexpr int kFewTokens = 32, kFewBufs = 4;
+constexpr int kFewTokens = 64, kFewBufs = 4;
 // weights of both blocks, tokens of both, the tokens' scales of both
 __host__ __device__ constexpr int head_few_stage(int n) { return 2 * 128 * 128 + 2 * n * 128 + 1024; }
 
-template <typename OUT>
-__global__ void __launch_bounds__(192, 1)
+template <int NT, typename OUT>
+__global__ void __launch_bounds__(NT * 4 + 64, 1)
     head_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ HeadParams p) {
-    constexpr int W = 4, NT = kFewTokens, BUFS = kFewBufs;
+    constexpr int W = NT / 8, COLS = 32, BUFS = kFewBufs;
     constexpr uint32_t kTmemCols = BUFS * 2 * NT;
     extern __shared__ uint8_t raw_smem[];
     __shared__ uint64_t full_[kHeadMaxStages], empty_[kHeadMaxStages], sfull_[BUFS], sempty_[BUFS];
@@ -440,17 +500,17 @@ __global__ void __launch_bounds__(192, 1)
         // (after a wait that ran out: the products in flight end by themselves)
         if (!ok && it > 0) mbar_wait_bounded(sfull + 8 * ((it - 1) % BUFS), ((it - 1) / BUFS) & 1u, kHeadDrainPolls);
     } else {
-        const int row = w * 32 + lane;
-        const uint32_t lanes = tmem + ((uint32_t)(w * 32) << 16);
+        const int quad = w & 3, row = quad * 32 + lane, col0 = (w >> 2) * COLS, cols = p.M - col0;
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)col0;
         uint32_t it = 0, s = 0;
         bool dead = false;                        // after a wait that ran out: no more waits, but every barrier of the adding warps
         float scale[2] = {0.f, 0.f};              // of the weights' blocks: these 32 and the next, one a lane
         while (walk.next()) {
             const float* sw = p.sw + (long long)walk.tile * p.work.blocks;
             scale[0] = walk.b0 + lane < walk.b1 ? __ldg(sw + walk.b0 + lane) : 0.f;
-            uint64_t acc[NT / 2];
+            uint64_t acc[COLS / 2];
 #pragma unroll
-            for (int i = 0; i < NT / 2; i++) acc[i] = 0ull;
+            for (int i = 0; i < COLS / 2; i++) acc[i] = 0ull;
             for (int b = walk.b0; b < walk.b1; b += 2, it++) {
                 const uint32_t buf = it % BUFS;
                 const int q = (b - walk.b0) & 31;
@@ -467,15 +527,15 @@ __global__ void __launch_bounds__(192, 1)
                 for (int h = 0; h < 2; h++) {
                     if (b + h < walk.b1) {
                         const uint64_t ff = h ? f2_pack(f1, f1) : f2_pack(f0, f0);
-                        uint32_t v[NT];
+                        uint32_t v[COLS];
                         tmem_ld32(lanes + buf * 2 * NT + h * NT, v);      // (columns behind the last token: not looked at)
                         tmem_ld_wait();
 #pragma unroll
-                        for (int c = 0; c < NT; c += 16)
-                            if (c < p.n) {
+                        for (int c = 0; c < COLS; c += 16)
+                            if (col0 + c < p.n) {
 #pragma unroll
                                 for (int i = c; i < c + 16; i += 4) {
-                                    const ulonglong2 g = sa[(h * p.n + i) / 4];
+                                    const ulonglong2 g = sa[(h * p.n + col0 + i) / 4];
                                     acc[i / 2] = f2_fma(f2_pack(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), f2_mul(g.x, ff), acc[i / 2]);
                                     acc[i / 2 + 1] = f2_fma(f2_pack(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), f2_mul(g.y, ff), acc[i / 2 + 1]);
                                 }
@@ -490,35 +550,25 @@ __global__ void __launch_bounds__(192, 1)
                 }
                 if (++s == stages) s = 0;
             }
-            float y[NT];
-#pragma unroll
-            for (int i = 0; i < NT / 2; i++) f2_unpack(acc[i], y[2 * i], y[2 * i + 1]);
             if (!walk.whole()) {
-                // slot 1: the tile begins in this run; slot 0: it began in an earlier one
-                float* mine = p.partial + (long long)(2 * (int)blockIdx.x + (walk.b0 == 0)) * 128 * p.n;
+                uint64_t sums[COLS / 2];
 #pragma unroll
-                for (int i = 0; i < NT; i++)
-                    if (i < p.M) mine[i * 128 + row] = y[i];
-                const long long u = (long long)walk.tile * p.work.blocks;
-                const int c0 = p.work.owner(u), c1 = p.work.owner(u + p.work.blocks - 1);
-                if (!head_last<W * 32>(p, c0, c1 - c0 + 1, &flag)) continue;
+                for (int i = 0; i < COLS / 2; i++) sums[i] = acc[i];
+                if (!head_share<W * 32, COLS>(p, 128 * NT, walk.tile, blockIdx.x, walk.b0 == 0, row, col0, cols, sums, &flag)) continue;
 #pragma unroll
-                for (int i = 0; i < NT; i++) y[i] = 0.f;
-                for (int c = c0; c <= c1; c++) {
-                    const float* from = p.partial + (long long)(2 * c + (c == c0)) * 128 * p.n;
-#pragma unroll
-                    for (int i = 0; i < NT; i++)
-                        if (i < p.M) y[i] += __ldcg(from + i * 128 + row);
-                }
+                for (int i = 0; i < COLS / 2; i++) acc[i] = sums[i];
             }
+            float y[COLS];
+#pragma unroll
+            for (int i = 0; i < COLS / 2; i++) f2_unpack(acc[i], y[2 * i], y[2 * i + 1]);
             const int v = walk.tile * 128 + row;
             if (v < p.V && !dead) {
-                OUT* o = (OUT*)p.out + v;
+                OUT* o = (OUT*)p.out + (long long)col0 * p.ldo + v;
 #pragma unroll
-                for (int i = 0; i < NT; i++) {
+                for (int i = 0; i < COLS; i++) {
                     OUT z;
                     head_to(z, y[i]);
-                    if (i < p.M) __stcs(o + i * p.ldo, z);
+                    if (i < cols) __stcs(o + i * p.ldo, z);
                 }
             }
         }
@@ -973,10 +1023,11 @@ static int head_launch(KERN kern, int threads, int smem, int grid, int cluster, 
 }
 template <typename OUT>
 static int head_run(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& out, const HeadParams& p, int smem, cudaStream_t stream) {
-    static bool done[3][64] = {};      // per device
+    static bool done[4][64] = {};      // per device
     const int n = p.work.workers;
-    if (p.M <= kFewTokens) return head_launch(head_few_kernel<OUT>, 192, smem, n, 1, stream, done[0], w, x, p);
-    if (p.M <= 128) return head_launch(head_more_kernel<false, OUT>, kMoreThreads, smem, n, 1, stream, done[1], w, x, out, p);
+    if (p.M <= 32) return head_launch(head_few_kernel<32, OUT>, 192, smem, n, 1, stream, done[0], w, x, p);
+    if (p.M <= kFewTokens) return head_launch(head_few_kernel<64, OUT>, 320, smem, n, 1, stream, done[1], w, x, p);
+    if (p.M <= 128) return head_launch(head_more_kernel<false, OUT>, kMoreThreads, smem, n, 1, stream, done[3], w, x, out, p);
     return head_launch(head_more_kernel<true, OUT>, kMoreThreads, smem, 2 * n, 2, stream, done[2], w, x, out, p);
 }
 
@@ -1040,7 +1091,7 @@ static int head_pitch(long long M) { return (int)((M + 255) / 256 * 256) + 256; 
 struct HeadLayout { size_t scales, arrived, partial, total; };
 static HeadLayout head_layout(long long M, long long K) {
     HeadLayout l;
-    const size_t blocks = (size_t)((K + 127) / 128), n = M <= kFewTokens ? (size_t)(M + 15) / 16 * 16 : 256;
+    const size_t blocks = (size_t)((K + 127) / 128), n = M <= 32 ? 32 : M <= kFewTokens ? 64 : 256;
     l.scales = ((size_t)M * (size_t)K + 255) / 256 * 256;
     l.arrived = l.scales + blocks * (size_t)head_pitch(M) * 4;
     l.partial = l.arrived + 2 * kHeadMaxWorkers * 4;
