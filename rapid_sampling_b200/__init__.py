@@ -79,9 +79,9 @@ def batch_token_logprobs(logits, tokens, temperature=1.0):
     Unlike the sampling calls, nothing is replaced: -inf masks a token; a row of nothing but -inf has log probability -inf,
     entropy 0 and gradient 0; NaN or +inf makes its row NaN.  A token >= V gives NaN and no gradient, a temperature outside
     [0.001, 1000] in a tensor counts as 1, and either raises ValueError from the next call on the device."""
-    if isinstance(temperature, (int, float)):
-        return _load_ext().token_logprobs(logits, tokens, temperature, None)
-    return _load_ext().token_logprobs(logits, tokens, 1.0, temperature)
+    if hasattr(temperature, "is_cuda"):
+        return _load_ext().token_logprobs(logits, tokens, 1.0, temperature)
+    return _load_ext().token_logprobs(logits, tokens, float(temperature), None)
 
 
 def batch_top_logprobs(logits, top_n, tokens=None, temperature=1.0):
@@ -91,9 +91,9 @@ def batch_top_logprobs(logits, top_n, tokens=None, temperature=1.0):
 
     Slots behind the last token that a mask of -inf leaves hold -inf and id -1; so do all slots of a position that is not
     scored (negative token; rank 0).  Rows with NaN or +inf: NaN, id -1, rank 0.  Not differentiable."""
-    if isinstance(temperature, (int, float)):
-        return _load_ext().top_logprobs(logits, top_n, tokens, temperature, None)
-    return _load_ext().top_logprobs(logits, top_n, tokens, 1.0, temperature)
+    if hasattr(temperature, "is_cuda"):
+        return _load_ext().top_logprobs(logits, top_n, tokens, 1.0, temperature)
+    return _load_ext().top_logprobs(logits, top_n, tokens, float(temperature), None)
 
 
 def lm_head_quantize(weight):

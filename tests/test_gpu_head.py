@@ -292,3 +292,42 @@ def test_vocab_parallel_sampling_from_hidden_states(B, V_local, penalised):
                 lambda: VocabParallelSampler(B, V_local, 0, 1, T=2).project(hidden, codes, scales, st_a, 0.8, 50, 0.9)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_weights_beyond_32_bits():
+    """Codes whose offsets pass 2^31, made and multiplied."""
+    import rapid_sampling_b200 as rs
+    K = 16384
+    V = 2 ** 31 // K + 1000
+    w = torch.zeros(V, K, dtype=torch.bfloat16, device="cuda")
+    some = list(range(128)) + list(range(V - 300, V))
+    w[some] = make(len(some), K, "bf16", 1, 0.02)
+    codes, scales = rs.lm_head_quantize(w)
+    blocks = sorted({v // 128 for v in some})
+    rows = torch.tensor([v for b in blocks for v in range(128 * b, min(128 * b + 128, V))], device="cuda")
+    want, want_scales = quantized(w[rows], 128)
+    assert torch.equal(scales[blocks], want_scales) and torch.equal(codes[rows].double(), want)
+    values = wide(want, want_scales, 128)
+    for M in (2, 40, 100, 130):
+        hidden = make(M, K, "bf16", M)
+        got = rs.lm_head_logits(hidden, codes, scales)[:, rows].double()
+        a = wide(*quantized(hidden, 1), 1)
+        bound = (128 + K // 128 + 2) * 2.0 ** -23 * (a.abs() @ values.abs().t()) + 2.0 ** -24 * (a @ values.t()).abs()
+        assert bool(((got - a @ values.t()).abs() <= bound + 1e-30).all())
+
+
+def test_results_beyond_32_bits():
+    """A result of more than 2^31 elements, aligned and not."""
+    import rapid_sampling_b200 as rs
+    K, V, M = 16, 1048579, 2100
+    codes, scales = rs.lm_head_quantize(make(V, K, "bf16", 1, 0.02))
+    hidden = make(M, K, "bf16", 2)
+    for columns in (V, V - 3):
+        got = rs.lm_head_logits(hidden, codes[:columns], scales[:-(-columns // 128)], dtype=torch.bfloat16)
+        for rows, cols in ((slice(0, 3), slice(0, 300)), (slice(M - 5, M), slice(columns - 300, columns))):
+            first = (columns - 300) // 128 * 128 if cols.start else 0
+            want = rs.lm_head_logits(hidden[rows], codes[first:columns], scales[first // 128:-(-columns // 128)], dtype=torch.float32)
+            want = want[:, -300:] if cols.start else want[:, :300]
+            # the same products to the last bits of fp32, rounded to bf16
+            assert bool(((got[rows, cols].float() - want).abs() <= 2.0 ** -8 * want.abs() * 1.001 + 1e-6).all())
+        del got
