@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) lp_rows_kernel(const __grid_con
         float most = -INFINITY;
         if (v + kStep <= sp.v1) {
             most = stat_add<DT>(a, x, c);
-            if (TOP) {
+            if (TOP && most >= xt) {      // nothing to count otherwise: nearly always, where the token is a likely one
                 typename Elem<DT>::Count n = Elem<DT>::none();
 #pragma unroll
                 for (int i = 0; i < kLpAhead; i++) Elem<DT>::reach(n, x[i], from(v + i * NT + t));
@@ -617,8 +617,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) lp_rows_kernel(const __grid_con
             for (int i = 0; i < kLpAhead; i++)
                 if (v + i * NT + t < sp.v1) {
                     const uint4 one[1] = {x[i]};
-                    most = fmaxf(most, stat_add<DT>(a, one, c));
-                    if (TOP) {
+                    const float here = stat_add<DT>(a, one, c);
+                    most = fmaxf(most, here);
+                    if (TOP && here >= xt) {
                         typename Elem<DT>::Count n = Elem<DT>::none();
                         Elem<DT>::reach(n, x[i], from(v + i * NT + t));
                         cnt += Elem<DT>::whole(n);
