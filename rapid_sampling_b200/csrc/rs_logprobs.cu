@@ -368,15 +368,16 @@ struct LpShared {
     float c_mx[16], c_s[16], c_u[16];
     int c_cnt[16];
 };
-// (Rows of CTAs with fewer than 256 threads are short and not shared.)
-template <int NT>
+// SHARED: the row is a cluster's.  Small, because what it takes is lost to the loads in flight, which pass through L1.
+template <int NT, bool SHARED>
 struct TopShared {
+    static constexpr int kThreads = NT;
     static constexpr int kCap = 640;                               // candidates for a list
-    static constexpr int kPieces = NT == 256 ? 32 : NT == 128 ? 16 : 2;      // steps that the maxima of pieces are kept of
+    static constexpr int kPieces = NT == 64 ? 2 : 16;              // steps that the maxima of pieces are kept of
     alignas(16) uint32_t key[NT];
     unsigned long long cand[kCap];
-    unsigned long long list[(NT == 256 ? 16 : 1) * kTopMax];       // the cluster's lists of top_n entries, in the first CTA; 0: none
-    alignas(16) uint32_t piece[kPieces * NT];
+    unsigned long long list[(SHARED ? 16 : 1) * kTopMax];          // the cluster's lists of top_n entries, in the first CTA; 0: none
+    alignas(16) uint16_t piece[kPieces * NT];                      // upper halves of keys
     short hot[kTopHot];
     int nhot, nfinite, ncand, count;
     uint32_t tau;
@@ -387,26 +388,27 @@ __device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
 
-// The maxima of pieces, a thread's vectors of a step or, in long parts, of 2^shift steps: where a list's entries are.
-template <int NT>
+// The maxima of pieces, a thread's vectors of a step or, in long parts, of 2^shift steps: where a list's entries are.  The
+// upper half of a key is kept: all of a 16-bit logit's, and of a 32-bit one's enough.
+template <class TS>
 __device__ __forceinline__ int top_shift_of(int steps) {
-    constexpr int most = TopShared<NT>::kPieces;
-    return steps <= most ? 0 : 32 - __clz((steps - 1) / most);
+    return steps <= TS::kPieces ? 0 : 32 - __clz((steps - 1) / TS::kPieces);
 }
-template <int NT>
-__device__ __forceinline__ void top_note(TopShared<NT>& sh, int step, int shift, float most) {
-    uint32_t* at = sh.piece + (step >> shift) * NT + threadIdx.x;
-    const uint32_t k = key_of(most);
-    *at = (step & ((1 << shift) - 1)) ? max(*at, k) : k;
+template <class TS>
+__device__ __forceinline__ void top_note(TS& sh, int step, int shift, float most) {
+    uint16_t* at = sh.piece + (step >> shift) * TS::kThreads + threadIdx.x;
+    const uint32_t k = key_of(most) >> 16;
+    *at = (uint16_t)((step & ((1 << shift) - 1)) ? max((uint32_t)*at, k) : k);
 }
-template <int NT>
-__device__ __forceinline__ void top_push(TopShared<NT>& sh, uint32_t key, int j) {
+template <class TS>
+__device__ __forceinline__ void top_push(TS& sh, uint32_t key, int j) {
     const int at = atomicAdd(&sh.ncand, 1);
-    if (at < TopShared<NT>::kCap) sh.cand[at] = ((unsigned long long)key << 32) | (uint32_t)~j;
+    if (at < TS::kCap) sh.cand[at] = ((unsigned long long)key << 32) | (uint32_t)~j;
 }
 // Elements of the CTA's part with a key of at least `at_least`.
-template <int DT, int NT>
-__device__ int top_count(const Span<DT>& sp, TopShared<NT>& sh, uint32_t at_least) {
+template <int DT, class TS>
+__device__ int top_count(const Span<DT>& sp, TS& sh, uint32_t at_least) {
+    constexpr int NT = TS::kThreads;
     constexpr int E = Elem<DT>::E;
     __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
@@ -427,8 +429,9 @@ __device__ int top_count(const Span<DT>& sp, TopShared<NT>& sh, uint32_t at_leas
 // order of their indices.  For parts whose n largest elements are not told apart by the threads' maxima: long runs of equal
 // logits, or large ones that crowd in few threads.  About 32 passes over the part at worst, 2 where the threads' n-th
 // largest maximum is the key, as with a mask of the type's lowest value.
-template <int DT, int NT>
-__device__ void top_exact(const Span<DT>& sp, TopShared<NT>& sh, int n) {
+template <int DT, class TS>
+__device__ void top_exact(const Span<DT>& sp, TS& sh, int n) {
+    constexpr int NT = TS::kThreads;
     constexpr int E = Elem<DT>::E;
     const int t = threadIdx.x;
     uint32_t lo = sh.tau, hi = 0xFF800001u;        // count(lo) >= n > count(hi): nothing lies above +inf's key
@@ -475,8 +478,9 @@ __device__ void top_exact(const Span<DT>& sp, TopShared<NT>& sh, int n) {
 // The n largest elements of the CTA's part (larger key first, then lower index), unordered, among sh.cand[0 .. result).
 // At least n threads have a maximum that reaches the n-th largest maximum of the groups, so the list lies within the elements
 // that reach it too, and those are in the few pieces whose maximum does: only they are read again.
-template <int DT, int NT>
-__device__ int top_collect(const Span<DT>& sp, TopShared<NT>& sh, float mx, int n) {
+template <int DT, class TS>
+__device__ int top_collect(const Span<DT>& sp, TS& sh, float mx, int n) {
+    constexpr int NT = TS::kThreads;
     constexpr int E = Elem<DT>::E;
     const int t = threadIdx.x;
     const uint32_t mine = key_of(mx);
@@ -505,10 +509,10 @@ __device__ int top_collect(const Span<DT>& sp, TopShared<NT>& sh, float mx, int 
     __syncthreads();
     const uint32_t tau = sh.tau;
     constexpr int kStep = kLpAhead * NT;
-    const int steps = (sp.v1 - sp.v0 + kStep - 1) / kStep, shift = top_shift_of<NT>(steps), pieces = ((steps + (1 << shift) - 1) >> shift) * NT;
+    const int steps = (sp.v1 - sp.v0 + kStep - 1) / kStep, shift = top_shift_of<TS>(steps), pieces = ((steps + (1 << shift) - 1) >> shift) * NT;
     if (mine >= tau)                               // a thread's own pieces
         for (int i = t; i < pieces; i += NT)
-            if (sh.piece[i] >= tau) {
+            if (sh.piece[i] >= tau >> 16) {
                 const int at = atomicAdd(&sh.nhot, 1);
                 if (at < kTopHot) sh.hot[at] = (short)i;
             }
@@ -544,18 +548,20 @@ __device__ int top_collect(const Span<DT>& sp, TopShared<NT>& sh, float mx, int 
         }
         __syncthreads();
     }
-    if (nhot > kTopHot || sh.ncand > TopShared<NT>::kCap) top_exact(sp, sh, n);
-    return min(sh.ncand, TopShared<NT>::kCap);      // (a row with NaN may offer more; its list is not used)
+    if (nhot > kTopHot || sh.ncand > TS::kCap) top_exact(sp, sh, n);
+    return min(sh.ncand, TS::kCap);      // (a row with NaN may offer more; its list is not used)
 }
 
 // One cluster of gridDim.x / rows CTAs per row (one CTA: no cluster).  Bound by HBM for many rows, by latency for few.
-template <int DT, bool TOP, int NT>
+template <int DT, bool TOP, int NT, bool SHARED>
 __global__ void __launch_bounds__(NT, 1024 / NT) lp_rows_kernel(const __grid_constant__ LpParams p, int log_parts) {
     constexpr int E = Elem<DT>::E;
     __shared__ LpShared sh;
-    __shared__ typename std::conditional<TOP, TopShared<NT>, int>::type top;
+    using TS = TopShared<NT, SHARED>;
+    __shared__ typename std::conditional<TOP, TS, int>::type top;
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-    const int parts = 1 << log_parts, part = parts > 1 ? (int)cluster_ctarank() : 0;
+    if (!SHARED) log_parts = 0;
+    const int parts = 1 << log_parts, part = SHARED ? (int)cluster_ctarank() : 0;
     const long long r = blockIdx.x >> log_parts;
     const LpRow row = lp_row(p, (uint32_t)r);
     Span<DT> sp(p, row);
@@ -600,7 +606,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) lp_rows_kernel(const __grid_con
         stat_one(a, x, c);
         if (TOP) cnt += j < token ? x >= xt : x > xt;
     });
-    const int top_shift = TOP ? top_shift_of<NT>((sp.v1 - sp.v0 + kStep - 1) / kStep) : 0;
+    const int top_shift = TOP ? top_shift_of<TS>((sp.v1 - sp.v0 + kStep - 1) / kStep) : 0;
     auto from = [&](int v) { return sp.index(v) < token ? xt : xt_above; };
     auto add = [&](const uint4 (&x)[kLpAhead], int v) {
         float most = -INFINITY;
@@ -887,9 +893,9 @@ static int lp_params(const rs_logprob_call* k, bool needs_tokens, LpParams* p, H
     return RS_OK;
 }
 
-template <int DT, bool TOP, int NT>
+template <int DT, bool TOP, int NT, bool SHARED>
 static int lp_launch(const LpParams& p, int parts, cudaStream_t stream) {
-    auto kern = lp_rows_kernel<DT, TOP, NT>;
+    auto kern = lp_rows_kernel<DT, TOP, NT, SHARED>;
     if (parts > 8) {
         static std::mutex mu;
         static bool done[64] = {};      // per device
@@ -941,21 +947,22 @@ static int lp_threads(int V, int size, int top_n) {
     return bytes <= 131072 ? 128 : 256;
 }
 
-template <bool TOP, int NT>
+template <bool TOP, int NT, bool SHARED>
 static int lp_typed(const LpParams& p, int dtype, int parts, cudaStream_t stream) {
     switch (dtype) {
-        case RS_DTYPE_F32: return lp_launch<RS_DTYPE_F32, TOP, NT>(p, parts, stream);
-        case RS_DTYPE_F16: return lp_launch<RS_DTYPE_F16, TOP, NT>(p, parts, stream);
-        default: return lp_launch<RS_DTYPE_BF16, TOP, NT>(p, parts, stream);
+        case RS_DTYPE_F32: return lp_launch<RS_DTYPE_F32, TOP, NT, SHARED>(p, parts, stream);
+        case RS_DTYPE_F16: return lp_launch<RS_DTYPE_F16, TOP, NT, SHARED>(p, parts, stream);
+        default: return lp_launch<RS_DTYPE_BF16, TOP, NT, SHARED>(p, parts, stream);
     }
 }
 template <bool TOP>
 static int lp_dispatch(const LpParams& p, int dtype, int sms, cudaStream_t stream) {
     const int parts = lp_parts(p.rows, p.V, sms);
-    const int threads = parts > 1 ? 256 : lp_threads(p.V, dtype == RS_DTYPE_F32 ? 4 : 2, TOP ? p.top_n : 0);
-    if (threads == 64) return lp_typed<TOP, 64>(p, dtype, parts, stream);
-    if (threads == 128) return lp_typed<TOP, 128>(p, dtype, parts, stream);
-    return lp_typed<TOP, 256>(p, dtype, parts, stream);
+    if (parts > 1) return lp_typed<TOP, 256, true>(p, dtype, parts, stream);
+    const int threads = lp_threads(p.V, dtype == RS_DTYPE_F32 ? 4 : 2, TOP ? p.top_n : 0);
+    if (threads == 64) return lp_typed<TOP, 64, false>(p, dtype, 1, stream);
+    if (threads == 128) return lp_typed<TOP, 128, false>(p, dtype, 1, stream);
+    return lp_typed<TOP, 256, false>(p, dtype, 1, stream);
 }
 template <int DT>
 static void lp_backward(const LpParams& p, int threads, unsigned grid, cudaStream_t st) {
