@@ -263,7 +263,7 @@ static rs_logprob_call logprob_call(const at::Tensor& logits, const c10::optiona
         const at::Tensor& t = *row_temperature;
         if (t.scalar_type() != at::kFloat || !t.is_cuda() || t.get_device() != logits.get_device())
             throw std::invalid_argument("temperature must be a float32 CUDA tensor on the logits' device !\n");
-        if (t.dim() == 0) {
+        if (t.numel() == 1) {      // strides 0: for every row
         } else if (t.sizes() == rows) {
             c.temperature_stride_b = d >= 2 ? t.stride(0) : 0;
             c.temperature_stride_t = d == 3 ? t.stride(1) : 0;

@@ -475,3 +475,15 @@ def test_calls_from_several_threads():
     [th.start() for th in threads]
     [th.join() for th in threads]
     assert not wrong
+
+
+def test_one_temperature_in_a_tensor_of_any_shape():
+    import rapid_sampling_b200 as rs
+    for rows in ((5,), (2, 3), ()):
+        x, t = make(rows, 1000, "f32", 60)
+        t = t.reshape(rows)
+        want = rs.batch_top_logprobs(x, 5, t, 0.625)
+        for shape in ((), (1,), (1, 1)):
+            one = torch.full(shape, 0.625, device="cuda")
+            assert all(torch.equal(a, b) for a, b in zip(rs.batch_top_logprobs(x, 5, t, one), want))
+            assert torch.equal(rs.batch_token_logprobs(x, t, one)[0], rs.batch_token_logprobs(x, t, 0.625)[0])
