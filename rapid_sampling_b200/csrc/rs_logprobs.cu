@@ -247,6 +247,8 @@ __device__ __forceinline__ LpRow lp_row(const LpParams& p, uint32_t r) {
     o.c = __fdiv_rn(kLog2e, t);
     return o;
 }
+// (x - m) / T; by way of halves, whose difference is finite however far apart the two lie
+__device__ __forceinline__ float lp_scaled(float x, float m, float inv_t) { return (0.5f * x - 0.5f * m) * (2.f * inv_t); }
 __device__ __forceinline__ void lp_report(const LpParams& p, int code) {
     atomicExch(&g_lp_status, code);
     if (p.mirror) *reinterpret_cast<volatile int*>(p.mirror) = code;
@@ -713,7 +715,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) lp_rows_kernel(const __grid_con
             const bool bad = !(b.mx < INFINITY), none = b.mx == -INFINITY;
             const float nan = __int_as_float(0x7FC00000);
             const float logs = log1pf(b.s);
-            const float lp = bad ? nan : none ? -INFINITY : (xt - b.mx) * row.inv_t - logs;
+            const float lp = bad ? nan : none ? -INFINITY : lp_scaled(xt, b.mx, row.inv_t) - logs;
             const float ent = bad ? nan : none ? 0.f : logs - b.u / (1.f + b.s) * 0.6931471805599453f;
             if (p.logprob) p.logprob[r] = lp;
             if (p.entropy) p.entropy[r] = ent;
@@ -732,7 +734,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) lp_rows_kernel(const __grid_con
         const float mx = sh.r_mx, logs = sh.r_logs;
         const bool bad = !(mx < INFINITY);
         auto put = [&](unsigned long long e, int at) {      // e = 0: a slot that stays empty
-            p.top[r * n + at] = bad ? __int_as_float(0x7FC00000) : e ? (of_key((uint32_t)(e >> 32)) - mx) * row.inv_t - logs : -INFINITY;
+            p.top[r * n + at] = bad ? __int_as_float(0x7FC00000) : e ? lp_scaled(of_key((uint32_t)(e >> 32)), mx, row.inv_t) - logs : -INFINITY;
             p.top_ids[r * n + at] = bad || !e ? -1 : (int)~(uint32_t)e;
         };
         const int all = parts * n;

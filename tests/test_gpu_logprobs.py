@@ -487,3 +487,11 @@ def test_one_temperature_in_a_tensor_of_any_shape():
             one = torch.full(shape, 0.625, device="cuda")
             assert all(torch.equal(a, b) for a, b in zip(rs.batch_top_logprobs(x, 5, t, one), want))
             assert torch.equal(rs.batch_token_logprobs(x, t, one)[0], rs.batch_token_logprobs(x, t, 0.625)[0])
+
+
+def test_logits_further_apart_than_the_largest_number():
+    """Their difference over the temperature is finite: a log probability is its correctly scaled value."""
+    x = torch.tensor([[3e38, -3e38, 0.0, 2.9e38], [-3.4e38, 3.4e38, -math.inf, 1e38]], device="cuda")
+    for temperature in (2.0, 4.0, 1000.0):
+        for token in range(4):
+            check_all(x, torch.full((2,), token, device="cuda"), temperature)
