@@ -481,6 +481,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("top_p"));
     m.def("batch_sampling_temperature_topk_topp", &batch_sampling_temperature_topk_topp, py::arg("logits"),
           py::arg("states"), py::arg("temperature"), py::arg("top_k"), py::arg("top_p"));
+        if (out.requires_grad() && at::GradMode::is_enabled())
+            throw std::invalid_argument("out must not require a gradient: the call is not differentiable !\n");
     m.def("batch_sampling_temperature_topk_topp_any", &sample_any, py::arg("logits"), py::arg("states"),
           py::arg("temperature"), py::arg("top_k"), py::arg("top_p"));
     m.def("batch_sampling_repetition_temperature_topk_topp_any", &sample_repetition_any, py::arg("logits"),
@@ -493,6 +495,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("tokens"), py::arg("temperature"), py::arg("row_temperature"));
     m.def("top_logprobs", &top_logprobs, py::arg("logits"), py::arg("top_n"), py::arg("tokens"), py::arg("temperature"),
           py::arg("row_temperature"));
+    if (out_.has_value() && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();      // graphs that saved `out` notice
     m.def("lm_head_quantize", &lm_head_quantize, py::arg("weight"));
     m.def("lm_head_logits", [](const at::Tensor& hidden, const at::Tensor& codes, const at::Tensor& scales, py::object dtype,
                                c10::optional<at::Tensor> out) {

@@ -331,3 +331,24 @@ def test_results_beyond_32_bits():
             # the same products to the last bits of fp32, rounded to bf16
             assert bool(((got[rows, cols].float() - want).abs() <= 2.0 ** -8 * want.abs() * 1.001 + 1e-6).all())
         del got
+
+
+def test_a_graph_notices_that_its_logits_were_written_over():
+    """log p's backward pass needs the logits: `out` into them must not pass unseen."""
+    import rapid_sampling_b200 as rs
+    codes, scales = rs.lm_head_quantize(make(300, 256, "f32", 1, 0.02))
+    h = make(4, 256, "f32", 2)
+    logits = rs.lm_head_logits(h, codes, scales).requires_grad_(True)
+    lp, _ = rs.batch_token_logprobs(logits, torch.zeros(4, dtype=torch.long, device="cuda"))
+    with pytest.raises(ValueError):
+        rs.lm_head_logits(h, codes, scales, out=logits)
+    with torch.no_grad():
+        rs.lm_head_logits(2 * h, codes, scales, out=logits)
+    with pytest.raises(RuntimeError):
+        lp.sum().backward()
+    with torch.inference_mode():
+        buf = torch.empty(4, 300, device="cuda")
+        rs.lm_head_logits(h, codes, scales, out=buf)
+    before = buf.clone()
+    rs.lm_head_logits(h, codes, scales, out=buf)              # no counter to keep
+    assert torch.equal(buf, before)
