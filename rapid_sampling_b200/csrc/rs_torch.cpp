@@ -4,11 +4,14 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 
 #include <map>
 #include <mutex>
 #include <stdexcept>
 #include <string>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/rapid_sampling_b200.h"
 
@@ -327,6 +330,26 @@ static at::Tensor token_logprobs_backward(const at::Tensor& logits, const at::Te
     return grad;
 }
 
+// Gradients of leaves whose accumulation belongs to the legacy default stream cannot be captured: that stream waits for
+// nothing in a capture, and the engine's attempt ends the process.  A leaf's accumulation keeps its stream as long as a graph of
+// the leaf lives, an earlier eager step's for instance.  So such a backward call is refused.
+static void check_captured_backward(const at::Tensor& logits) {
+    if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
+    const auto start = logits.grad_fn() ? logits.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(logits);
+    std::vector<torch::autograd::Node*> todo = {start.get()};
+    std::unordered_set<torch::autograd::Node*> seen;
+    while (!todo.empty()) {
+        torch::autograd::Node* n = todo.back();
+        todo.pop_back();
+        if (!n || !seen.insert(n).second) continue;
+        const auto s = dynamic_cast<torch::autograd::AccumulateGrad*>(n) ? n->stream() : std::nullopt;
+        if (s && s->device_type() == c10::DeviceType::CUDA && *s == at::cuda::getDefaultCUDAStream(s->device_index()).unwrap())
+            throw std::runtime_error("the backward pass of batch_token_logprobs cannot be captured while an eager graph of the same leaves, made on "
+                                     "the default stream, is alive !\n");
+        for (const auto& e : n->next_edges()) todo.push_back(e.function.get());
+    }
+}
+
 struct RowTemperature {      // no input of the graph
     c10::optional<at::Tensor> t;
 };
@@ -345,6 +368,7 @@ class TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
         if (at::GradMode::is_enabled()) throw std::runtime_error("batch_token_logprobs is differentiable once: no create_graph !\n");
         const auto saved = ctx->get_saved_variables();
+        check_captured_backward(saved[0]);
         at::Tensor grad;
         if (g[0].defined() || g[1].defined()) {
             auto maybe = [](const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
@@ -457,6 +481,8 @@ static at::Tensor lm_head_logits(const at::Tensor& hidden, const at::Tensor& cod
         out = *out_;
         if (!out.is_cuda() || out.get_device() != dev || out.sizes() != at::IntArrayRef(shape) || out.scalar_type() != dtype)
             throw std::invalid_argument("out must have the hidden states' shape with V columns, the requested type, and their device !\n");
+        if (out.requires_grad() && at::GradMode::is_enabled())
+            throw std::invalid_argument("out must not require a gradient: the call is not differentiable !\n");
     } else {
         out = at::empty(shape, at::TensorOptions().dtype(dtype).device(hidden.device()));
     }
@@ -469,6 +495,7 @@ static at::Tensor lm_head_logits(const at::Tensor& hidden, const at::Tensor& cod
     const int rc = rs_head_logits(hidden.data_ptr(), hdt, M, K, step, codes.data_ptr(), scales.data_ptr<float>(), V, out.data_ptr(), odt,
                                   std::max(ostep, V), ws.data_ptr(), (size_t)ws.numel(), stream);
     if (rc != RS_OK) fail(rc, "");
+    if (out_.has_value() && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();      // graphs that saved `out` notice
     return out;
 }
 
@@ -481,8 +508,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("top_p"));
     m.def("batch_sampling_temperature_topk_topp", &batch_sampling_temperature_topk_topp, py::arg("logits"),
           py::arg("states"), py::arg("temperature"), py::arg("top_k"), py::arg("top_p"));
-        if (out.requires_grad() && at::GradMode::is_enabled())
-            throw std::invalid_argument("out must not require a gradient: the call is not differentiable !\n");
     m.def("batch_sampling_temperature_topk_topp_any", &sample_any, py::arg("logits"), py::arg("states"),
           py::arg("temperature"), py::arg("top_k"), py::arg("top_p"));
     m.def("batch_sampling_repetition_temperature_topk_topp_any", &sample_repetition_any, py::arg("logits"),
@@ -495,7 +520,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("tokens"), py::arg("temperature"), py::arg("row_temperature"));
     m.def("top_logprobs", &top_logprobs, py::arg("logits"), py::arg("top_n"), py::arg("tokens"), py::arg("temperature"),
           py::arg("row_temperature"));
-    if (out_.has_value() && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();      // graphs that saved `out` notice
     m.def("lm_head_quantize", &lm_head_quantize, py::arg("weight"));
     m.def("lm_head_logits", [](const at::Tensor& hidden, const at::Tensor& codes, const at::Tensor& scales, py::object dtype,
                                c10::optional<at::Tensor> out) {

@@ -495,3 +495,50 @@ def test_logits_further_apart_than_the_largest_number():
     for temperature in (2.0, 4.0, 1000.0):
         for token in range(4):
             check_all(x, torch.full((2,), token, device="cuda"), temperature)
+
+
+def test_a_backward_pass_captured_beside_an_eager_graph_is_refused():
+    """In a process of its own: without the refusal, torch's engine would end it."""
+    import subprocess
+    import sys
+    code = """
+import torch, rapid_sampling_b200 as rs
+t = torch.randint(0, 5000, (6,), device="cuda")
+h = torch.randn(6, 64, device="cuda")
+for weight in (None, torch.randn(64, 5000, device="cuda", requires_grad=True)):
+    leaf = torch.randn(6, 5000, device="cuda", requires_grad=True) if weight is None else weight
+    logits = (lambda: leaf) if weight is None else (lambda: h @ leaf)
+    def step():
+        loss = rs.batch_token_logprobs(logits(), t)[0].sum()
+        loss.backward()
+        return loss
+    kept = rs.batch_token_logprobs(logits(), t)[0].sum()          # an eager graph that stays
+    leaf.grad = torch.zeros_like(leaf)
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    except RuntimeError as e:
+        assert "alive" in str(e), e
+    else:
+        raise SystemExit("not refused")
+    torch.cuda.synchronize()
+    kept.backward()                                               # the process and the graph go on
+    want = leaf.grad.clone()
+    del kept
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    leaf.grad.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.allclose(leaf.grad, want, rtol=0, atol=1e-4)
+print("fine")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout[-500:] + r.stderr[-2000:]
