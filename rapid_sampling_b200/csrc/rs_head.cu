@@ -18,6 +18,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cmath>
 #include <cstring>
 #include <mutex>
 
@@ -250,8 +251,8 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int
 // ---- how the work is split ----------------------------------------------------------------------------------------------
 // A unit is one tile of the result and one block of 128 columns of K; unit u = tile * blocks + block.  Either every worker (a
 // CTA, or a pair of them) takes whole tiles in turn, or the units are cut into equal runs of neighbours (`split`), so that all
-// workers end together however many tiles there are.  Then a tile may lie in the runs of several workers: each leaves its
-// sums in the workspace, and the one that is done last adds them up in the order of the workers.
+// workers end together however many tiles there are; head_split decides.  In runs a tile may lie with several workers: each
+// leaves its sums in the workspace, and the one that is done last adds them up in a fixed order.
 struct HeadWork {
     long long units;
     int workers, blocks, tiles, split;
@@ -290,8 +291,8 @@ struct HeadParams {
     long long ldo;
     HeadWork work;
     int M, V, pitch;
-    int n;                   // rows of tokens a stage holds, a multiple of 16
-    int token_tiles;         // more tokens: tiles of 128, or of 256 for pairs
+    int n;                   // rows of tokens that a CTA brings, a multiple of 16 and at most 128
+    int token_tiles;         // more tokens: tiles of 128, or of 256 for pairs (few: 1)
     int stages;
     int boxes;               // pairs: the copy engine stores the result
     int wide_store;          // more tokens, else: bytes of a store that the result's rows allow (32, 16, or 0)
@@ -587,11 +588,12 @@ __global__ void __launch_bounds__(NT * 4 + 64, 1)
 
 // ---- more tokens ------------------------------------------------------------------------------------------------------------
 // The tokens are the accumulator's lanes and 256 rows of weights its columns: a thread's sums of a block then share one scale,
-// its token's times the block's, where weights on the lanes need one of each token (reading those from shared memory cost a
-// quarter of the time at 64 tokens).  Up to 128 tokens a CTA has a tile to itself and the time is that of the weights' bytes.
-// Beyond, a pair of CTAs shares a tile of 256 tokens by 256 weight rows: each CTA brings 128 tokens and 128 weight rows, its
-// accumulator holds its 128 tokens by all 256 weight rows, and one thread of the first CTA issues the products of both; the
-// pair reads 64 KB for a unit where two CTAs of their own would read 96 KB.
+// its token's times the block's, where weights on the lanes need one of each token.  Up to 128 tokens a CTA has a tile to itself
+// and the time is that of the weights' bytes.  Beyond, a pair of CTAs shares a tile of 256 tokens by 256 weight rows (but see
+// head_by_pairs): each CTA brings 128 tokens and 128 weight rows, its accumulator holds its 128 tokens by all 256 weight rows,
+// and one thread of the first CTA issues the products of both; the pair reads 64 KB for a unit where two CTAs of their own
+// read 96 KB.  What bounds a unit: 1170 cycles with everything; products and copies without the adding 1040, the copies alone
+// 930 (L2 to shared memory at 9.9 TB/s), the products alone 980.
 constexpr int kMoreAdders = 8, kMoreThreads = kMoreAdders * 32 + 64;      // warps that add, threads of a CTA
 // weights, then tokens; a CTA by itself brings only the `n` rows of tokens that there are (in steps of 16): what the other lanes
 // multiply is whatever lies behind, and nobody looks at their sums.  (The products read 128 rows all the same: behind the last
@@ -1027,13 +1029,46 @@ static int head_launch(KERN kern, int threads, int smem, int grid, int cluster, 
     return RS_OK;
 }
 template <typename OUT>
-static int head_run(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& out, const HeadParams& p, int smem, cudaStream_t stream) {
+static int head_run(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& out, const HeadParams& p, bool pair, int smem, cudaStream_t stream) {
     static bool done[4][64] = {};      // per device
     const int n = p.work.workers;
     if (p.M <= 32) return head_launch(head_few_kernel<32, OUT>, 192, smem, n, 1, stream, done[0], w, x, p);
     if (p.M <= kFewTokens) return head_launch(head_few_kernel<64, OUT>, 320, smem, n, 1, stream, done[1], w, x, p);
-    if (p.M <= 128) return head_launch(head_more_kernel<false, OUT>, kMoreThreads, smem, n, 1, stream, done[3], w, x, out, p);
+    if (!pair) return head_launch(head_more_kernel<false, OUT>, kMoreThreads, smem, n, 1, stream, done[3], w, x, out, p);
     return head_launch(head_more_kernel<true, OUT>, kMoreThreads, smem, 2 * n, 2, stream, done[2], w, x, out, p);
+}
+
+// More than 128 tokens: pairs, unless the last one's second half would have no tokens and that costs more than pairs gain, a
+// tenth.  us for pairs / single CTAs, K = 4096, V = 32768: 384 tokens 89 / 79, 640 127 / 122, 896 146 / 164, 1408 221 / 239.
+static bool head_by_pairs(long long M) {
+    const long long tiles = (M + 127) / 128;
+    return M > 128 && tiles != 3 && tiles != 5;
+}
+// How the units are given out: whole tiles in turn, every tile in equal runs of its own, or equal runs throughout, where most
+// workers share two tiles.  Each way's time is estimated in that of a unit when all workers are busy; with few of them a unit
+// takes `alone` of it.  Sharing a tile costs what its sums take through L2 (from 65 tokens on 128 KB a CTA, below that 16 or
+// 32): `first` for two workers, `next` for each more, `runs` for equal runs.  With 65 to 128 tokens whole tiles in turn leave
+// HBM idle whenever all workers store theirs.  us for whole tiles / the best number of runs each / equal runs:
+//   64 tokens, K = 4096, V = 151936: 141 / - / 135;   64, 2048, 50304: 31 / - / 38;      64, 4096, 19000: 35 / - / 31;
+//   33 tokens, K = 4992, V = 2000: 24 / 22 (2) / 28;  8, 6976, 11215: 25 / - / 28;       1, 4096, 151936: 104 / - / 103;
+//   128 tokens, K = 4096, V = 151936: 160 / - / 137;  80, 2048, 65536: 37 / - / 50;      128, 8192, 1000: 48 / 33 (3) / 53;
+//   467 tokens, K = 4192, V = 3565: 34 / 40 (2) / 56; 757, 960, 5863: 19 / - / 38;       251, 6112, 114533: 241 / - / 222.
+static void head_split(HeadWork& k, long long M) {
+    struct Costs { float alone, first, next, runs; };
+    const Costs c = M <= kFewTokens ? Costs{0.55f, 6.f, 1.f, 10.f} : head_by_pairs(M) ? Costs{0.8f, 19.f, 8.f, 25.f} : Costs{0.65f, 9.5f, 4.f, 27.f};
+    const int W = k.workers, rest = k.tiles % W;
+    auto busy = [&](long long workers) { return fmaxf((float)workers / (float)W, c.alone); };
+    float best = (float)k.blocks * ((float)(k.tiles / W) + (rest ? busy(rest) : 0.f));
+    if (M > kFewTokens && M <= 128 && k.tiles > W) best *= 1.25f;
+    int workers = k.tiles < W ? k.tiles : W, split = 0;
+    for (int parts = 2; (long long)parts * k.tiles <= W && parts * 4 <= k.blocks; parts++) {
+        const float cost = (float)((k.blocks + parts - 1) / parts) * busy(parts * k.tiles) + c.first + c.next * (float)(parts - 2);
+        if (cost < best) { best = cost; workers = parts * k.tiles; split = 1; }
+    }
+    const float cost = (float)k.units / (float)W + c.runs + (k.tiles < W ? c.next * (float)(W / k.tiles) : 0.f);
+    if (cost < best && k.units >= 4LL * W) { workers = W; split = 1; }
+    k.workers = workers;
+    k.split = split;
 }
 
 // Pairs of CTAs that the device runs at once.
@@ -1092,7 +1127,7 @@ static int head_quantize(const void* src, int dtype, long long stride, long long
 }
 
 static bool head_dtype(int d) { return d == RS_DTYPE_F32 || d == RS_DTYPE_F16 || d == RS_DTYPE_BF16; }
-static int head_pitch(long long M) { return (int)((M + 255) / 256 * 256) + 256; }      // a tile's scales never end behind a row
+static int head_pitch(long long M) { return (int)((M + 255) / 256 * 256) + 256; }      // a multiple of a tile: its scales never end behind a row
 struct HeadLayout { size_t scales, arrived, partial, total; };
 static HeadLayout head_layout(long long M, long long K) {
     HeadLayout l;
@@ -1164,9 +1199,9 @@ int rs_head_logits(const void* hidden, int32_t hidden_dtype, int64_t M, int64_t 
     p.arrived = (int*)(ws + l.arrived);
     p.polls = host_wait_polls();
     p.mirror = dev.mirror;
-    const bool few = M <= kFewTokens, pair = M > 128;
-    p.n = pair ? 128 : (int)((M + 15) / 16 * 16);
-    p.token_tiles = pair ? (int)((M + 255) / 256) : 1;
+    const bool few = M <= kFewTokens, pair = head_by_pairs(M);
+    p.n = M >= 128 ? 128 : (int)((M + 15) / 16 * 16);
+    p.token_tiles = (int)(pair ? (M + 255) / 256 : (M + 127) / 128);
     const int tile_v = few ? 128 : 256;
     HeadWork& k = p.work;
     k.blocks = (int)((K + 127) / 128);
@@ -1180,11 +1215,7 @@ int rs_head_logits(const void* hidden, int32_t hidden_dtype, int64_t M, int64_t 
         if ((rc = head_pairs(&pairs))) return rc;
         k.workers = k.workers / 2 < pairs ? k.workers / 2 : pairs;
     }
-    // Whole tiles where the last round of them wastes little, for what a split tile costs: 256 KB written and read a pair.
-    const long long rounds = (tiles + k.workers - 1) / k.workers;
-    k.split = few || rounds * k.workers * 100 > tiles * 103;
-    if (k.split && k.units < 4LL * k.workers) k.workers = (int)((k.units + 3) / 4);
-    if (!k.split && tiles < k.workers) k.workers = (int)tiles;
+    head_split(k, M);
     const int per = few ? head_few_stage(p.n) : head_more_stage(pair, p.n);
     const uintptr_t step = (uintptr_t)out_device | (uintptr_t)out_stride * os;
     p.wide_store = step % 32 == 0 ? 32 : step % 16 == 0 ? 16 : 0;
@@ -1208,9 +1239,9 @@ int rs_head_logits(const void* hidden, int32_t hidden_dtype, int64_t M, int64_t 
     p.turn_at = p.stages * per + (few ? 0 : head_more_tail(pair, p.n));
     const int smem = p.stages * per + tail + 1024;
     switch (out_dtype) {
-        case RS_DTYPE_F32: return head_run<float>(w, x, out, p, smem, (cudaStream_t)stream);
-        case RS_DTYPE_F16: return head_run<__half>(w, x, out, p, smem, (cudaStream_t)stream);
-        default: return head_run<__nv_bfloat16>(w, x, out, p, smem, (cudaStream_t)stream);
+        case RS_DTYPE_F32: return head_run<float>(w, x, out, p, pair, smem, (cudaStream_t)stream);
+        case RS_DTYPE_F16: return head_run<__half>(w, x, out, p, pair, smem, (cudaStream_t)stream);
+        default: return head_run<__nv_bfloat16>(w, x, out, p, pair, smem, (cudaStream_t)stream);
     }
 }
 

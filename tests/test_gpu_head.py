@@ -352,3 +352,18 @@ def test_a_graph_notices_that_its_logits_were_written_over():
     before = buf.clone()
     rs.lm_head_logits(h, codes, scales, out=buf)              # no counter to keep
     assert torch.equal(buf, before)
+
+
+@pytest.mark.parametrize("M,K,V", [
+    (33, 4992, 2000), (3, 7088, 3094), (64, 4096, 19000), (50, 640, 40000),      # up to 64 tokens: own runs of a tile, equal runs, whole tiles
+    (128, 8192, 1000), (100, 8192, 40000), (80, 512, 60000),                     # up to 128
+    (286, 6928, 1301), (384, 1024, 5003), (600, 512, 40000),                     # more, one CTA a tile
+    (512, 16384, 500), (256, 8192, 19000), (700, 640, 9001)])                    # pairs
+def test_every_way_of_giving_out_the_work(M, K, V):
+    import rapid_sampling_b200 as rs
+    codes, scales = rs.lm_head_quantize(make(V, K, "bf16", M, 0.02))
+    h = make(M, K, "bf16", K)
+    out = rs.lm_head_logits(h, codes, scales)
+    check(h, codes, scales, out)
+    assert torch.equal(out, rs.lm_head_logits(h, codes, scales))
+    assert rs.device_status() == 0
