@@ -329,6 +329,10 @@ struct HeadWait {
         if (p.mirror) *reinterpret_cast<volatile int*>(p.mirror) = RS_ERR_TIMEOUT;
         return false;
     }
+    // For a converged warp.  What is ready costs 73 cycles so, and 104 by way of the loop (155 with one lane waiting for all).
+    __device__ __forceinline__ bool warp(uint32_t bar, uint32_t parity) const {
+        return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || __all_sync(0xffffffffu, (*this)(bar, parity));
+    }
 };
 // A thread's sums of one row and `cols` tokens in a slot of the workspace: four tokens of 128 rows together, so that both the
 // threads' 16 bytes and a warp's 512 are contiguous.
@@ -454,7 +458,7 @@ __global__ void __launch_bounds__(NT * 4 + 64, 1)
         bool ok = true;
         while (ok && walk.next())
             for (int b = walk.b0; b < walk.b1; b += 2, it++) {
-                if (it >= stages && !__all_sync(0xffffffffu, wait(empty + 8 * s, ph ^ 1u))) { ok = false; break; }
+                if (it >= stages && !wait.warp(empty + 8 * s, ph ^ 1u)) { ok = false; break; }
                 if (elect_one()) {
                     const uint32_t at = base + s * stage_bytes, bar = full + 8 * s, n = (uint32_t)min(2, walk.b1 - b);
                     mbar_expect_tx(bar, n * (128u * 128u + (uint32_t)p.n * 132u));
@@ -472,7 +476,7 @@ __global__ void __launch_bounds__(NT * 4 + 64, 1)
         const uint32_t n = min(it, stages);
         for (uint32_t i = 0; i < n; i++) {
             const uint32_t k = it - 1 - i, st = k % stages, parity = (k / stages) & 1u;
-            if (!ok || !wait(empty + 8 * st, parity)) {
+            if (!ok || !wait.warp(empty + 8 * st, parity)) {
                 ok = false;
                 mbar_wait_bounded(full + 8 * st, parity, kHeadDrainPolls);
             }
@@ -485,8 +489,8 @@ __global__ void __launch_bounds__(NT * 4 + 64, 1)
         while (ok && walk.next())
             for (int b = walk.b0; b < walk.b1; b += 2, it++) {
                 const uint32_t buf = it % BUFS;
-                if (it >= BUFS && !__all_sync(0xffffffffu, wait(sempty + 8 * buf, ((it / BUFS) & 1u) ^ 1u))) { ok = false; break; }
-                if (!__all_sync(0xffffffffu, wait(full + 8 * s, ph))) { ok = false; break; }
+                if (!wait.warp(full + 8 * s, ph)) { ok = false; break; }
+                if (it >= BUFS && !wait.warp(sempty + 8 * buf, ((it / BUFS) & 1u) ^ 1u)) { ok = false; break; }
                 tmem_fence_after();
                 if (elect_one()) {
                     const uint64_t da = desc + ((s * stage_bytes) >> 4), db = da + (32768u >> 4);
@@ -525,7 +529,7 @@ __global__ void __launch_bounds__(NT * 4 + 64, 1)
                     scale[1] = b + 32 + lane < walk.b1 ? __ldg(sw + b + 32 + lane) : 0.f;
                 }
                 const float f0 = __shfl_sync(0xffffffffu, scale[0], q), f1 = __shfl_sync(0xffffffffu, scale[0], q + 1);
-                if (!dead) dead = !__all_sync(0xffffffffu, wait(sfull + 8 * buf, (it / BUFS) & 1u));
+                if (!dead) dead = !wait.warp(sfull + 8 * buf, (it / BUFS) & 1u);
                 if (dead) break;
                 tmem_fence_after();
                 const ulonglong2* sa = reinterpret_cast<const ulonglong2*>(base_p + s * stage_bytes + 32768u + 2 * x_bytes);
@@ -802,7 +806,7 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
             const int vt = walk.tile / p.token_tiles, mt = walk.tile - vt * p.token_tiles;
             const int v0 = vt * 256 + rank * 128, m0 = mt * 128 * CTAS + rank * 128;
             for (int b = walk.b0; b < walk.b1; b++, it++) {
-                if (it >= stages && !__all_sync(0xffffffffu, wait(empty + 8 * s, ph ^ 1u))) { ok = false; break; }
+                if (it >= stages && !wait.warp(empty + 8 * s, ph ^ 1u)) { ok = false; break; }
                 if (elect_one()) {
                     const uint32_t at = base + s * stage_bytes, bar = first_full + 8 * s;
                     if constexpr (PAIR) {
@@ -822,7 +826,7 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
         const uint32_t n = min(it, stages);           // as in head_few_kernel; a pair's copies count on the first CTA's barriers
         for (uint32_t i = 0; i < n; i++) {
             const uint32_t k = it - 1 - i, st = k % stages, parity = (k / stages) & 1u;
-            if (!ok || !wait(empty + 8 * st, parity)) {
+            if (!ok || !wait.warp(empty + 8 * st, parity)) {
                 ok = false;
                 if (rank == 0) mbar_wait_bounded(full + 8 * st, parity, kHeadDrainPolls);
             }
@@ -836,8 +840,8 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
             while (ok && walk.next())
                 for (int b = walk.b0; b < walk.b1; b++, it++) {
                     const uint32_t buf = it & 1u;
-                    if (it >= 2 && !__all_sync(0xffffffffu, wait(sempty + 8 * buf, ((it >> 1) & 1u) ^ 1u))) { ok = false; break; }
-                    if (!__all_sync(0xffffffffu, wait(full + 8 * s, ph))) { ok = false; break; }
+                    if (!wait.warp(full + 8 * s, ph)) { ok = false; break; }
+                    if (it >= 2 && !wait.warp(sempty + 8 * buf, ((it >> 1) & 1u) ^ 1u)) { ok = false; break; }
                     tmem_fence_after();
                     if (elect_one()) {
                         const uint64_t db = desc + ((s * stage_bytes) >> 4), da = db + (kWeights >> 4);
@@ -890,7 +894,7 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
                     w2 = __ldg(sw + b + 2);
                 }
                 const uint64_t ff = f2_pack(f, f);
-                if (!dead) dead = !__all_sync(0xffffffffu, wait(sfull + 8 * buf, (it >> 1) & 1u));
+                if (!dead) dead = !wait.warp(sfull + 8 * buf, (it >> 1) & 1u);
                 if (dead) break;
                 tmem_fence_after();
 #pragma unroll
