@@ -490,7 +490,7 @@ __device__ int top_collect(const Span<DT>& sp, TS& sh, float mx, int n) {
     // reach it) and a quarter of the time that the n-th largest of all threads' takes
     const int busy = min(NT, sp.v1 - sp.v0);      // threads that have vectors
     int lg = 0;
-    while (lg < 5 && (busy >> (lg + 1)) * 5 >= n * 8) lg++;
+    while (lg < 5 && NT >> (lg + 1) >= 4 && (busy >> (lg + 1)) * 5 >= n * 8) lg++;      // (four keys are read at a time)
     const int groups = NT >> lg;
     uint32_t of_group = mine;
     for (int step = 1; step < (1 << lg); step *= 2) of_group = max(of_group, __shfl_xor_sync(0xffffffffu, of_group, step));
