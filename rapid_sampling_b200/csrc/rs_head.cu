@@ -7,9 +7,9 @@
 // and is added in fp32 registers.  Products of e4m3 values are exact, a block's 128 of them are summed in the tensor core's fp32
 // (measured against 64 bits: 1e-7 relative for K = 4096, where a plain fp32 product is 1e-6 off).
 //
-// What bounds it (B200, K = 4096, us): few tokens, the weights' bytes: V = 151936, 1 token 102 of 95 at the measured copy rate,
-// 64 tokens 128 (140 under the power cap) of 101.  Many tokens, the copies from L2 and the power cap: V = 65536, 2048 tokens 547
-// for a short while, 640 under the cap (1.72 PFLOP/s).
+// What bounds it (B200, K = 4096, us): few tokens, the weights' bytes: V = 151936, 1 token 103 of 95 at the measured copy rate,
+// 64 tokens 127 (135 under the power cap) of 98.  Many tokens, the adding of the blocks' sums: V = 65536, 2048 tokens 523 for a
+// short while (2.10 PFLOP/s), 575 under the cap.
 #include "rs_common.cuh"
 #include "rs_host.cuh"
 #include "../../include/rapid_sampling_b200.h"
@@ -596,8 +596,9 @@ __global__ void __launch_bounds__(NT * 4 + 64, 1)
 // and the time is that of the weights' bytes.  Beyond, a pair of CTAs shares a tile of 256 tokens by 256 weight rows (but see
 // head_by_pairs): each CTA brings 128 tokens and 128 weight rows, its accumulator holds its 128 tokens by all 256 weight rows,
 // and one thread of the first CTA issues the products of both; the pair reads 64 KB for a unit where two CTAs of their own
-// read 96 KB.  What bounds a unit: 1170 cycles with everything; products and copies without the adding 1040, the copies alone
-// 930 (L2 to shared memory at 9.9 TB/s), the products alone 980.
+// read 96 KB.  What bounds a unit of 256 x 256 x 128 is the adding: 1050 cycles with everything; 740 without the adding, of which
+// 70 are scales and stores; 512 the products alone at the tensor core's rate.  Neither half the adding's loads nor half its
+// additions would be enough by themselves (each alone 800): the registers that the sums leave are too few to keep both going.
 constexpr int kMoreAdders = 8, kMoreThreads = kMoreAdders * 32 + 64;      // warps that add, threads of a CTA
 // weights, then tokens; a CTA by itself brings only the `n` rows of tokens that there are (in steps of 16): what the other lanes
 // multiply is whatever lies behind, and nobody looks at their sums.  (The products read 128 rows all the same: behind the last
