@@ -367,3 +367,11 @@ def test_every_way_of_giving_out_the_work(M, K, V):
     check(h, codes, scales, out)
     assert torch.equal(out, rs.lm_head_logits(h, codes, scales))
     assert rs.device_status() == 0
+
+
+@pytest.mark.parametrize("M", [1, 40, 100, 200, 300])
+def test_the_largest_K(M):
+    import rapid_sampling_b200 as rs
+    codes, scales = rs.lm_head_quantize(make(270, 65536, "bf16", 1, 0.01))
+    h = make(M, 65536, "bf16", 2)
+    check(h, codes, scales, rs.lm_head_logits(h, codes, scales))

@@ -565,3 +565,9 @@ def test_the_most_probable_token_of_short_rows(V, dtype):
             best = min(best, a.elapsed_time(b))
         return best
     assert us(1) < 2 * us(2)
+
+
+@pytest.mark.parametrize("rows,dtype", [((2,), "f32"), ((2,), "f16"), ((300,), "bf16"), ((300,), "f32")])
+def test_the_longest_rows_and_lists(rows, dtype):
+    x, t = make(rows, 1048576, dtype, 80)
+    check_all(x, t, 0.9, top_n=64, grads=False)
