@@ -596,9 +596,9 @@ __global__ void __launch_bounds__(NT * 4 + 64, 1)
 // and the time is that of the weights' bytes.  Beyond, a pair of CTAs shares a tile of 256 tokens by 256 weight rows (but see
 // head_by_pairs): each CTA brings 128 tokens and 128 weight rows, its accumulator holds its 128 tokens by all 256 weight rows,
 // and one thread of the first CTA issues the products of both; the pair reads 64 KB for a unit where two CTAs of their own
-// read 96 KB.  What bounds a unit of 256 x 256 x 128 is the adding: 1050 cycles with everything; 740 without the adding, of which
-// 70 are scales and stores; 512 the products alone at the tensor core's rate.  Neither half the adding's loads nor half its
-// additions would be enough by themselves (each alone 800): the registers that the sums leave are too few to keep both going.
+// read 96 KB.  What bounds it is the adding: 2048 tokens, K = 4096, V = 65536 take 523 us, and in copies of the kernel 402 without
+// the adding, 371 without scales and stores too; with the reading of the accumulators but not the additions 443, the other way
+// round 449: the sums leave too few registers to keep both going at once.
 constexpr int kMoreAdders = 8, kMoreThreads = kMoreAdders * 32 + 64;      // warps that add, threads of a CTA
 // weights, then tokens; a CTA by itself brings only the `n` rows of tokens that there are (in steps of 16): what the other lanes
 // multiply is whatever lies behind, and nobody looks at their sums.  (The products read 128 rows all the same: behind the last
