@@ -6,8 +6,10 @@
 //     d/dx_j (g log p_t + h H) = 1/T (g [j = t] - p_j (g + h (ln p_j + H)))
 // A row is read once: every thread keeps the maximum it has seen, and the two sums relative to it.  Maxima are compared on
 // the logits as they are; exponents are taken as ((x - m) log2(e)/T) so that neither masks of the type's lowest value nor a
-// row made of nothing else overflow.  Sums are held without the maximum's own 1 ("excess", s - 1) from the thread level up:
-// log p of a token of probability nearly one is -log1p(excess), which keeps its digits.
+// row made of nothing else overflow.  log p of a token of probability nearly one is -log1p(excess), the excess being s without
+// the maximum's own 1.  Sums are held so from the thread level up, all but the one of the thread that has the maximum apart from
+// that thread's, whose additions to the 1 lose what lies below 2^-24; where the excess is small its elements are read again
+// (lp_rest).
 #include "rs_device.cuh"
 #include "rs_host.cuh"
 #include "../../include/rapid_sampling_b200.h"
@@ -26,6 +28,9 @@ constexpr int kTopMax = 64;            // longest list of alternatives
 constexpr int kTopHot = 256;           // most pieces of a part that are looked at again (a list of 64 has about 100)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFloor = -160.f;       // exponent from which on exp2f is zero; keeps 0 * inf out of the second sum
+// Excess below which the maximum's thread is read again.  Its own sum is off by 2^-24 for each of its additions at most (17, and one
+// a step, of which a row of 151936 has up to 37), so the excess keeps its digits to 2^-12 from here on, and to 2^-16 as a rule.
+constexpr float kSmallExcess = 0.015625f;
 
 __device__ int g_lp_status;            // status word of these calls on this device (rs_logprobs_status)
 
@@ -303,12 +308,19 @@ __device__ __forceinline__ float stat_add(Stat& a, const uint4 (&v)[U], float c)
     a.u += u0 + u1;
     return most;
 }
-// The lanes' statistics as one, in every lane.  s comes and goes as the excess: the sum without the maximum's own 1 (-1: no
-// element above -inf).  Terms are added in a fixed order.
-__device__ __forceinline__ Stat stat_warp(Stat a, float c) {
-    Stat r;
+// Statistics of many threads.  The sum is w = 1 + own + s: own is the excess of the thread `who`, which has the maximum (-1: no
+// element above -inf), s what all others add.
+struct Group {
+    float mx, s, u, own;
+    int who;
+    __device__ __forceinline__ float excess() const { return s + own; }
+};
+__device__ __forceinline__ Group group_none() { return {-INFINITY, 0.f, 0.f, -1.f, 0}; }
+// The lanes' statistics as one, in every lane.  Terms are added in a fixed order.
+__device__ __forceinline__ Group group_warp(const Group& a, float c) {
+    Group r;
     r.mx = warp_max_nan(a.mx);
-    const float d = fmaxf((ref_of(a.mx) - ref_of(r.mx)) * c, kFloor), f = ex2(d), w = 1.f + a.s;
+    const float d = fmaxf((ref_of(a.mx) - ref_of(r.mx)) * c, kFloor), f = ex2(d), w = (1.f + a.own) + a.s;
     const int owner = __ffs(__ballot_sync(0xffffffffu, a.mx == r.mx)) - 1;
     r.s = (int)(threadIdx.x & 31) == owner ? a.s : f * w;
     r.u = f * fmaf(d, w, a.u);
@@ -317,6 +329,8 @@ __device__ __forceinline__ Stat stat_warp(Stat a, float c) {
         r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
         r.u += __shfl_xor_sync(0xffffffffu, r.u, o);
     }
+    r.own = __shfl_sync(0xffffffffu, a.own, owner);      // (a NaN has no owner, and its sums are not used)
+    r.who = __shfl_sync(0xffffffffu, a.who, owner);
     return r;
 }
 
@@ -331,10 +345,9 @@ struct Span {
     int head, nvec, V;       // of the row
     int v0, v1;              // this CTA's vectors
     bool first, last;
-    __device__ __forceinline__ Span(const LpParams& p, const LpRow& w) {
+    __device__ __forceinline__ Span(const LpParams& p, const LpRow& w) : Span((const T*)p.logits + w.b * p.sb + w.t * p.st, p.V) {}
+    __device__ __forceinline__ Span(const T* at, int n) : row(at), V(n) {
         constexpr int E = Elem<DT>::E;
-        row = (const T*)p.logits + w.b * p.sb + w.t * p.st;
-        V = p.V;
         head = (int)((16u - ((uint32_t)(uintptr_t)row & 15u)) & 15u) / (int)sizeof(T);
         if (head > V) head = V;
         nvec = (V - head) / E;
@@ -362,13 +375,57 @@ struct Span {
     }
 };
 
+// The excess of thread `th`, which has the row's maximum `mx`, by one warp: its vectors and single elements are read again and
+// what lies below the maximum is added by itself; every further element equal to the maximum counts 1.  It costs such a row the
+// latency of its loads, 1.3 us, which the other rows on the multiprocessor hide in part.  us without and with, every row of such
+// logits: statistics of 4088 rows of 151936 bf16 195 / 201, 16384 of 4096 43 / 53; with a list of 20 249 / 258 and 105 / 112.
+template <int DT, int NT>
+__device__ __forceinline__ float lp_rest(const typename Elem<DT>::T* row, int V, int v0, int v1, bool first, bool last, int th, float mx, float c) {
+    constexpr int E = Elem<DT>::E;
+    Span<DT> sp(row, V);
+    sp.v0 = v0; sp.v1 = v1; sp.first = first; sp.last = last;
+    const int lane = threadIdx.x & 31;
+    float rest = 0.f;
+    int equal = 0;
+    auto add = [&](float x) {
+        const float e = ex2(fmaxf((x - mx) * c, kFloor));
+        equal += x == mx;
+        rest += x == mx ? 0.f : e;
+    };
+    if (lane == 0) sp.singles(th, [&](int, float x) { add(x); });
+    for (int v = v0 + th + lane * NT; v < v1; v += 4 * 32 * NT) {
+        uint4 raw[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (v + i * 32 * NT < v1) raw[i] = ld_stream(sp.vec + v + i * 32 * NT);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (v + i * 32 * NT < v1) {
+                float x[E];
+                widen<DT>(raw[i], x);
+#pragma unroll
+                for (int k = 0; k < E; k++) add(x[k]);
+            }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
+    return rest + (float)((int)warp_sum_u32((uint32_t)equal) - 1);
+}
+
+// A call of its own leaves the statistics' loop the registers it had (inlined: 196 -> 203 us for the 4088 rows, nothing small about
+// their excess); with a list inlining is as good or better (252 -> 250).
+template <int DT, int NT>
+__device__ __noinline__ float lp_rest_called(const typename Elem<DT>::T* row, int V, int v0, int v1, bool first, bool last, int th, float mx, float c) {
+    return lp_rest<DT, NT>(row, V, v0, v1, first, last, th, mx, c);
+}
+
 // ---- statistics, rank and alternatives of rows ---------------------------------------------------------------------
 struct LpShared {
-    float mx[16], s[16], u[16];       // warps of the CTA (8), then CTAs of the cluster (16)
-    int cnt[16];
-    float r_mx, r_logs, r_inv_t;
-    float c_mx[16], c_s[16], c_u[16];
-    int c_cnt[16];
+    float mx[8], s[8], u[8], own[8];                     // the CTA's warps
+    int who[8], cnt[8];
+    float c_mx[16], c_s[16], c_u[16], c_own[16];         // the cluster's CTAs
+    int c_who[16], c_cnt[16];
+    float r_mx, r_logs;
 };
 // SHARED: the row is a cluster's.  Small, because what it takes is lost to the loads in flight, which pass through L1.
 template <int NT, bool SHARED>
@@ -660,29 +717,30 @@ __global__ void __launch_bounds__(NT, 1024 / NT) lp_rows_kernel(const __grid_con
         v += kStep;
     }
     const float my_mx = a.mx;
-    a.s -= 1.f;
-    a = stat_warp(a, c);
+    const Group of_warp = group_warp({a.mx, 0.f, a.u, a.s - 1.f, t}, c);
     if (TOP) cnt = (int)warp_sum_u32((uint32_t)cnt);
     if (lane == 0) {
-        sh.mx[w] = a.mx; sh.s[w] = a.s; sh.u[w] = a.u;
+        sh.mx[w] = of_warp.mx; sh.s[w] = of_warp.s; sh.u[w] = of_warp.u; sh.own[w] = of_warp.own; sh.who[w] = of_warp.who;
         if (TOP) sh.cnt[w] = cnt;
     }
     __syncthreads();
     if (parts > 1) cluster_wait();                // every CTA of the cluster runs: its shared memory may be written
     if (w == 0) {
-        Stat b = {-INFINITY, -1.f, 0.f};
-        if (lane < NT / 32) b = {sh.mx[lane], sh.s[lane], sh.u[lane]};
-        b = stat_warp(b, c);
+        Group b = group_none();
+        if (lane < NT / 32) b = {sh.mx[lane], sh.s[lane], sh.u[lane], sh.own[lane], sh.who[lane]};
+        b = group_warp(b, c);
         int n = TOP ? (int)warp_sum_u32(lane < NT / 32 ? (uint32_t)sh.cnt[lane] : 0u) : 0;
         if (parts > 1) {
             if (lane == 0) {
                 st_cluster_f32(map_to_cta(smem_addr(&sh.c_mx[part]), 0), b.mx);
                 st_cluster_f32(map_to_cta(smem_addr(&sh.c_s[part]), 0), b.s);
                 st_cluster_f32(map_to_cta(smem_addr(&sh.c_u[part]), 0), b.u);
+                st_cluster_f32(map_to_cta(smem_addr(&sh.c_own[part]), 0), b.own);
+                st_cluster_u32(map_to_cta(smem_addr(&sh.c_who[part]), 0), (uint32_t)b.who);
                 if (TOP) st_cluster_u32(map_to_cta(smem_addr(&sh.c_cnt[part]), 0), (uint32_t)n);
             }
         } else if (lane == 0) {
-            sh.c_mx[0] = b.mx; sh.c_s[0] = b.s; sh.c_u[0] = b.u;
+            sh.c_mx[0] = b.mx; sh.c_s[0] = b.s; sh.c_u[0] = b.u; sh.c_own[0] = b.own; sh.c_who[0] = b.who;
             if (TOP) sh.c_cnt[0] = n;
         }
     }
@@ -707,16 +765,26 @@ __global__ void __launch_bounds__(NT, 1024 / NT) lp_rows_kernel(const __grid_con
     }
     // the first CTA has everything
     if (w == 0) {
-        Stat b = {-INFINITY, -1.f, 0.f};
-        if (lane < parts) b = {sh.c_mx[lane], sh.c_s[lane], sh.c_u[lane]};
-        b = stat_warp(b, c);
-        int above = TOP ? (int)warp_sum_u32(lane < parts ? (uint32_t)sh.c_cnt[lane] : 0u) : 0;
+        const int from = SHARED ? lane : 0;
+        Group b = group_none();
+        if (from < parts) b = {sh.c_mx[from], sh.c_s[from], sh.c_u[from], sh.c_own[from], from * NT + sh.c_who[from]};
+        int above = TOP && from < parts ? sh.c_cnt[from] : 0;
+        if (SHARED) {
+            b = group_warp(b, c);
+            if (TOP) above = (int)warp_sum_u32((uint32_t)above);
+        }
+        const bool bad = !(b.mx < INFINITY), none = b.mx == -INFINITY;
+        if (!bad && !none && b.excess() < kSmallExcess) {
+            const int of = b.who / NT;
+            sp.share(of, log_parts);
+            if constexpr (TOP) b.own = lp_rest<DT, NT>(sp.row, sp.V, sp.v0, sp.v1, sp.first, sp.last, b.who % NT, b.mx, c);
+            else b.own = lp_rest_called<DT, NT>(sp.row, sp.V, sp.v0, sp.v1, sp.first, sp.last, b.who % NT, b.mx, c);
+        }
         if (lane == 0) {
-            const bool bad = !(b.mx < INFINITY), none = b.mx == -INFINITY;
             const float nan = __int_as_float(0x7FC00000);
-            const float logs = log1pf(b.s);
+            const float excess = b.excess(), logs = log1pf(excess);
             const float lp = bad ? nan : none ? -INFINITY : lp_scaled(xt, b.mx, row.inv_t) - logs;
-            const float ent = bad ? nan : none ? 0.f : logs - b.u / (1.f + b.s) * 0.6931471805599453f;
+            const float ent = bad ? nan : none ? 0.f : logs - b.u / (1.f + excess) * 0.6931471805599453f;
             if (p.logprob) p.logprob[r] = lp;
             if (p.entropy) p.entropy[r] = ent;
             if (p.stats) p.stats[r] = make_float2(b.mx, logs * kLog2e);

@@ -571,3 +571,53 @@ def test_the_most_probable_token_of_short_rows(V, dtype):
 def test_the_longest_rows_and_lists(rows, dtype):
     x, t = make(rows, 1048576, dtype, 80)
     check_all(x, t, 0.9, top_n=64, grads=False)
+
+
+# distances in elements between a row's maximum and its runner-up: a neighbour in the same 16 bytes, and other vectors of the same
+# thread, in the same step and in later ones, whatever the number of threads
+def _runners_up(V, size):
+    E = 16 // size
+    return sorted({d for d in [1, 2] + [E * nt * k for nt in (64, 128, 256) for k in (1, 3, 4, 9)] if 8 + d < V})
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V,rows", [(4, 0), (9, 0), (1500, 0), (1500, 400), (5000, 400), (70000, 0), (70000, 400)])
+def test_confident_rows_keep_the_runner_up(V, rows, dtype):
+    """Rows of one token of probability nearly one and one other, which the same thread may hold: log p = -log1p(r) with
+    r = exp(-gap / T), H = log1p(r) + gap/T r / (1 + r), and gradients of +-r / (1 + r).  The exponent's argument has three roundings of
+    2^-24, so r is off by 2^-23 * 2 gap/T at most, and by 2^-22 for the exponential; sums, log1p, expm1 and quotients take
+    another 2^-21 at most.  (Gaps of 16-bit types too: all values are whole.)"""
+    import rapid_sampling_b200 as rs
+    size = 4 if dtype == "f32" else 2
+    cases = [(gap, d, at, way) for gap in (3.0, 8.0, 17.0, 40.0) for d in (_runners_up(V, size) or [1]) for at in (0, min(8, V - 1 - d)) for way in (0, 1)]
+    cases = cases * (1 + rows // len(cases))
+    n = len(cases)
+    x = torch.full((n, V), -math.inf, device="cuda")
+    gap = torch.tensor([c[0] for c in cases], device="cuda")
+    r = torch.arange(n, device="cuda")
+    one, other = (torch.tensor([at + (0 if way == first else d) for _, d, at, way in cases], device="cuda") for first in (0, 1))
+    x[r, one] = 3.0
+    x[r, other] = 3.0 - gap
+    x = x.to(DT[dtype])
+    for T in (1.0, 0.5):
+        z = gap.double() / T
+        rest = torch.exp(-z)
+        tol = 2.0 ** -23 * 2 * z + 2.0 ** -20
+        want, H = -torch.log1p(rest), torch.log1p(rest) + z * rest / (1 + rest)
+        lp, ent = rs.batch_token_logprobs(x, one, T)
+        assert bool(((lp.double() - want).abs() <= tol * want.abs()).all()), (lp, want)
+        assert bool(((ent.double() - H).abs() <= tol * H).all()), (ent, H)
+        lp2, rank, ent2, top, ids = rs.batch_top_logprobs(x, 2, one, T)
+        assert torch.equal(lp2, top[:, 0]) and bool((rank == 1).all()) and torch.equal(ids.long(), torch.stack([one, other], 1))
+        assert bool(((lp2.double() - want).abs() <= tol * want.abs()).all()) and bool(((ent2.double() - H).abs() <= tol * H).all())
+        second = want - z
+        assert bool(((top[:, 1].double() - second).abs() <= tol * second.abs()).all())
+        leaf = x.clone().requires_grad_(True)
+        grad, = torch.autograd.grad(rs.batch_token_logprobs(leaf, one, T)[0].sum(), leaf)
+        want = rest / (1 + rest) / T
+        half = torch.finfo(DT[dtype]).eps / 2 * want + torch.finfo(DT[dtype]).smallest_normal * torch.finfo(DT[dtype]).eps
+        assert bool(((grad[r, one].double() - want).abs() <= tol * want + half).all())
+        assert bool(((grad[r, other].double() + want).abs() <= tol * want + half).all())
+        grad[r, one] = grad[r, other] = 0
+        assert not grad.any()
+    assert rs.device_status() == 0
