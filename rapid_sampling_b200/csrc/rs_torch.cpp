@@ -3,6 +3,7 @@
 // Argument names follow the reference's README so keyword calls work as well as positional ones.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 
@@ -40,24 +41,26 @@ at::Tensor workspace_for(int device, cudaStream_t stream, size_t bytes) {
 // Host mirror of the device status word, one pinned int per device: the kernels store a non-zero status there as
 // well, so a failure (a bounded wait that gave up, a per-row temperature out of range) is noticed by the NEXT call
 // on that device from host memory alone -- no copy, no synchronisation on the hot path.
-struct Mirror {
-    at::Tensor word;   // pinned int32[1]
-};
+// The word is made by the first call, also where that call is being captured: a graph keeps the word's address that its
+// capture saw, so a word made later would never hear of its replays.  Kept for the life of the process, for the same reason.
 std::mutex g_mirror_mu;
-std::map<int, Mirror> g_mirror;
-volatile int* mirror_for(int device) {
+std::map<int, int*> g_mirror;
+volatile int* mirror_for(int device) {      // of the current device
     std::lock_guard<std::mutex> lk(g_mirror_mu);
-    Mirror& m = g_mirror[device];
-    if (!m.word.defined()) {
-        m.word = at::zeros({1}, at::TensorOptions().dtype(at::kInt)).pin_memory();
-        if (rs_set_status_mirror(m.word.data_ptr<int>()) != RS_OK) throw std::runtime_error("rs_set_status_mirror failed !\n");
+    int*& word = g_mirror[device];
+    if (!word) {
+        void* at = nullptr;
+        c10::cuda::CUDAStreamCaptureModeGuard relaxed{cudaStreamCaptureModeRelaxed};      // an allocation is no part of the graph
+        if (cudaHostAlloc(&at, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess)
+            throw std::runtime_error("no pinned memory for the status word !\n");
+        *(int*)at = 0;
+        if (rs_set_status_mirror((int*)at) != RS_OK) {
+            cudaFreeHost(at);
+            throw std::runtime_error("rs_set_status_mirror failed !\n");
+        }
+        word = (int*)at;
     }
-    return m.word.data_ptr<int>();
-}
-bool mirror_known(int device) {
-    std::lock_guard<std::mutex> lk(g_mirror_mu);
-    const auto it = g_mirror.find(device);
-    return it != g_mirror.end() && it->second.word.defined();
+    return word;
 }
 [[noreturn]] void throw_status(const char* what, int device, int v) {
     std::string msg = std::string(what) + " on cuda:" + std::to_string(device) + " reported: " + rs_status_string(v) + " !\n";
@@ -217,14 +220,12 @@ at::Tensor sample_repetition_any(at::Tensor& logits, at::Tensor& penalties, at::
 
 // ---- log probabilities ---------------------------------------------------------------------------------------------
 
-// The same for the calls that have no workspace.  A call that is being captured neither raises nor creates the mirror:
-// both would touch the device outside the graph.
+// The same for the calls that have no workspace.  A call that is being captured does not raise: clearing the device's word would
+// become a part of the graph.
 static void raise_pending_logprobs(int device, cudaStream_t stream) {
-    auto capturing = [] { return at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None; };
-    if (!mirror_known(device) && capturing()) return;
     volatile int* w = mirror_for(device);
     const int v = *w;
-    if (v == 0 || capturing()) return;
+    if (v == 0 || at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) return;
     *w = 0;
     rs_logprobs_status(stream);      // clears the device's word
     throw_status("an earlier call", device, v);

@@ -621,3 +621,38 @@ def test_confident_rows_keep_the_runner_up(V, rows, dtype):
         grad[r, one] = grad[r, other] = 0
         assert not grad.any()
     assert rs.device_status() == 0
+
+
+def test_a_graph_that_holds_the_first_calls_reports_what_its_replays_meet():
+    """A process whose first calls are captured ones: a replay with a bad token or temperature raises from the next call."""
+    import subprocess
+    import sys
+    code = """
+import torch, rapid_sampling_b200 as rs
+x = torch.randn(6, 5000, device="cuda"); t = torch.randint(0, 5000, (6,), device="cuda"); heat = torch.ones(6, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    lp, _ = rs.batch_token_logprobs(x, t, heat)
+def refused(word):
+    g.replay(); torch.cuda.synchronize()
+    try:
+        rs.batch_top_logprobs(x, 3)
+    except ValueError as e:
+        assert word in str(e), e
+    else:
+        raise SystemExit("not raised")
+    assert rs.device_status() == 0
+g.replay(); torch.cuda.synchronize()
+assert torch.equal(lp, rs.batch_token_logprobs(x, t, heat)[0])
+t[2] = 5000
+refused("token")
+t[2] = 7; heat[3] = 0
+refused("Temperature")
+heat[3] = 1
+g.replay(); torch.cuda.synchronize()
+assert torch.equal(lp, rs.batch_token_logprobs(x, t, heat)[0])
+print("fine")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout[-500:] + r.stderr[-2000:]
