@@ -37,6 +37,11 @@ at::Tensor workspace_for(int device, cudaStream_t stream, size_t bytes) {
         w = at::zeros({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device));
     return w;
 }
+at::Tensor workspace_if_any(int device, cudaStream_t stream) {
+    std::lock_guard<std::mutex> lk(g_ws_mu);
+    const auto it = g_ws_cache.find({device, stream});
+    return it == g_ws_cache.end() ? at::Tensor() : it->second;
+}
 
 // Host mirror of the device status word, one pinned int per device: the kernels store a non-zero status there as
 // well, so a failure (a bounded wait that gave up, a per-row temperature out of range) is noticed by the NEXT call
@@ -228,6 +233,8 @@ static void raise_pending_logprobs(int device, cudaStream_t stream) {
     if (v == 0 || at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) return;
     *w = 0;
     rs_logprobs_status(stream);      // clears the device's word
+    const at::Tensor ws = workspace_if_any(device, stream);      // it may have been a sampling call's, whose workspace has it too
+    if (ws.defined()) rs_clear_status(ws.data_ptr(), stream);
     throw_status("an earlier call", device, v);
 }
 

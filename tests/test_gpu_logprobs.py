@@ -656,3 +656,19 @@ print("fine")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
     assert r.returncode == 0 and "fine" in r.stdout, r.stdout[-500:] + r.stderr[-2000:]
+
+
+def test_an_error_of_a_sampling_call_is_reported_once():
+    """Whichever call raises it."""
+    import rapid_sampling_b200 as rs
+    x, t = make((4,), 4096, "f32", 90)
+    heat = torch.tensor([1.0, 0.0, 1.0, 1.0], device="cuda")
+    codes, scales = rs.lm_head_quantize(torch.randn(256, 64, device="cuda"))
+    for call in (lambda: rs.batch_token_logprobs(x, t), lambda: rs.batch_top_logprobs(x, 3),
+                 lambda: rs.lm_head_logits(torch.zeros(2, 64, device="cuda"), codes, scales)):
+        rs.batch_sampling_rows(x, rs.setup_rand(1, 4), heat)
+        torch.cuda.synchronize()
+        with pytest.raises(ValueError, match="Temperature"):
+            call()
+        assert rs.device_status() == 0
+        call()
