@@ -436,6 +436,7 @@ static int dtype_of(const at::Tensor& t, const char* name) {
 // Elements between the rows of (..., n); every row must follow the one before at the same distance.
 static int64_t row_stride(const at::Tensor& t, const char* name) {
     const int64_t d = t.dim();
+    if (t.numel() == 0) return t.size(-1);      // strides of an empty tensor mean nothing
     if (t.size(-1) > 1 && t.stride(-1) != 1) throw std::invalid_argument(std::string(name) + " must be contiguous along the last dimension !\n");
     int64_t step = 0, rows = 1;      // of the dimensions so far, from the last
     for (int64_t i = d - 2; i >= 0; i--) {

@@ -375,3 +375,16 @@ def test_the_largest_K(M):
     codes, scales = rs.lm_head_quantize(make(270, 65536, "bf16", 1, 0.01))
     h = make(M, 65536, "bf16", 2)
     check(h, codes, scales, rs.lm_head_logits(h, codes, scales))
+
+
+@pytest.mark.parametrize("shape", [(0,), (0, 4), (2, 0), (3, 2, 0), (3, 0, 2), (0, 0)])
+def test_no_hidden_states(shape):
+    """An empty result, whichever dimension is empty, into `out` as well."""
+    import rapid_sampling_b200 as rs
+    codes, scales = rs.lm_head_quantize(make(300, 256, "bf16", 1, 0.02))
+    hidden = torch.empty(shape + (256,), device="cuda")
+    assert rs.lm_head_logits(hidden, codes, scales).shape == shape + (300,)
+    out = torch.empty(shape + (300,), device="cuda", dtype=torch.float16)
+    assert rs.lm_head_logits(hidden, codes, scales, out=out) is out or out.shape == shape + (300,)
+    with pytest.raises(ValueError):
+        rs.lm_head_logits(hidden[..., :128], codes, scales)
