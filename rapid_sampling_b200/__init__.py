@@ -69,7 +69,8 @@ def batch_sampling_rows(logits, states, temperature=None, top_k=None, top_p=None
 
 def batch_token_logprobs(logits, tokens, temperature=1.0):
     """Log probability of one given token per row, and the row's entropy, under softmax(logits / temperature): float32
-    tensors of the tokens' shape.  Differentiable with respect to the logits (both results, first order).
+    tensors of the tokens' shape.  Differentiable with respect to the logits (both results, first order, in reverse mode:
+    second derivatives and forward-mode tangents are refused).
 
     logits: float32, float16 or bfloat16, (V,), (B, V) or (B, T, V), every position a row; any strides but along V, and any
     V up to 1048576.  tokens: int32 or int64, the logits' shape without V.  temperature: a number, or a float32 CUDA tensor

@@ -393,6 +393,10 @@ static pybind11::tuple token_logprobs(const at::Tensor& logits, const at::Tensor
                                       const c10::optional<at::Tensor>& row_temperature) {
     if (row_temperature.has_value() && row_temperature->requires_grad())
         throw std::invalid_argument("the temperature is not differentiated: it must not require a gradient !\n");
+    // a result without a tangent would count as a constant
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+        (logits._fw_grad(0).defined() || (row_temperature.has_value() && row_temperature->_fw_grad(0).defined())))
+        throw std::invalid_argument("batch_token_logprobs is differentiable in reverse mode only: no forward-mode tangents !\n");
     if (logits.requires_grad() && at::GradMode::is_enabled()) {
         const auto r = TokenLogprobs::apply(logits, tokens, temperature, RowTemperature{row_temperature});
         return pybind11::make_tuple(r[0], r[1]);

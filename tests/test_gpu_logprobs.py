@@ -672,3 +672,22 @@ def test_an_error_of_a_sampling_call_is_reported_once():
             call()
         assert rs.device_status() == 0
         call()
+
+
+def test_forward_mode_is_refused():
+    """Tangents are not propagated: results without one would count as constants."""
+    import rapid_sampling_b200 as rs
+    import torch.autograd.forward_ad as fwd
+    x, t = make((3,), 100, "f32", 91)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        heat = fwd.make_dual(torch.ones(3, device="cuda"), torch.ones(3, device="cuda"))
+        for bad in (lambda: rs.batch_token_logprobs(dual, t), lambda: rs.batch_token_logprobs(x, t, heat)):
+            with pytest.raises((ValueError, RuntimeError)):
+                bad()
+        close(rs.batch_token_logprobs(x, t)[0], reference(x, t)["logprobs"], 100)
+        close(rs.batch_token_logprobs(fwd.unpack_dual(dual).primal, t)[0], reference(x, t)["logprobs"], 100)
+        with torch.inference_mode():                                    # tangents are off
+            close(rs.batch_token_logprobs(dual, t)[0], reference(x, t)["logprobs"], 100)
+    with pytest.raises((ValueError, RuntimeError)):
+        torch.func.jvp(lambda y: rs.batch_token_logprobs(y, t)[0], (x,), (torch.ones_like(x),))

@@ -38,3 +38,18 @@ def test_offered_by_the_package():
     assert "batch_token_logprobs" in rs.__all__ and "batch_top_logprobs" in rs.__all__
     from rapid_sampling_b200 import abi
     assert abi.status_string(abi.RS_ERR_TOKEN) == "a token id is no column of the logits"
+
+
+def test_forward_mode_is_refused():
+    import pytest
+    import torch
+    import torch.autograd.forward_ad as fwd
+    import rapid_sampling_b200 as rs
+    x, t = torch.zeros(2, 5), torch.zeros(2, dtype=torch.long)
+    with fwd.dual_level():
+        with pytest.raises(ValueError, match="tangents"):
+            rs.batch_token_logprobs(fwd.make_dual(x, torch.ones_like(x)), t)
+        with pytest.raises(ValueError, match="CUDA"):
+            rs.batch_token_logprobs(x, t)
+    with pytest.raises(ValueError, match="tangents"):
+        torch.func.jvp(lambda y: rs.batch_token_logprobs(y, t)[0], (x,), (torch.ones_like(x),))
