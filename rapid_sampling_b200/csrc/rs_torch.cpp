@@ -6,6 +6,7 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/graph_task.h>
 
 #include <map>
 #include <mutex>
@@ -340,16 +341,23 @@ static at::Tensor token_logprobs_backward(const at::Tensor& logits, const at::Te
 
 // Gradients of leaves whose accumulation belongs to the legacy default stream cannot be captured: that stream waits for
 // nothing in a capture, and the engine's attempt ends the process.  A leaf's accumulation keeps its stream as long as a graph of
-// the leaf lives, an earlier eager step's for instance.  So such a backward call is refused.
+// the leaf lives, an earlier eager step's for instance.  So such a backward call is refused, where the pass at hand reaches the
+// leaf: what lies behind the tensors that torch.autograd.grad was asked for is left alone.
 static void check_captured_backward(const at::Tensor& logits) {
     if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
+    const auto* asked = torch::autograd::get_current_graph_task_exec_info();      // empty: every node that can be reached
+    auto reached = [&](torch::autograd::Node* n) {
+        if (!asked || asked->empty()) return true;
+        const auto it = asked->find(n);
+        return it != asked->end() && it->second.should_execute();
+    };
     const auto start = logits.grad_fn() ? logits.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(logits);
     std::vector<torch::autograd::Node*> todo = {start.get()};
     std::unordered_set<torch::autograd::Node*> seen;
     while (!todo.empty()) {
         torch::autograd::Node* n = todo.back();
         todo.pop_back();
-        if (!n || !seen.insert(n).second) continue;
+        if (!n || !reached(n) || !seen.insert(n).second) continue;
         const auto s = dynamic_cast<torch::autograd::AccumulateGrad*>(n) ? n->stream() : std::nullopt;
         if (s && s->device_type() == c10::DeviceType::CUDA && *s == at::cuda::getDefaultCUDAStream(s->device_index()).unwrap())
             throw std::runtime_error("the backward pass of batch_token_logprobs cannot be captured while an eager graph of the same leaves, made on "

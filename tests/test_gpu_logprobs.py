@@ -691,3 +691,50 @@ def test_forward_mode_is_refused():
             close(rs.batch_token_logprobs(dual, t)[0], reference(x, t)["logprobs"], 100)
     with pytest.raises((ValueError, RuntimeError)):
         torch.func.jvp(lambda y: rs.batch_token_logprobs(y, t)[0], (x,), (torch.ones_like(x),))
+
+
+def test_a_captured_backward_pass_that_stops_before_such_leaves_is_not_refused():
+    """Only the leaves that the pass reaches matter: a gradient of the logits alone leaves the weight behind them alone."""
+    import subprocess
+    import sys
+    code = """
+import torch, rapid_sampling_b200 as rs
+t = torch.randint(0, 5000, (6,), device="cuda")
+h = torch.randn(6, 64, device="cuda")
+w = torch.randn(64, 5000, device="cuda", requires_grad=True)
+other = torch.randn(5000, device="cuda", requires_grad=True)
+kept = (w * 2).sum()                                          # an eager graph of the weight that stays
+def step(inputs=None):
+    logits = h @ w + other
+    lp, ent = rs.batch_token_logprobs(logits, t, 0.9)
+    return torch.autograd.grad(lp.sum() + 0.1 * ent.sum(), inputs or [logits])[0]
+want, want_other = step().clone(), step([other]).clone()
+side = torch.cuda.Stream()
+side.wait_stream(torch.cuda.current_stream())
+with torch.cuda.stream(side):
+    step()
+    step([other])
+torch.cuda.current_stream().wait_stream(side)
+torch.cuda.synchronize()
+for inputs, expect in ((None, want), ([other], want_other)):
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step(inputs)
+    got.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, expect)
+for bad in (lambda: step([w]), lambda: rs.batch_token_logprobs(h @ w, t)[0].sum().backward()):      # reach it
+    try:
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            bad()
+    except RuntimeError as e:
+        assert "alive" in str(e), e
+    else:
+        raise SystemExit("not refused")
+    torch.cuda.synchronize()
+kept.backward()
+print("fine")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout[-500:] + r.stderr[-2000:]
