@@ -39,7 +39,7 @@ def _run(cmd, verbose):
 
 
 CU_SOURCES = ["rs_sampler.cu", "rs_rowcta.cu", "rs_vocab_parallel.cu", "rs_logprobs.cu", "rs_head.cu"]
-HEADERS = [os.path.join(CSRC, h) for h in ("rs_device.cuh", "rs_common.cuh", "rs_rowcta.cuh", "rs_host.cuh")] + \
+HEADERS = [os.path.join(CSRC, h) for h in ("rs_device.cuh", "rs_common.cuh", "rs_rowcta.cuh", "rs_host.cuh", "rs_head_drain.cuh")] + \
     [os.path.join(INCLUDE, "rapid_sampling_b200.h")]
 OBJ_DIR = os.path.join(HERE, "build")
 

@@ -11,6 +11,7 @@
 // 64 tokens 127 (135 under the power cap) of 98.  Many tokens, the adding of the blocks' sums: V = 65536, 2048 tokens 523 for a
 // short while (2.10 PFLOP/s), 575 under the cap.
 #include "rs_common.cuh"
+#include "rs_head_drain.cuh"
 #include "rs_host.cuh"
 #include "../../include/rapid_sampling_b200.h"
 
@@ -334,6 +335,24 @@ struct HeadWait {
         return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || __all_sync(0xffffffffu, (*this)(bar, parity));
     }
 };
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+// After a wait that ran out, by one warp once all others have stopped: waits for the copies, products and arrivals that the steps
+// so far left on their way into this CTA.  A pair's copies count on the first CTA's barriers (`copies`: this one's), those of a step
+// that only one of the two had begun by an arrival of the other's copying warp here (drain_owed).
+__device__ __noinline__ void head_drain(uint32_t full, uint32_t empty, uint32_t sfull, uint32_t stages, uint32_t bufs, uint32_t issued,
+                                        uint32_t products, bool copies) {
+    DrainSteps d = drain_recent(products, stages);
+    for (uint32_t k = d.from; k < d.to; k++) mbar_wait_bounded(empty + 8 * drain_slot(k, stages), drain_parity(k, stages), kHeadDrainPolls);
+    d = drain_recent(products, bufs);
+    for (uint32_t k = d.from; k < d.to; k++) mbar_wait_bounded(sfull + 8 * drain_slot(k, bufs), drain_parity(k, bufs), kHeadDrainPolls);
+    d = drain_recent(issued, stages);
+    for (uint32_t k = d.from; copies && k < d.to; k++)
+        mbar_wait_bounded(full + 8 * drain_slot(k, stages), drain_parity(k, stages), kHeadDrainPolls);
+}
 // A thread's sums of one row and `cols` tokens in a slot of the workspace: four tokens of 128 rows together, so that both the
 // threads' 16 bytes and a warp's 512 are contiguous.
 template <int COLS>
@@ -423,7 +442,7 @@ __global__ void __launch_bounds__(NT * 4 + 64, 1)
     constexpr uint32_t kTmemCols = BUFS * 2 * NT;
     extern __shared__ uint8_t raw_smem[];
     __shared__ uint64_t full_[kHeadMaxStages], empty_[kHeadMaxStages], sfull_[BUFS], sempty_[BUFS];
-    __shared__ uint32_t tmem_at;
+    __shared__ uint32_t tmem_at, issued, products;
     __shared__ int gave_up, flag;
     const uint32_t base = (smem_addr(raw_smem) + 1023u) & ~1023u;
     const uint8_t* const base_p = raw_smem + (base - smem_addr(raw_smem));
@@ -471,16 +490,10 @@ __global__ void __launch_bounds__(NT * 4 + 64, 1)
                 __syncwarp();
                 if (++s == stages) { s = 0; ph ^= 1u; }
             }
-        // nothing may still be on its way into shared memory when the CTA ends: neither a copy nor, in the ordinary
-        // case, the arrival that frees a stage
-        const uint32_t n = min(it, stages);
-        for (uint32_t i = 0; i < n; i++) {
-            const uint32_t k = it - 1 - i, st = k % stages, parity = (k / stages) & 1u;
-            if (!ok || !wait.warp(empty + 8 * st, parity)) {
-                ok = false;
-                mbar_wait_bounded(full + 8 * st, parity, kHeadDrainPolls);
-            }
-        }
+        // nothing may still be on its way into shared memory when the CTA ends: neither a copy nor the arrival that frees a stage
+        const DrainSteps last = drain_recent(it, stages);
+        for (uint32_t k = last.from; ok && k < last.to; k++) ok = wait.warp(empty + 8 * drain_slot(k, stages), drain_parity(k, stages));
+        if (lane == 0) issued = it;
     } else if (w == W + 1) {
         const uint32_t idesc = head_idesc(128, p.n);
         const uint64_t desc = head_desc(base);
@@ -507,8 +520,7 @@ __global__ void __launch_bounds__(NT * 4 + 64, 1)
                 __syncwarp();
                 if (++s == stages) { s = 0; ph ^= 1u; }
             }
-        // (after a wait that ran out: the products in flight end by themselves)
-        if (!ok && it > 0) mbar_wait_bounded(sfull + 8 * ((it - 1) % BUFS), ((it - 1) / BUFS) & 1u, kHeadDrainPolls);
+        if (lane == 0) products = it;
     } else {
         const int quad = w & 3, row = quad * 32 + lane, col0 = (w >> 2) * COLS, cols = p.M - col0;
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)col0;
@@ -586,6 +598,10 @@ __global__ void __launch_bounds__(NT * 4 + 64, 1)
     __syncwarp();
     tmem_fence_before();
     __syncthreads();
+    if (gave_up) {
+        if (w == W) head_drain(full, empty, sfull, stages, BUFS, issued, products, true);
+        __syncthreads();
+    }
     tmem_fence_after();
     if (w == W + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
@@ -760,8 +776,8 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
     const uint32_t stage_bytes = (uint32_t)head_more_stage(PAIR, p.n);
     extern __shared__ uint8_t raw_smem[];
     __shared__ uint64_t full_[kHeadMaxStages], empty_[kHeadMaxStages], sfull_[2], sempty_[2];
-    __shared__ uint32_t tmem_at;
-    __shared__ int gave_up, flag;
+    __shared__ uint32_t tmem_at, issued, products;
+    __shared__ int gave_up, flag, other_gave_up;
     const uint32_t base = (smem_addr(raw_smem) + 1023u) & ~1023u;
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = PAIR ? (int)cluster_ctarank() : 0, worker = (int)blockIdx.x / CTAS;
@@ -776,7 +792,7 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
             mbar_init(sfull + 8 * i, 1);
             mbar_init(sempty + 8 * i, CTAS * W);      // a pair's: those of the first CTA, both CTAs' adding warps
         }
-        gave_up = 0;
+        gave_up = other_gave_up = 0;
         fence_mbar_init();
     }
     if (w == W + 1) {
@@ -824,14 +840,9 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
                 if (++s == stages) { s = 0; ph ^= 1u; }
             }
         }
-        const uint32_t n = min(it, stages);           // as in head_few_kernel; a pair's copies count on the first CTA's barriers
-        for (uint32_t i = 0; i < n; i++) {
-            const uint32_t k = it - 1 - i, st = k % stages, parity = (k / stages) & 1u;
-            if (!ok || !wait.warp(empty + 8 * st, parity)) {
-                ok = false;
-                if (rank == 0) mbar_wait_bounded(full + 8 * st, parity, kHeadDrainPolls);
-            }
-        }
+        const DrainSteps last = drain_recent(it, stages);      // as in head_few_kernel
+        for (uint32_t k = last.from; ok && k < last.to; k++) ok = wait.warp(empty + 8 * drain_slot(k, stages), drain_parity(k, stages));
+        if (lane == 0) issued = it;
     } else if (w == W + 1) {
         if (rank == 0) {
             const uint32_t idesc = head_idesc(128 * CTAS, NT);
@@ -862,7 +873,7 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
                     __syncwarp();
                     if (++s == stages) { s = 0; ph ^= 1u; }
                 }
-            if (!ok && it > 0) mbar_wait_bounded(sfull + 8 * ((it - 1) & 1u), ((it - 1) >> 1) & 1u, kHeadDrainPolls);
+            if (lane == 0) products = it;
         }
     } else {
         const int quad = w & 3, col0 = (w >> 2) * COLS, row = quad * 32 + lane;
@@ -960,8 +971,26 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
     tmem_fence_before();
     __syncthreads();
     if constexpr (PAIR) {
+        if (threadIdx.x == 0 && gave_up) st_cluster_u32(map_to_cta(smem_addr(&other_gave_up), (uint32_t)rank ^ 1u), 1u);
+        __syncwarp();
         cluster_arrive();
         cluster_wait();                               // neither CTA leaves while the other's products, copies or arrivals may reach it
+        if (gave_up || other_gave_up) {               // the same in both: and none of its own either
+            if (w == W) {
+                const uint32_t other = ld_cluster_u32(map_to_cta(smem_addr(&issued), (uint32_t)rank ^ 1u));
+                const uint32_t multiplied = ld_cluster_u32(map_to_cta(smem_addr(&products), 0)), first_full = map_to_cta(full, 0);
+                const DrainSteps owed = drain_owed(issued, other);
+                for (uint32_t k = owed.from; k < owed.to; k++)
+                    if (lane == 0) mbar_arrive_cluster(first_full + 8 * drain_slot(k, stages));
+                head_drain(full, empty, sfull, stages, 2, max(issued, other), multiplied, rank == 0);
+                __syncwarp();
+            }
+            cluster_arrive();
+            cluster_wait();
+        }
+    } else if (gave_up) {
+        if (w == W) head_drain(full, empty, sfull, stages, 2, issued, products, true);
+        __syncthreads();
     }
     tmem_fence_after();
     if (w == W + 1) {
