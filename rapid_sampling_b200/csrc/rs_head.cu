@@ -952,16 +952,23 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
                     }
                 }
             }
+            // the place once more, from what the compiler cannot keep in registers through the loop above (us for pairs, 2048 x 4096 x
+            // 65536 bf16 / 32768 f32: 524 / 288, with the places kept 529 / 290)
+            uint32_t tile = (uint32_t)walk.tile, tid;
+            asm volatile("" : "+r"(tile));
+            asm volatile("mov.u32 %0, %%tid.x;" : "=r"(tid));
+            const int here = (int)(tid >> 5), vt1 = (int)tile / p.token_tiles;
+            const int m0 = ((int)tile - vt1 * p.token_tiles) * 128 * CTAS + rank * 128 + (here & 3) * 32, v1 = vt1 * 256 + (here >> 2) * COLS;
             if (PAIR && p.boxes) {
-                if (!dead && m - lane < p.M && v0 < p.V)
-                    head_store_box<COLS, OUT>(&map_out, base + stages * stage_bytes + (uint32_t)(w * kStoreBytes), acc, lane, m - lane, v0, p.V);
-            } else if (!dead && m - lane < p.M && v0 < p.V) {
-                OUT* o = (OUT*)p.out + (long long)(m - lane) * p.ldo + v0;
-                if (p.wide_store) {
-                    if (m < p.M) head_store<COLS, OUT>(o + lane * p.ldo, acc, p.V - v0, p.wide_store);
+                if (!dead && m0 < p.M && v1 < p.V)
+                    head_store_box<COLS, OUT>(&map_out, base + stages * stage_bytes + (uint32_t)(here * kStoreBytes), acc, lane, m0, v1, p.V);
+            } else if (!dead && m0 < p.M && v1 < p.V) {
+                OUT* o = (OUT*)p.out + (long long)m0 * p.ldo + v1;
+                if (!PAIR && p.wide_store) {               // (a pair's wide stores are boxes)
+                    if (m0 + lane < p.M) head_store<COLS, OUT>(o + lane * p.ldo, acc, p.V - v1, p.wide_store);
                 } else {
-                    float* buf = reinterpret_cast<float*>(raw_smem + (base - smem_addr(raw_smem)) + p.turn_at + (uint32_t)(w * kTurnBytes));
-                    head_store_turned<COLS, OUT>(o, p.ldo, buf, acc, lane, p.M - (m - lane), p.V - v0);
+                    float* buf = reinterpret_cast<float*>(raw_smem + (base - smem_addr(raw_smem)) + p.turn_at + (uint32_t)(here * kTurnBytes));
+                    head_store_turned<COLS, OUT>(o, p.ldo, buf, acc, lane, p.M - m0, p.V - v1);
                 }
             }
         }

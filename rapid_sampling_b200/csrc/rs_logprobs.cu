@@ -75,7 +75,6 @@ template <int DT> struct Elem;
 template <> struct Elem<RS_DTYPE_F32> {
     using T = float;
     static constexpr int E = 4;
-    static constexpr uint32_t kNone = 0xFF800000u;      // a word of -inf
     static __device__ __forceinline__ void pairs(const uint4& v, uint64_t (&x)[2]) {
         x[0] = f2_pack(__uint_as_float(v.x), __uint_as_float(v.y));
         x[1] = f2_pack(__uint_as_float(v.z), __uint_as_float(v.w));
@@ -108,7 +107,6 @@ template <> struct Elem<RS_DTYPE_F32> {
 template <> struct Elem<RS_DTYPE_F16> {
     using T = __half;
     static constexpr int E = 8;
-    static constexpr uint32_t kNone = 0xFC00FC00u;
     static __device__ __forceinline__ __half2 h2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
     static __device__ __forceinline__ void pairs(const uint4& v, uint64_t (&x)[4]) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -149,7 +147,6 @@ template <> struct Elem<RS_DTYPE_F16> {
 template <> struct Elem<RS_DTYPE_BF16> {
     using T = __nv_bfloat16;
     static constexpr int E = 8;
-    static constexpr uint32_t kNone = 0xFF80FF80u;
     static __device__ __forceinline__ __nv_bfloat162 h2(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
     static __device__ __forceinline__ void pairs(const uint4& v, uint64_t (&x)[4]) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
