@@ -156,6 +156,9 @@ class VocabParallelSampler:
         from . import lm_head_logits
         if self.T != 1:
             raise ValueError("project makes one position per row, but this sampler was made for T=%d" % self.T)
+        if hidden.device != self.ws.device or (hidden.is_cuda and torch.cuda.current_device() != hidden.get_device()):
+            # the product follows its tensors, the sampler's stages the current device
+            raise ValueError("hidden must live on the sampler's device (%s), and that must be the current one" % self.ws.device)
         if tuple(codes.shape) != (self.V_local, hidden.shape[-1]) or tuple(hidden.shape[:-1]) != (self.B,):
             raise ValueError("project takes hidden states (B, K) and codes (V_local, K)")
         if out is None:

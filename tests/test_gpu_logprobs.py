@@ -581,7 +581,7 @@ def _runners_up(V, size):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("V,rows", [(4, 0), (9, 0), (1500, 0), (1500, 400), (5000, 400), (70000, 0), (70000, 400)])
+@pytest.mark.parametrize("V,rows", [(4, 0), (9, 0), (1500, 0), (1500, 400), (5000, 400), (5003, 400), (70000, 0), (70003, 0), (70003, 400)])
 def test_confident_rows_keep_the_runner_up(V, rows, dtype):
     """Rows of one token of probability nearly one and one other, which the same thread may hold: log p = -log1p(r) with
     r = exp(-gap / T), H = log1p(r) + gap/T r / (1 + r), and gradients of +-r / (1 + r).  The exponent's argument has three roundings of
@@ -589,7 +589,7 @@ def test_confident_rows_keep_the_runner_up(V, rows, dtype):
     another 2^-21 at most.  (Gaps of 16-bit types too: all values are whole.)"""
     import rapid_sampling_b200 as rs
     size = 4 if dtype == "f32" else 2
-    cases = [(gap, d, at, way) for gap in (3.0, 8.0, 17.0, 40.0) for d in (_runners_up(V, size) or [1]) for at in (0, min(8, V - 1 - d)) for way in (0, 1)]
+    cases = [(gap, d, at, way) for gap in (3.0, 8.0, 17.0, 40.0) for d in (_runners_up(V, size) or [1]) for at in (0, min(8, V - 1 - d), V - 1 - d) for way in (0, 1)]
     cases = cases * (1 + rows // len(cases))
     n = len(cases)
     x = torch.full((n, V), -math.inf, device="cuda")

@@ -96,3 +96,19 @@ def test_two_rank_vocab_parallel_driver(fast, defer):
         pen_full = pen_full * 0.5 + hit
     got = np.concatenate([res[0][2], res[1][2]], axis=1)
     assert np.allclose(got, pen_full.numpy(), rtol=1e-6, atol=0)
+
+
+def test_projecting_from_another_device_is_refused():
+    """Before anything is bound or launched."""
+    import pytest
+    from rapid_sampling_b200.vocab_parallel import VocabParallelSampler
+
+    class Nothing:
+        def __getattr__(self, name):
+            raise AssertionError(name)
+    vp = VocabParallelSampler(2, 256, 0, 1, device="cpu", compute=Nothing())
+    codes = torch.empty(256, 64, dtype=torch.float8_e4m3fn, device="meta")
+    scales, states = torch.empty(2, 1, device="meta"), torch.empty(128, dtype=torch.int8, device="meta")
+    for call in (vp.project, vp.sample_hidden):
+        with pytest.raises(ValueError, match="device"):
+            call(torch.empty(2, 64, device="meta"), codes, scales, states, 0.8, 50, 0.9)
