@@ -150,9 +150,12 @@ class VocabParallelSampler:
     def project(self, hidden, codes, scales, states, temperature, top_k, top_p, penalties=None, presence_penalty=0.0,
                 repetition_penalty=0.0, penalty_decay=0.0, out=None):
         """This rank's logits (B, V_local) from hidden states (B, K), the same on every rank, and this rank's rows of an fp8
-        lm_head (`lm_head_quantize` of its V_local weight rows).  The product is made in column slabs small enough for L2 and
-        each slab's row maxima are handed over at once, so that `sample(logits, ..., max_from_tiles=True)` with the same
-        arguments needs no pass for them.  `out`: a contiguous float32 buffer to use again."""
+        lm_head (`lm_head_quantize` of its V_local weight rows).  The rows' maxima are handed over as one tile, so that
+        `sample(logits, ..., max_from_tiles=True)` with the same arguments needs no pass for them.  `out`: a contiguous float32
+        buffer to use again."""
+        # One product and one pass for the maxima: in column slabs of 32 MB, whose maxima would come from L2, every slab's start and
+        # end and its own quantizing of the hidden states cost more (us on the GPU, K = 4096, one call / slabs: 64 rows of 151936
+        # 139 / 154, 256 233 / 278, 1024 rows of 65536 340 / 470; the product alone 127, 200, 293).
         from . import lm_head_logits
         if self.T != 1:
             raise ValueError("project makes one position per row, but this sampler was made for T=%d" % self.T)
@@ -166,11 +169,8 @@ class VocabParallelSampler:
         elif tuple(out.shape) != (self.B, self.V_local) or out.dtype != torch.float32 or not out.is_contiguous():
             raise ValueError("out must be a contiguous float32 tensor (B, V_local)")
         self.begin_tiles(out, states, temperature, top_k, top_p, penalties, presence_penalty, repetition_penalty, penalty_decay)
-        cols = max(128, (1 << 23) // self.B // 128 * 128)          # 32 MB a slab; whole blocks of the codes' scales
-        for col in range(0, self.V_local, cols):
-            tile = out[:, col:col + cols]
-            lm_head_logits(hidden, codes[col:col + cols], scales[col // 128:(col + cols) // 128], out=tile)
-            self.push_tile(tile, col)
+        lm_head_logits(hidden, codes, scales, out=out)
+        self.push_tile(out, 0)
         return out
 
     def sample_hidden(self, hidden, codes, scales, states, temperature, top_k, top_p, penalties=None, presence_penalty=0.0,

@@ -388,3 +388,20 @@ def test_no_hidden_states(shape):
     assert rs.lm_head_logits(hidden, codes, scales, out=out) is out or out.shape == shape + (300,)
     with pytest.raises(ValueError):
         rs.lm_head_logits(hidden[..., :128], codes, scales)
+
+
+def test_projecting_is_one_product():
+    """However large the result: the hidden states are quantized once and multiplied once."""
+    import rapid_sampling_b200 as rs
+    from rapid_sampling_b200.vocab_parallel import VocabParallelSampler
+    B, V, K = 1100, 32768, 128
+    codes, scales = rs.lm_head_quantize(make(V, K, "bf16", 1, 0.2))
+    hidden = make(B, K, "bf16", 2)
+    vp, states = VocabParallelSampler(B, V, 0, 1), rs.setup_rand(5, B)
+    before = rs.kernel_launch_count()
+    logits = vp.project(hidden, codes, scales, states, 0.8, 50, 0.9)
+    assert rs.kernel_launch_count() - before == 2
+    assert torch.equal(logits, rs.lm_head_logits(hidden, codes, scales))
+    other = rs.setup_rand(5, B)
+    got = vp.sample(logits, states, 0.8, 50, 0.9, max_from_tiles=True)
+    assert torch.equal(got, VocabParallelSampler(B, V, 0, 1).sample(logits, other, 0.8, 50, 0.9)) and torch.equal(states, other)
