@@ -5,7 +5,6 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/graph_task.h>
 
 #include <map>
@@ -339,10 +338,10 @@ static at::Tensor token_logprobs_backward(const at::Tensor& logits, const at::Te
     return grad;
 }
 
-// Gradients of leaves whose accumulation belongs to the legacy default stream cannot be captured: that stream waits for
-// nothing in a capture, and the engine's attempt ends the process.  A leaf's accumulation keeps its stream as long as a graph of
-// the leaf lives, an earlier eager step's for instance.  So such a backward call is refused, where the pass at hand reaches the
-// leaf: what lies behind the tensors that torch.autograd.grad was asked for is left alone.
+// Gradients for nodes that belong to the legacy default stream cannot be captured: that stream waits for nothing in a capture, and
+// the engine's attempt spoils the capture or ends the process.  Such are the nodes of an eager forward pass, and the accumulation
+// of a leaf as long as an eager graph of it lives, an earlier step's for instance.  So such a backward call is refused, where the
+// pass at hand hands such a node a gradient: what lies behind the tensors that torch.autograd.grad was asked for is left alone.
 static void check_captured_backward(const at::Tensor& logits) {
     if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
     const auto* asked = torch::autograd::get_current_graph_task_exec_info();      // empty: every node that can be reached
@@ -358,10 +357,10 @@ static void check_captured_backward(const at::Tensor& logits) {
         torch::autograd::Node* n = todo.back();
         todo.pop_back();
         if (!n || !reached(n) || !seen.insert(n).second) continue;
-        const auto s = dynamic_cast<torch::autograd::AccumulateGrad*>(n) ? n->stream() : std::nullopt;
+        const auto s = n->stream();
         if (s && s->device_type() == c10::DeviceType::CUDA && *s == at::cuda::getDefaultCUDAStream(s->device_index()).unwrap())
-            throw std::runtime_error("the backward pass of batch_token_logprobs cannot be captured while an eager graph of the same leaves, made on "
-                                     "the default stream, is alive !\n");
+            throw std::runtime_error("the backward pass of batch_token_logprobs cannot be captured: it leads into an eager graph, made on the default "
+                                     "stream, or to leaves of which such a graph is alive !\n");
         for (const auto& e : n->next_edges()) todo.push_back(e.function.get());
     }
 }

@@ -738,3 +738,37 @@ print("fine")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
     assert r.returncode == 0 and "fine" in r.stdout, r.stdout[-500:] + r.stderr[-2000:]
+
+
+def test_a_captured_backward_pass_into_an_eager_forward_pass_is_refused():
+    """Before the engine spoils the capture: torch's generators stay usable."""
+    import subprocess
+    import sys
+    code = """
+import torch, rapid_sampling_b200 as rs
+t = torch.randint(0, 5000, (6,), device="cuda")
+h = torch.randn(6, 64, device="cuda")
+w = torch.randn(64, 5000, device="cuda", requires_grad=True)
+logits = h @ w                                                # eager, on the default stream
+for bad in (lambda x: torch.autograd.grad(rs.batch_token_logprobs(x, t)[0].sum(), x), lambda x: rs.batch_token_logprobs(x, t)[0].sum().backward()):
+    try:
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            bad(logits)
+    except RuntimeError as e:
+        assert "eager graph" in str(e), e
+    else:
+        raise SystemExit("not refused")
+    torch.cuda.synchronize()
+    torch.randn(3, device="cuda")
+x = logits.detach().requires_grad_(True)                      # the way to do it
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got, = torch.autograd.grad(rs.batch_token_logprobs(x, t)[0].sum(), x)
+g.replay()
+torch.cuda.synchronize()
+want, = torch.autograd.grad(rs.batch_token_logprobs(logits, t)[0].sum(), logits)
+assert torch.equal(got, want)
+print("fine")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout[-500:] + r.stderr[-2000:]
