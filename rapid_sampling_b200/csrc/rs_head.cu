@@ -7,9 +7,11 @@
 // and is added in fp32 registers.  Products of e4m3 values are exact, a block's 128 of them are summed in the tensor core's fp32
 // (measured against 64 bits: 1e-7 relative for K = 4096, where a plain fp32 product is 1e-6 off).
 //
-// What bounds it (B200, K = 4096, us): few tokens, the weights' bytes: V = 151936, 1 token 103 of 95 at the measured copy rate,
-// 64 tokens 127 (135 under the power cap) of 98.  Many tokens, the adding of the blocks' sums: V = 65536, 2048 tokens 523 for a
-// short while (2.10 PFLOP/s), 575 under the cap.
+// What bounds it (B200, K = 4096, us): few tokens, the weights' bytes: V = 151936, 1 token 103 to 107 of 95 at the measured copy
+// rate, 64 tokens 126 of 101 (133 to 149 in a loop of seconds, under the power cap).  Many tokens, the adding of the blocks' sums:
+// V = 65536, 2048 tokens 515 to 523 for a short while (2.1 PFLOP/s), 575 to 615 under the cap, by the GPU.
+//
+// The product of a block's two scales is one fp32 number: where it is subnormal (scales of 2^-63 both, say) results lose digits.
 #include "rs_common.cuh"
 #include "rs_head_drain.cuh"
 #include "rs_host.cuh"
@@ -612,7 +614,7 @@ __global__ void __launch_bounds__(NT * 4 + 64, 1)
 // and the time is that of the weights' bytes.  Beyond, a pair of CTAs shares a tile of 256 tokens by 256 weight rows (but see
 // head_by_pairs): each CTA brings 128 tokens and 128 weight rows, its accumulator holds its 128 tokens by all 256 weight rows,
 // and one thread of the first CTA issues the products of both; the pair reads 64 KB for a unit where two CTAs of their own
-// read 96 KB.  What bounds it is the adding: 2048 tokens, K = 4096, V = 65536 take 523 us, and in copies of the kernel 402 without
+// read 96 KB.  What bounds it is the adding: 2048 tokens, K = 4096, V = 65536 take 515 to 523 us, and in copies of the kernel 402 without
 // the adding, 371 without scales and stores too; with the reading of the accumulators but not the additions 443, the other way
 // round 449: the sums leave too few registers to keep both going at once.
 constexpr int kMoreAdders = 8, kMoreThreads = kMoreAdders * 32 + 64;      // warps that add, threads of a CTA
