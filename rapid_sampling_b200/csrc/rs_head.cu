@@ -727,7 +727,8 @@ __device__ __forceinline__ void head_store_turned(OUT* o, long long ldo, float* 
 }
 
 // The same by way of shared memory, 8 KB a warp, for the warp's 32 rows: two boxes of 128 bytes by 32 rows at a time, which the
-// copy engine stores (and cuts off behind the last row and column) while the warp goes on with the next tile.  All CTAs end
+// copy engine stores (and cuts off behind the last row and the last whole 16 bytes of a row: it writes no less, so that the few
+// columns behind, from `whole` on, are stored one by one) while the warp goes on with the next tile.  All CTAs end
 // their tiles at about the same time: stores by the threads themselves waited 3.6 us a tile for one another (16 % of the time at
 // 2048 tokens).  128-byte swizzle: the 16-byte column c of row r lies at c ^ (r % 8).
 constexpr int kStoreBytes = 8192;
@@ -735,8 +736,10 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sr
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
 }
 template <int COLS, typename OUT>
-__device__ __forceinline__ void head_store_box(const CUtensorMap* map, uint32_t buf, const uint64_t (&acc)[COLS / 2], int lane, int m, int v0, int V) {
-    constexpr int PER = 128 / (int)sizeof(OUT);       // columns of a box
+__device__ __forceinline__ void head_store_box(const CUtensorMap* map, uint32_t buf, const uint64_t (&acc)[COLS / 2], int lane, int m, int v0,
+                                               const HeadParams& p) {
+    constexpr int PER16 = 16 / (int)sizeof(OUT);
+    const int whole = p.V / PER16 * PER16;    constexpr int PER = 128 / (int)sizeof(OUT);       // columns of a box
 #pragma unroll
     for (int c0 = 0; c0 < COLS; c0 += 2 * PER) {
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the boxes before have been read
@@ -759,11 +762,27 @@ __device__ __forceinline__ void head_store_box(const CUtensorMap* map, uint32_t 
             const uint32_t at = buf + (uint32_t)(i / 8) * 4096u + (uint32_t)lane * 128u + (uint32_t)(((i & 7) ^ (lane & 7)) * 16);
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
         }
+        if (whole < p.V && whole >= v0 + c0 && whole < v0 + c0 + 2 * PER && m + lane < p.M) {      // what this lane has just written
+            const uint32_t i = (uint32_t)(whole - v0 - c0) / PER16;
+            const uint32_t at = buf + (i / 8u) * 4096u + (uint32_t)lane * 128u + ((i & 7u) ^ (uint32_t)(lane & 7)) * 16u;
+            OUT* o = (OUT*)p.out + (long long)(m + lane) * p.ldo + whole;
+            for (int k = 0; k < p.V - whole; k++) {
+                if constexpr (sizeof(OUT) == 4) {
+                    uint32_t x;
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at + 4u * (uint32_t)k) : "memory");
+                    *reinterpret_cast<uint32_t*>(o + k) = x;
+                } else {
+                    uint16_t x;
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(at + 2u * (uint32_t)k) : "memory");
+                    *reinterpret_cast<uint16_t*>(o + k) = x;
+                }
+            }
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
-            if (v0 + c0 < V) tma_store_2d(map, buf, v0 + c0, m);
-            if (v0 + c0 + PER < V) tma_store_2d(map, buf + 4096u, v0 + c0 + PER, m);
+            if (v0 + c0 < whole) tma_store_2d(map, buf, v0 + c0, m);
+            if (v0 + c0 + PER < whole) tma_store_2d(map, buf + 4096u, v0 + c0 + PER, m);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
     }
@@ -963,7 +982,7 @@ __global__ void __launch_bounds__(kMoreThreads, 1)
             const int m0 = ((int)tile - vt1 * p.token_tiles) * 128 * CTAS + rank * 128 + (here & 3) * 32, v1 = vt1 * 256 + (here >> 2) * COLS;
             if (PAIR && p.boxes) {
                 if (!dead && m0 < p.M && v1 < p.V)
-                    head_store_box<COLS, OUT>(&map_out, base + stages * stage_bytes + (uint32_t)(here * kStoreBytes), acc, lane, m0, v1, p.V);
+                    head_store_box<COLS, OUT>(&map_out, base + stages * stage_bytes + (uint32_t)(here * kStoreBytes), acc, lane, m0, v1, p);
             } else if (!dead && m0 < p.M && v1 < p.V) {
                 OUT* o = (OUT*)p.out + (long long)m0 * p.ldo + v1;
                 if (!PAIR && p.wide_store) {               // (a pair's wide stores are boxes)
@@ -1262,6 +1281,8 @@ int rs_head_logits(const void* hidden, int32_t hidden_dtype, int64_t M, int64_t 
     const int per = few ? head_few_stage(p.n) : head_more_stage(pair, p.n);
     const uintptr_t step = (uintptr_t)out_device | (uintptr_t)out_stride * os;
     p.wide_store = step % 32 == 0 ? 32 : step % 16 == 0 ? 16 : 0;
+    const long long whole = V / (long long)(16 / os) * (long long)(16 / os);      // columns of a row that boxes store
+    if (pair && whole == 0) p.wide_store = 0;
     p.boxes = pair && p.wide_store;
     // behind the stages: the boxes to store, or what the products read beyond the last stage and the rows to turn
     const int tail = few ? 0 : p.boxes ? kMoreAdders * kStoreBytes : head_more_tail(pair, p.n) + (p.wide_store ? 0 : kMoreAdders * kTurnBytes);
@@ -1276,7 +1297,7 @@ int rs_head_logits(const void* hidden, int32_t hidden_dtype, int64_t M, int64_t 
         const CUtensorMapDataType type = out_dtype == RS_DTYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                          : out_dtype == RS_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-        if ((rc = head_map(&out, type, (int)os, out_device, M, V, (long long)(out_stride * (int64_t)os), 32))) return rc;
+        if ((rc = head_map(&out, type, (int)os, out_device, M, whole, (long long)(out_stride * (int64_t)os), 32))) return rc;
     }
     if ((rc = head_quantize<true>(hidden, hidden_dtype, hidden_stride, M, K, ws, sa, p.pitch, p.arrived, (cudaStream_t)stream))) return rc;
     p.turn_at = p.stages * per + (few ? 0 : head_more_tail(pair, p.n));

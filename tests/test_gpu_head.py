@@ -405,3 +405,23 @@ def test_projecting_is_one_product():
     other = rs.setup_rand(5, B)
     got = vp.sample(logits, states, 0.8, 50, 0.9, max_from_tiles=True)
     assert torch.equal(got, VocabParallelSampler(B, V, 0, 1).sample(logits, other, 0.8, 50, 0.9)) and torch.equal(states, other)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("M", [129, 300, 700])
+def test_columns_behind_the_result_stay_as_they_are(M, dtype):
+    """Rows at multiples of 16 and 32 bytes whose result ends anywhere within 16: what lies behind it in the same buffer is not
+    written, nor what lies behind the last row."""
+    import rapid_sampling_b200 as rs
+    K, per = 128, 16 // (4 if dtype == "f32" else 2)
+    hidden = make(M, K, "bf16", 2)
+    codes, scales = rs.lm_head_quantize(make(1100, K, "bf16", 1, 0.02))
+    for V in list(range(1, 2 * per + 2)) + [127, 129, 255, 257, 258, 259, 500, 639, 1001, 1002, 1003, 1005, 1007, 1023]:
+        got = rs.lm_head_logits(hidden, codes[:V], scales[:-(-V // 128)])
+        check(hidden, codes[:V], scales[:-(-V // 128)], got)
+        for first in (0, per):
+            for wide in (-(-(first + V) // per) * per, -(-(first + V) // (2 * per)) * 2 * per + 2 * per):
+                buf = torch.full((M + 1, wide), 7.0, device="cuda", dtype=DT[dtype])
+                rs.lm_head_logits(hidden, codes[:V], scales[:-(-V // 128)], out=buf[:M, first:first + V])
+                assert torch.equal(buf[:M, first:first + V], got.to(DT[dtype])), (V, first, wide)
+                assert bool((buf[:M, :first] == 7).all()) and bool((buf[:M, first + V:] == 7).all()) and bool((buf[M] == 7).all()), (V, first, wide)
