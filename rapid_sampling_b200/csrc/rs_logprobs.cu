@@ -7,9 +7,8 @@
 // A row is read once: every thread keeps the maximum it has seen, and the two sums relative to it.  Maxima are compared on
 // the logits as they are; exponents are taken as ((x - m) log2(e)/T) so that neither masks of the type's lowest value nor a
 // row made of nothing else overflow.  log p of a token of probability nearly one is -log1p(excess), the excess being s without
-// the maximum's own 1.  Sums are held so from the thread level up, all but the one of the thread that has the maximum apart from
-// that thread's, whose additions to the 1 lose what lies below 2^-24; where the excess is small its elements are read again
-// (lp_rest).
+// the maximum's own 1.  What the other threads hold is added up apart from that 1.  The maximum's own thread adds to it and loses
+// what lies below 2^-24 there; where the excess is small, its elements are read again and added by themselves (lp_rest).
 #include "rs_device.cuh"
 #include "rs_host.cuh"
 #include "../../include/rapid_sampling_b200.h"
